@@ -4,6 +4,7 @@
 """
 from __future__ import annotations
 
+import concurrent.futures
 import os
 import subprocess
 import sys
@@ -30,6 +31,8 @@ def hipcc_version() -> str:
     return f"{hip} clang-{clang}"
 
 
+SOURCES = ("flame_attn.hip", "flame_packed.hip", "flame_paged.hip")      # of the attention library
+
 STATIC_LIB_PATH = os.path.join(LIB_DIR, "libflame_attn_hip.a")
 
 
@@ -45,19 +48,23 @@ def _run(cmd, verbose):
 
 
 def build_lib(verbose: bool = False, extra=()) -> str:
-    """One compilation of flame_attn.hip to an object, from which both the shared library (what the tests, the
+    """One compilation of each source to an object, from which both the shared library (what the tests, the
     benchmark and the ctypes binding load) and the static archive (what a Rust build script links, as the reference's
     build.rs links its own kernels) are made."""
     os.makedirs(LIB_DIR, exist_ok=True)
-    src = os.path.join(CSRC, "flame_attn.hip")
-    obj = os.path.join(LIB_DIR, "flame_attn.o")
     compile_flags = [f for f in FLAGS if f != "-shared"]
-    _run([HIPCC, *compile_flags, f'-DFLAME_ATTN_HIPCC_VERSION="{hipcc_version()}"', *extra, "-c", src, "-o", obj], verbose)
-    _run([HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", obj, "-o", LIB_PATH], verbose)
+    version = f'-DFLAME_ATTN_HIPCC_VERSION="{hipcc_version()}"'
+    objects = [os.path.join(LIB_DIR, os.path.splitext(name)[0] + ".o") for name in SOURCES]
+    with concurrent.futures.ThreadPoolExecutor(len(SOURCES)) as pool:
+        for job in [pool.submit(_run, [HIPCC, *compile_flags, version, *extra, "-c", os.path.join(CSRC, name), "-o", obj], verbose)
+                    for name, obj in zip(SOURCES, objects)]:
+            job.result()
+    _run([HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", *objects, "-o", LIB_PATH], verbose)
     if os.path.exists(STATIC_LIB_PATH):
         os.remove(STATIC_LIB_PATH)
-    _run(["ar", "rcs", STATIC_LIB_PATH, obj], verbose)
-    os.remove(obj)
+    _run(["ar", "rcs", STATIC_LIB_PATH, *objects], verbose)
+    for obj in objects:
+        os.remove(obj)
     return LIB_PATH
 
 

@@ -153,6 +153,68 @@ def cudnn_sdpa_bwd(q, k, v, o, do, stats, scale, grads=None):
     return dq, dk, dv
 
 
+# ---------------------------------------------------------------- packed sequences
+def packed_fwd_workspace_bytes(n_seqs, T_q, T_kv, H, D) -> int:
+    """Bytes with which flame_attn_packed_fwd_bf16 cuts the walks of a problem that leaves compute units idle into parts
+    (0 where it would not)."""
+    f = lib().flame_attn_packed_fwd_workspace_bytes
+    f.restype = ctypes.c_size_t
+    return int(f(n_seqs, T_q, T_kv, H, D))
+
+
+def attn_packed_fwd(q, k, v, cu_q, cu_k, scale, causal=True, want_lse=True, out=None, lse_out=None, workspace=None):
+    """O, LSE = flame_attn_packed_fwd_bf16(...): sequences of different lengths one behind the other.
+
+    q [T_q, H, D], k/v [T_kv, H_kv, D] bf16, D stride 1; cu_q, cu_k: int32 [sequences + 1] on the device, the bounds of
+    the sequences' rows.  causal: query i attends to key j <= i + (keys - queries) of its sequence.  Returns o [T_q, H, D]
+    and lse fp32 [H, T_q] (None without want_lse); rows behind the last sequence are 0 and -inf.  `workspace`: uint8 device
+    tensor, used where it holds packed_fwd_workspace_bytes(...) (allocated here when omitted)."""
+    return host().attn_packed_fwd(q, k, v, cu_q, cu_k, scale, causal, want_lse, out, lse_out, workspace)
+
+
+def packed_bwd_workspace_bytes(n_seqs, T_q, T_kv, H, H_kv, D) -> int:
+    f = lib().flame_attn_packed_bwd_workspace_bytes
+    f.restype = ctypes.c_size_t
+    return int(f(n_seqs, T_q, T_kv, H, H_kv, D))
+
+
+def attn_packed_bwd(q, k, v, o, do, lse, cu_q, cu_k, scale, causal=True, workspace=None, grads=None):
+    """dQ, dK, dV = flame_attn_packed_bwd_bf16(...).  `workspace`: uint8 device tensor, best of
+    packed_bwd_workspace_bytes(...) bytes (allocated here when omitted), at least two fp32 values per query row and head."""
+    dq, dk, dv = grads if grads is not None else (None, None, None)
+    return host().attn_packed_bwd(q, k, v, o, do, lse, cu_q, cu_k, scale, causal, workspace, dq, dk, dv)
+
+
+# ---------------------------------------------------------------- paged cache of keys and values
+def paged_workspace_bytes(B, H, H_kv, N, D, page, table_pages, prefix_pages=0) -> int:
+    f = lib().flame_attn_paged_workspace_bytes
+    f.restype = ctypes.c_size_t
+    return int(f(B, H, H_kv, N, D, page, table_pages, prefix_pages))
+
+
+def attn_paged_fwd(q, k_cache, v_cache, page_table, kv_len, scale, prefix_table=None, prefix_len=None, want_lse=False, out=None,
+                   workspace=None):
+    """O, LSE = flame_attn_paged_fwd_bf16(...): the last N tokens of every sequence against a paged cache.
+
+    q [B, H, N, D]; caches bf16 [pages, H_kv, page, D]; page_table int32 [B, pages of a sequence], kv_len int32 [B]: a
+    sequence's own keys, the N new ones among them; prefix_table int32 [pages] and prefix_len int32 [1]: keys that all
+    sequences share in front of their own.  `workspace`: uint8 device tensor of at least paged_workspace_bytes(...) bytes
+    (allocated here when omitted; 0: none is needed).  lse fp32 [B * H, N] or None.  Inference only."""
+    return host().attn_paged_fwd(q, k_cache, v_cache, page_table, kv_len, scale, prefix_table, prefix_len, want_lse, out, workspace)
+
+
+def kv_store(k, v, k_cache, v_cache, page_table, cu, start):
+    """flame_kv_store_bf16(...): rows k, v [rows, H_kv, D] of the sequences that cu (int32 [sequences + 1]) bounds to the
+    places start[b], start[b] + 1, ... (int32 [sequences]) of their pages."""
+    host().kv_store(k, v, k_cache, v_cache, page_table, cu, start)
+
+
+def kv_copy_pages(k_cache, v_cache, src, dst):
+    """flame_kv_copy_pages_bf16(...): page src[i] to page dst[i] (sequences of ints) in both caches, [pages, H_kv, page, D]
+    or [layers, pages, H_kv, page, D], in all layers.  A page that is written twice, or read and written, is refused."""
+    host().kv_copy_pages(k_cache, v_cache, src, dst)
+
+
 KERNEL_KINDS = ("fwd", "unused1", "bwd_dkdv", "bwd_dq", "sage_kmean", "sage_quant", "sage_fwd", "input_prep",
                 "bwd_merge", "bwd_joint", "bwd_rows", "reserved11")
 

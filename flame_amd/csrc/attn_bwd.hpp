@@ -27,6 +27,7 @@
 #include <type_traits>
 
 #include "attn_common.hpp"
+#include "packed_units.hpp"
 
 namespace fattn {
 
@@ -86,7 +87,7 @@ struct BwdTile {
 
 template <int D>
 __device__ __forceinline__ void dkdv_store(const BwdParams& p, uint16_t* own, const f32x16 (&dkacc)[D / 32], const f32x16 (&dvacc)[D / 32],
-                                           int b, int hh, int kw0, float dv_scale = 1.0f);
+                                           uint16_t* dkbase, uint16_t* dvbase, int Sk, int kw0, float dv_scale = 1.0f);
 
 // VECMASK (with HASMASK): the keep-mask rows are contiguous and 16-byte aligned, Sq is a multiple of 64, Sk
 // of 128, and there is no causal flag.  The 64 x 128 mask bytes of a step then travel to LDS with the step's other copies (two more
@@ -100,8 +101,12 @@ __device__ __forceinline__ void dkdv_store(const BwdParams& p, uint16_t* own, co
 // DEALT: the units come in the order of causal_order.hpp (deals_units, which the host asks).
 // block / nblocks: this workgroup's index in the dK/dV grid and the size of that grid (the kernel's own launch, or
 // the dK/dV part of bwd_joint_kernel's).
-template <int D, bool HASMASK, bool TIMING, bool VECMASK = false, int DROP = kDropNone, bool BITS = false, bool DEALT = false>
-__device__ __forceinline__ void bwd_dkdv_body(const BwdParams& p, const int block, const int nblocks) {
+// PACKED: the unit is a key block of one of several sequences of different lengths (packed_units.hpp), `u`, and the walk goes
+// through the query tiles of the u.rep heads that share the key head: the cut tiles of all heads, then the others head by head, all
+// into the same sums.
+template <int D, bool HASMASK, bool TIMING, bool VECMASK = false, int DROP = kDropNone, bool BITS = false, bool DEALT = false, bool PACKED = false>
+__device__ __forceinline__ void bwd_dkdv_body(const BwdParams& p, const int block, const int nblocks, const PackedUnit& u = PackedUnit()) {
+    static_assert(!PACKED || (!HASMASK && !BITS && !DEALT && !TIMING && DROP == kDropNone), "packed sequences: causal flag and lengths only");
     static_assert(!VECMASK || HASMASK, "VECMASK is a special case of HASMASK");
     static_assert(!BITS || (!HASMASK && DROP == kDropNone), "bits stand for the mask");
     constexpr bool DROPOUT = DROP != kDropNone;
@@ -122,9 +127,14 @@ __device__ __forceinline__ void bwd_dkdv_body(const BwdParams& p, const int bloc
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 31, h = lane >> 5;
 
-    const int n_kt = (p.Sk + BN - 1) / BN;
-    int wg, part = 0, nparts = 1;
-    if (p.n_whole < 0) {
+    const int Sq = PACKED ? u.Sq : p.Sq, Sk = PACKED ? u.Sk : p.Sk;
+    const int past = PACKED ? u.past : 0;             // under the causal flag query i attends to key j <= i + past
+    const int n_kt = (Sk + BN - 1) / BN;
+    int wg = 0, part = 0, nparts = 1;
+    if constexpr (PACKED) {
+        wg = u.unit;
+        part = u.part;
+    } else if (p.n_whole < 0) {
         wg = xcd_remap_heads(block, nblocks, n_kt, p.m.kv_len || p.key_mask, false);
     } else if (block < p.n_whole) {
         wg = xcd_remap(block, p.n_whole);
@@ -134,7 +144,7 @@ __device__ __forceinline__ void bwd_dkdv_body(const BwdParams& p, const int bloc
         wg = p.n_whole + e / nparts;
         part = e % nparts;
     }
-    int kt = wg % n_kt, bh = wg / n_kt;
+    int kt = PACKED ? u.tile : wg % n_kt, bh = PACKED ? 0 : wg / n_kt;
     if constexpr (DEALT) {       // under the causal flag the first key blocks have the longest walks
         int t, s;
         dealt_unit(block, n_kt, p.B, p.H, p.m.kv_len || p.key_mask, t, s);
@@ -145,22 +155,28 @@ __device__ __forceinline__ void bwd_dkdv_body(const BwdParams& p, const int bloc
     const int k0 = kt * BN;
     const int kw0 = k0 + 32 * wave;
 
-    const uint16_t* qbase = p.q + b * p.qs.b + hh * p.qs.h;
-    const uint16_t* kbase = p.k + b * p.ks.b + hh * p.ks.h;
-    const uint16_t* vbase = p.v + b * p.vs.b + hh * p.vs.h;
-    const uint16_t* dobase = p.dout + b * p.dos.b + hh * p.dos.h;
-    const float* lsebase = p.lse2 + (int64_t)bh * p.Sq;
-    const float* ndeltabase = p.ndelta + (int64_t)bh * p.Sq;
+    // PACKED: of the first head that shares this key head
+    const uint16_t* qbase = PACKED ? p.q + u.q_at(p.qs) : p.q + b * p.qs.b + hh * p.qs.h;
+    const uint16_t* kbase = PACKED ? p.k + u.k_at(p.ks) : p.k + b * p.ks.b + hh * p.ks.h;
+    const uint16_t* vbase = PACKED ? p.v + u.k_at(p.vs) : p.v + b * p.vs.b + hh * p.vs.h;
+    const uint16_t* dobase = PACKED ? p.dout + u.q_at(p.dos) : p.dout + b * p.dos.b + hh * p.dos.h;
+    const float* lsebase = p.lse2 + (PACKED ? u.stat_row() : (int64_t)bh * p.Sq);
+    const float* ndeltabase = p.ndelta + (PACKED ? u.stat_row() : (int64_t)bh * p.Sq);
+    auto store_rows = [&](const f32x16 (&dkacc)[D / 32], const f32x16 (&dvacc)[D / 32], float dv_scale) {
+        uint16_t* const dkbase = PACKED ? p.dk + u.k_at(p.dks) : p.dk + b * p.dks.b + hh * p.dks.h;
+        uint16_t* const dvbase = PACKED ? p.dv + u.k_at(p.dvs) : p.dv + b * p.dvs.b + hh * p.dvs.h;
+        dkdv_store<D>(p, lds + wave * 32 * RS, dkacc, dvacc, dkbase, dvbase, Sk, kw0, dv_scale);
+    };
 
-    int klimit = p.Sk;
-    if (p.m.kv_len) klimit = min(klimit, max(p.m.kv_len[b], 0));
+    int klimit = Sk;
+    if (!PACKED && p.m.kv_len) klimit = min(klimit, max(p.m.kv_len[b], 0));
     const uint8_t* mbase = HASMASK ? mask_head_base(p.m, b, hh) : nullptr;
 
     // A keep-mask of keys is a key length with holes: a lane owns one key, so its P and dS need no test, and the columns of
     // the excluded keys are zeroed before the store.  Two loads per wavefront tell whether any of the 128 keys is attended.
     bool dead = false;
     uint64_t any_alive = ~0ull;
-    if (!HASMASK && p.key_mask) {
+    if (!HASMASK && !PACKED && p.key_mask) {
         const uint8_t* kmask = mask_head_base(p.m, b, hh);
         bool alive[2];
 #pragma unroll
@@ -172,8 +188,8 @@ __device__ __forceinline__ void bwd_dkdv_body(const BwdParams& p, const int bloc
         any_alive = b0 | b1;
         dead = ((((wave & 2) ? b1 : b0) >> (32 * (wave & 1) + n)) & 1ull) == 0;
     }
-    const int n_qt = (p.Sq + BM - 1) / BM;
-    int qt_begin = p.m.causal && !BITS ? (k0 / BM) : 0;
+    const int n_qt = (Sq + BM - 1) / BM;
+    int qt_begin = p.m.causal && !BITS ? (PACKED ? max(k0 - past, 0) : k0) / BM : 0;
     KeyTiles qtiles;                       // BITS: of queries
     const uint64_t* bcols = nullptr;       // this lane's key's word of query tile 0; tiles lie 64 bit_nkt words apart
     if constexpr (BITS) {
@@ -186,7 +202,7 @@ __device__ __forceinline__ void bwd_dkdv_body(const BwdParams& p, const int bloc
         bcols = p.m.bit_cols + (int64_t)plane * p.m.bit_nqt * (64 * p.m.bit_nkt) + kw0 + n;
         if (qtiles.n_tiles == 0) any_alive = 0;
     }
-    if (k0 >= klimit || any_alive == 0 || (!BITS && p.m.causal && k0 >= p.Sq)) {
+    if (k0 >= klimit || any_alive == 0 || (PACKED ? qt_begin >= n_qt : !BITS && p.m.causal && k0 >= p.Sq)) {
         // Nothing attends to these keys (past the key length, masked, or past the last query under the causal flag):
         // dK = dV = 0, written at once.  Padded batches launch many such workgroups; they must not cost a
         // prologue each.
@@ -195,10 +211,15 @@ __device__ __forceinline__ void bwd_dkdv_body(const BwdParams& p, const int bloc
         for (int db = 0; db < D / 32; ++db)
 #pragma unroll
             for (int r = 0; r < 16; ++r) zero[db][r] = 0.f;
-        dkdv_store<D>(p, lds + wave * 32 * RS, zero, zero, b, hh, kw0);
+        if (!PACKED || part == 0) store_rows(zero, zero, 1.0f);
         return;
     }
-    const int n_it = BITS ? qtiles.n_tiles : n_qt - qt_begin;
+    const int rep = PACKED ? u.rep : 1;
+    const int n_it_head = BITS ? qtiles.n_tiles : n_qt - qt_begin, n_it = rep * n_it_head;
+    if constexpr (PACKED) {
+        nparts = packed_parts(u, n_it);
+        if (part >= nparts) return;
+    }
     // The walk visits the query tiles that need per-element exclusions first (all of them when an explicit
     // mask is given, else the causal diagonal tiles and a partial last tile) and the fully attended ones afterwards, so that each of the two loops runs one
     // specialised, branch-free body.  The order of the tiles does not matter to the sums.
@@ -209,16 +230,28 @@ __device__ __forceinline__ void bwd_dkdv_body(const BwdParams& p, const int bloc
     if (n_it > 0) {
         if (BITS) lead_end = n_it - qtiles.n_whole;
         else if (all_masked) lead_end = n_qt;
+        else if (PACKED && p.m.causal) lead_end = max(qt_begin, min(n_qt, (max(k0 + BN - 1 - past, 0) + BM - 1) / BM));
         else if (p.m.causal) lead_end = max(qt_begin, min(n_qt, (k0 + BN - 2) / BM + 1));
     }
     const int n_lead = lead_end - qt_begin;
-    const int tail_extra = (n_it > 0 && !BITS && !all_masked && (p.Sq % BM) != 0 && lead_end < n_qt) ? 1 : 0;
-    const int n_masked = n_lead + tail_extra;
+    const int tail_extra = (n_it > 0 && !BITS && !all_masked && (Sq % BM) != 0 && lead_end < n_qt) ? 1 : 0;
+    const int n_masked_head = n_lead + tail_extra, n_masked = rep * n_masked_head;
+    const int n_full_head = PACKED ? max(n_it_head - n_masked_head, 1) : 1;       // (divisors)
+    const int n_cut_head = PACKED ? max(n_masked_head, 1) : 1;
     auto tile_of = [&](int it) {
+        if constexpr (PACKED) {
+            const int j = packed_uniform(it < n_masked ? it % n_cut_head : (it - n_masked) % n_full_head);
+            const int full = lead_end + j, cut = qt_begin + j, last = n_qt - 1, lead = n_lead;       // (values: the compiler would choose among addresses)
+            return it >= n_masked ? full : j < lead ? cut : last;
+        }
         if constexpr (BITS) return qtiles.tile(it < n_masked ? qtiles.n_whole + it : it - n_masked);
         if (it < n_lead) return qt_begin + it;
         if (it < n_masked) return n_qt - 1;
         return lead_end + (it - n_masked);
+    };
+    auto head_of = [&](int it) {           // PACKED: of step `it`, counted from u.head
+        if constexpr (PACKED) return packed_uniform(it < n_masked ? it / n_cut_head : (it - n_masked) / n_full_head);
+        else return 0;
     };
     // ---- per-lane LDS offsets (elements), constant over the walk
     int roff[DC];          // 16-byte row reads: row (32*blk + n), logical granule 2*dc + h
@@ -304,17 +337,21 @@ __device__ __forceinline__ void bwd_dkdv_body(const BwdParams& p, const int bloc
         return lds0 + (uint32_t)(T::LDS_BYTES + stg * T::MASK_STAGE_BYTES + (wave * 2 + jm) * 1024);
     };
     auto mask_tile = [&](int qt) { return mbase + (int64_t)qt * BM * p.m.sq + k0; };
-    auto issue_q_tile = [&](int qt, int stg) {
+    auto issue_q_tile = [&](int qt, int head, int stg) {
         const int q0 = qt * BM;
-        if (q0 + BM <= p.Sq) {
-            const uint16_t* qt_base = qbase + (int64_t)q0 * p.qs.n;
-            const uint16_t* dot_base = dobase + (int64_t)q0 * p.dos.n;
+        const uint16_t* const qhead = PACKED ? qbase + head * p.qs.h : qbase;
+        const uint16_t* const dohead = PACKED ? dobase + head * p.dos.h : dobase;
+        const float* const lsehead = PACKED ? lsebase + (int64_t)head * u.total_q : lsebase;
+        const float* const ndeltahead = PACKED ? ndeltabase + (int64_t)head * u.total_q : ndeltabase;
+        if (q0 + BM <= Sq) {
+            const uint16_t* qt_base = qhead + (int64_t)q0 * p.qs.n;
+            const uint16_t* dot_base = dohead + (int64_t)q0 * p.dos.n;
 #pragma unroll
             for (int i = 0; i < NDQ; ++i) {
                 dma16u(qt_base, q_lane_off[i], q_dst(stg, 0, i));
                 dma16u(dot_base, do_lane_off[i], q_dst(stg, 1, i));
             }
-            if (wave < 2) dma4((wave == 0 ? lsebase : ndeltabase) + q0 + lane, rows_dst(stg));
+            if (wave < 2) dma4((wave == 0 ? lsehead : ndeltahead) + q0 + lane, rows_dst(stg));
             if (VECMASK) {
 #pragma unroll
                 for (int jm = 0; jm < 2; ++jm) dma16u(mask_tile(qt), m_lane_off[jm], mask_dst(stg, jm));
@@ -324,14 +361,14 @@ __device__ __forceinline__ void bwd_dkdv_body(const BwdParams& p, const int bloc
             for (int i = 0; i < NDQ; ++i) {
                 const int ji = wave * NDQ + i;
                 const int row = ji * RPD + dma_row_in;
-                const int qi = min(q0 + row, p.Sq - 1);
+                const int qi = min(q0 + row, Sq - 1);
                 const int c = src_granule(dma_gran ^ swz<D>(row), p.d);
-                dma16(qbase + (int64_t)qi * p.qs.n + c * 8, q_dst(stg, 0, i));
-                dma16(dobase + (int64_t)qi * p.dos.n + c * 8, q_dst(stg, 1, i));
+                dma16(qhead + (int64_t)qi * p.qs.n + c * 8, q_dst(stg, 0, i));
+                dma16(dohead + (int64_t)qi * p.dos.n + c * 8, q_dst(stg, 1, i));
             }
             if (wave < 2) {
-                const int qi = min(q0 + lane, p.Sq - 1);
-                dma4((wave == 0 ? lsebase : ndeltabase) + qi, rows_dst(stg));
+                const int qi = min(q0 + lane, Sq - 1);
+                dma4((wave == 0 ? lsehead : ndeltahead) + qi, rows_dst(stg));
             }
         }
     };
@@ -417,7 +454,7 @@ __device__ __forceinline__ void bwd_dkdv_body(const BwdParams& p, const int bloc
     // (VECMASK: every step needs exclusions and the straight-line loop comes first, so it starts in stage 0)
     int st = VECMASK ? 0 : (3 - n_masked_here % 3) % 3;        // LDS stage of the step about to run
     if (it_hi > it_lo) {
-        issue_q_tile(tile_of(it_lo), st);
+        issue_q_tile(tile_of(it_lo), head_of(it_lo), st);
         wait_vm0();
         __syncthreads();
 #pragma unroll
@@ -532,7 +569,7 @@ __device__ __forceinline__ void bwd_dkdv_body(const BwdParams& p, const int bloc
                     drop = (keep_bits[qb] & (1u << (8 * g + t))) == 0;
                 } else {
                     // bitwise, not short-circuit: one select per element instead of a chain of branches
-                    drop = (key >= klimit) | (qi >= p.Sq) | ((p.m.causal != 0) & (key > qi));
+                    drop = (key >= klimit) | (qi >= Sq) | ((p.m.causal != 0) & (key > qi + past));
                     if (HASMASK) drop |= mk[qb][r] == 0;
                 }
                 pr = drop ? 0.f : pr;
@@ -578,7 +615,7 @@ __device__ __forceinline__ void bwd_dkdv_body(const BwdParams& p, const int bloc
         // in two halves around an MFMA: destination into M0, then the copy.  nq_base / ndo_base / nrow_base
         // are the wave-uniform addresses of the next tile's Q rows, dO rows and lse2 (even waves) or
         // -delta (odd waves) rows; waves 2 and 3 repeat the row copies of waves 0 and 1.
-        const bool next_full = COPY == 1 || (qt_next * BM + BM) <= p.Sq;
+        const bool next_full = COPY == 1 || (qt_next * BM + BM) <= Sq;
         const bool copying = COPY == 1 || (COPY == 2 && have_next && next_full);
         auto copy_dst_of = [&](int j) {
             return j < 2 * NDQ ? q_dst(nxt, j & 1, j >> 1) : rows_lds0 + 4u * (uint32_t)(nxt * T::ROW_FLOATS + (wave & 1) * BM);
@@ -603,7 +640,7 @@ __device__ __forceinline__ void bwd_dkdv_body(const BwdParams& p, const int bloc
                 else dma16u(nq_base, q_lane_off[j >> 1], copy_dst_of(j));
             }
         };
-        if (COPY == 2 && have_next && !next_full) issue_q_tile(qt_next, nxt);   // partial tile: slow path, all at once
+        if (COPY == 2 && have_next && !next_full) issue_q_tile(qt_next, head_of(it + 1), nxt);   // partial tile: slow path, all at once
 
         // The element-wise work of a block trails the hand-emitted MFMAs that produced its S and dP by
         // LAG MFMA slots (see mfma32_vgpr_bacc), so its last LAG slices run at the start of the phase after.
@@ -738,8 +775,9 @@ __device__ __forceinline__ void bwd_dkdv_body(const BwdParams& p, const int bloc
     }
     for (int it = it_m; it < n_masked_here + it_lo; ++it) {
         const int qn = it + 1 < it_hi ? tile_of(it + 1) : 0;
-        step(std::true_type{}, I2{}, IM{}, st, it, tile_of(it), qn, qbase + qn * q_tile_stride, dobase + qn * do_tile_stride,
-             rowbase + qn * BM);
+        const int hn = PACKED && it + 1 < it_hi ? head_of(it + 1) : 0;
+        step(std::true_type{}, I2{}, IM{}, st, it, tile_of(it), qn, qbase + qn * q_tile_stride + hn * p.qs.h, dobase + qn * do_tile_stride + hn * p.dos.h,
+             rowbase + qn * BM + (int64_t)hn * u.total_q);
         st = st == 2 ? 0 : st + 1;
     }
     // every tile after the first n_masked is a full, fully attended one, and they are consecutive;
@@ -750,6 +788,15 @@ __device__ __forceinline__ void bwd_dkdv_body(const BwdParams& p, const int bloc
         const uint16_t* nq = qbase + (qt + 1) * q_tile_stride;     // the tile after the current one
         const uint16_t* ndo = dobase + (qt + 1) * do_tile_stride;
         const float* nrow = rowbase + (qt + 1) * BM;
+        // PACKED: the tile after the current one is tile `ahead` of the full ones of its head
+        int ahead = 0;
+        if constexpr (PACKED) {
+            const int f = it + 1 - n_masked, head = packed_uniform(f / n_full_head);
+            ahead = f - head * n_full_head;
+            nq = qbase + (lead_end + ahead) * q_tile_stride + head * p.qs.h;
+            ndo = dobase + (lead_end + ahead) * do_tile_stride + head * p.dos.h;
+            nrow = rowbase + (lead_end + ahead) * BM + (int64_t)head * u.total_q;
+        }
         // BITS: the list says how many tiles to go on (from the one the pointers are at; kept as steps, not as places: pointers
         // formed anew from the bases took so many scalar registers that 560 bytes per lane went to scratch)
         int listed = it + 1, at_tile = qt + 1;
@@ -768,6 +815,14 @@ __device__ __forceinline__ void bwd_dkdv_body(const BwdParams& p, const int bloc
             if constexpr (BITS) {
                 on_by_list();
                 return;
+            }
+            if constexpr (PACKED) {
+                if (++ahead == n_full_head) {          // on to the next head
+                    ahead = 0;
+                    nq += p.qs.h - n_full_head * q_tile_stride;
+                    ndo += p.dos.h - n_full_head * do_tile_stride;
+                    nrow += u.total_q - n_full_head * BM;
+                }
             }
             nq += q_tile_stride;
             ndo += do_tile_stride;
@@ -800,7 +855,7 @@ __device__ __forceinline__ void bwd_dkdv_body(const BwdParams& p, const int bloc
     if (nparts > 1) {
         // fp32 partial sums of this slice, in accumulator order: [tensor][db][group of four][thread], so that the lanes of a
         // wavefront write, and the merge reads, 1 KiB at a time
-        float* dst = p.split_ws + ((size_t)(wg - p.n_whole) * nparts + part) * (size_t)(2 * BN * D);
+        float* dst = p.split_ws + (PACKED ? (size_t)wg : (size_t)(wg - p.n_whole) * nparts + part) * (size_t)(2 * BN * D);
 #pragma unroll
         for (int db = 0; db < DB; ++db)
 #pragma unroll
@@ -823,7 +878,7 @@ __device__ __forceinline__ void bwd_dkdv_body(const BwdParams& p, const int bloc
             }
     }
     __syncthreads();              // nobody reads a tile any more
-    dkdv_store<D>(p, lds + wave * 32 * RS, dkacc, dvacc, b, hh, kw0, DROP == kDropFlat || DROP == kDropRows64 ? p.m.drop_scale : 1.0f);
+    store_rows(dkacc, dvacc, DROP == kDropFlat || DROP == kDropRows64 ? p.m.drop_scale : 1.0f);
 }
 
 template <int D, bool HASMASK, bool TIMING, bool VECMASK = false, int DROP = kDropNone, bool BITS = false>
@@ -835,18 +890,19 @@ __global__ __launch_bounds__(256) void bwd_dkdv_dealt_kernel(const BwdParams p) 
     bwd_dkdv_body<D, false, false, false, kDropNone, BITS, true>(p, (int)blockIdx.x, (int)gridDim.x);
 }
 
-// dK^T / dV^T accumulators (rows = d, column = a lane's key) of the 32 keys from kw0 on -> bf16 rows of dK (scaled) and dV
+// dK^T / dV^T accumulators (rows = d, column = a lane's key) of the 32 keys from kw0 on -> bf16 rows of dK (scaled) and dV, of which
+// dkbase and dvbase are key 0
 template <int D>
 __device__ __forceinline__ void dkdv_store(const BwdParams& p, uint16_t* own, const f32x16 (&dkacc)[D / 32], const f32x16 (&dvacc)[D / 32],
-                                           int b, int hh, int kw0, float dv_scale) {
+                                           uint16_t* dkbase, uint16_t* dvbase, int Sk, int kw0, float dv_scale) {
     const auto rows_of = [&](const f32x16 (&acc)[D / 32], float s) {
         return [&acc, s](int db, int g) {
             const f32x16& a = acc[db];
             return u32x2{pack_bf16(a[4 * g] * s, a[4 * g + 1] * s), pack_bf16(a[4 * g + 2] * s, a[4 * g + 3] * s)};
         };
     };
-    store_rows32<D>(own, p.dk + b * p.dks.b + hh * p.dks.h + (int64_t)kw0 * p.dks.n, p.dks.n, p.Sk - kw0, p.d, rows_of(dkacc, p.scale));
-    store_rows32<D>(own, p.dv + b * p.dvs.b + hh * p.dvs.h + (int64_t)kw0 * p.dvs.n, p.dvs.n, p.Sk - kw0, p.d, rows_of(dvacc, dv_scale));
+    store_rows32<D>(own, dkbase + (int64_t)kw0 * p.dks.n, p.dks.n, Sk - kw0, p.d, rows_of(dkacc, p.scale));
+    store_rows32<D>(own, dvbase + (int64_t)kw0 * p.dvs.n, p.dvs.n, Sk - kw0, p.d, rows_of(dvacc, dv_scale));
 }
 
 // Sums the fp32 partials that the split workgroups of one key block left behind and writes dK, dV; keys that nothing attends
@@ -916,8 +972,10 @@ struct BwdDqTile {
 // EXCL, DEALT: see there.  Only the general form compiles per-element mask loads in; the others fit two workgroups per unit.
 // KG = 2: two groups of NW wavefronts share the workgroup's queries, each walks one half of the key tiles in LDS stages of its
 // own, and the second adds its dQ to the first's through LDS: for grids that give a compute unit one workgroup at most.
-template <int D, int EXCL, int NW, int DROP, int KG, bool DEALT>
-__device__ __forceinline__ void bwd_dq_body(const BwdParams& p) {
+// PACKED: the unit is a query tile of one of several sequences of different lengths (packed_units.hpp), `u`.
+template <int D, int EXCL, int NW, int DROP, int KG, bool DEALT, bool PACKED = false>
+__device__ __forceinline__ void bwd_dq_body(const BwdParams& p, const PackedUnit& u = PackedUnit()) {
+    static_assert(!PACKED || (EXCL == kExNone && DROP == kDropNone && !DEALT), "packed sequences: causal flag and lengths only");
     static_assert(KG == 1 || (KG == 2 && EXCL == kExNone), "key groups: nothing excluded but by causal flag and key lengths");
     constexpr bool HASMASK = EXCL == kExRows16 || EXCL == kExGeneral, VECMASK = EXCL == kExRows16, BITS = EXCL == kExBits, KEYS = EXCL == kExKeys || BITS;
     using T = BwdDqTile<D>;
@@ -935,18 +993,24 @@ __device__ __forceinline__ void bwd_dq_body(const BwdParams& p) {
     uint16_t* lds = lds_all + (KG == 1 ? 0 : group * (T::LDS_BYTES / 2));
     const int n = lane & 31, h = lane >> 5;
 
-    const int n_qt = (p.Sq + BM - 1) / BM;
+    const int Sq = PACKED ? u.Sq : p.Sq, Sk = PACKED ? u.Sk : p.Sk;
+    const int past = PACKED ? u.past : 0;             // under the causal flag query i attends to key j <= i + past
+    const int n_qt = (Sq + BM - 1) / BM;
     const bool falling = !(EXCL == kExKeys) && p.m.causal && !p.m.kv_len;
-    int wg, part = 0;
-    if (p.dq_parts > 1) {
+    int wg = 0, part = 0;
+    if constexpr (PACKED) {
+        wg = u.unit;
+        part = u.part;
+    } else if (p.dq_parts > 1) {
         const int all = xcd_remap_split(blockIdx.x, gridDim.x);
         part = all % p.dq_parts;
         wg = all / p.dq_parts;
     } else {
         wg = p.dq_base + xcd_remap_heads<KG == 1 && !BITS>(blockIdx.x, gridDim.x, n_qt, p.m.kv_len || KEYS, falling);
     }
-    int qt = wg % n_qt, bh = wg / n_qt;
-    if constexpr (DEALT) {
+    int qt = PACKED ? u.tile : wg % n_qt, bh = PACKED ? 0 : wg / n_qt;
+    if constexpr (PACKED) {
+    } else if constexpr (DEALT) {
         int t, s;
         dealt_unit<!BITS>(blockIdx.x, n_qt, p.B, p.H, !falling, t, s);
         qt = __builtin_amdgcn_readfirstlane(falling ? n_qt - 1 - t : t);
@@ -954,25 +1018,30 @@ __device__ __forceinline__ void bwd_dq_body(const BwdParams& p) {
     } else if (falling && p.dq_parts == 1) {
         causal_longest_first<KG == 1>(wg, n_qt, gridDim.x, qt, bh);
     }
-    if (!BITS && (KEYS || p.m.kv_len) && p.dq_parts == 1) bh = longest_batches_first<KEYS>(bh, p.B, p.H, p.Sk, p.m);
+    if (!PACKED && !BITS && (KEYS || p.m.kv_len) && p.dq_parts == 1) bh = longest_batches_first<KEYS>(bh, p.B, p.H, p.Sk, p.m);
     const int b = bh / p.H, hh = bh % p.H;
     const int q0 = qt * BM;
     const int qw0 = q0 + wave * 32;
 
-    const uint16_t* qbase = p.q + b * p.qs.b + hh * p.qs.h;
-    const uint16_t* kbase = p.k + b * p.ks.b + hh * p.ks.h;
-    const uint16_t* vbase = p.v + b * p.vs.b + hh * p.vs.h;
-    const uint16_t* dobase = p.dout + b * p.dos.b + hh * p.dos.h;
+    const uint16_t* qbase = PACKED ? p.q + u.q_at(p.qs) : p.q + b * p.qs.b + hh * p.qs.h;
+    const uint16_t* kbase = PACKED ? p.k + u.k_at(p.ks) : p.k + b * p.ks.b + hh * p.ks.h;
+    const uint16_t* vbase = PACKED ? p.v + u.k_at(p.vs) : p.v + b * p.vs.b + hh * p.vs.h;
+    const uint16_t* dobase = PACKED ? p.dout + u.q_at(p.dos) : p.dout + b * p.dos.b + hh * p.dos.h;
+    auto obase = [&]() { return PACKED ? p.o + u.q_at(p.os) : p.o + b * p.os.b + hh * p.os.h; };
+    auto stat_row = [&]() { return PACKED ? u.stat_row() : (int64_t)bh * p.Sq; };
 
-    int klimit = p.Sk;
-    if (p.m.kv_len) klimit = min(klimit, max(p.m.kv_len[b], 0));
+    int klimit = Sk;
+    if (!PACKED && p.m.kv_len) klimit = min(klimit, max(p.m.kv_len[b], 0));
     int kend = klimit;
-    if (p.m.causal) kend = min(kend, q0 + BM);
+    if (p.m.causal) kend = min(kend, q0 + BM + past);
+    if constexpr (PACKED) kend = max(kend, 0);
     int n_tiles = (kend + BN - 1) / BN;
     const uint8_t* mbase = HASMASK || EXCL == kExKeys ? mask_head_base(p.m, b, hh) : nullptr;
     int t_lo = 0;             // first tile of this workgroup's share of the walk
-    if (p.dq_parts > 1) {
-        const int per = (n_tiles + p.dq_parts - 1) / p.dq_parts;
+    const int parts = PACKED ? packed_parts(u, n_tiles) : p.dq_parts;
+    if (PACKED && part >= parts) return;
+    if (parts > 1) {
+        const int per = PACKED ? packed_uniform((n_tiles + parts - 1) / parts) : (n_tiles + parts - 1) / parts;
         t_lo = part * per;
         n_tiles = min(n_tiles, t_lo + per) - t_lo;      // not positive: nothing to do
     }
@@ -1045,7 +1114,7 @@ __device__ __forceinline__ void bwd_dq_body(const BwdParams& p) {
 
     // ---- Q and dO fragments (B operands: column = query, 8 consecutive d), per-query scalars; through stage 1
     const int qrow = qw0 + n;
-    const bool qok = qrow < p.Sq;
+    const bool qok = qrow < Sq;
     bf16x8 qf[DC], dof[DC];
     // Per-query scalars, formed here and also left in the workspace for the dK/dV kernel that runs next:
     //   delta = rowsum(dO * O)   (the bf16 O that the forward saved)
@@ -1054,10 +1123,10 @@ __device__ __forceinline__ void bwd_dq_body(const BwdParams& p) {
     {
         uint16_t* const pass = lds + T::STAGE_ELEMS + wave * 1024;
         u32x4 wq[DC], wd[DC], wo[DC];
-        load_rows32<D>(wq, qbase + (int64_t)qw0 * p.qs.n, p.qs.n, p.Sq - qw0, p.d);
-        load_rows32<D>(wd, dobase + (int64_t)qw0 * p.dos.n, p.dos.n, p.Sq - qw0, p.d);
-        load_rows32<D>(wo, p.o + b * p.os.b + hh * p.os.h + (int64_t)qw0 * p.os.n, p.os.n, p.Sq - qw0, p.d);
-        const float l = qok ? p.lse[(int64_t)bh * p.Sq + qrow] : 0.f;
+        load_rows32<D>(wq, qbase + (int64_t)qw0 * p.qs.n, p.qs.n, Sq - qw0, p.d);
+        load_rows32<D>(wd, dobase + (int64_t)qw0 * p.dos.n, p.dos.n, Sq - qw0, p.d);
+        load_rows32<D>(wo, obase() + (int64_t)qw0 * p.os.n, p.os.n, Sq - qw0, p.d);
+        const float l = qok ? p.lse[stat_row() + qrow] : 0.f;
         fragments_of_rows32<D>(pass, wq, [&](auto dc, u32x4 f) { qf[decltype(dc)::value] = __builtin_bit_cast(bf16x8, f); });
         fragments_of_rows32<D>(pass, wd, [&](auto dc, u32x4 f) { dof[decltype(dc)::value] = __builtin_bit_cast(bf16x8, f); });
         float part = 0.f;
@@ -1071,8 +1140,8 @@ __device__ __forceinline__ void bwd_dq_body(const BwdParams& p) {
             lse2 = (l == -INFINITY) ? INFINITY : l * kLog2e;
             delta = part;
             if (h == 0 && group == 0) {
-                p.ndelta[(int64_t)bh * p.Sq + qrow] = -delta;
-                p.lse2[(int64_t)bh * p.Sq + qrow] = lse2;
+                p.ndelta[stat_row() + qrow] = -delta;
+                p.lse2[stat_row() + qrow] = lse2;
             }
         }
     }
@@ -1182,7 +1251,7 @@ __device__ __forceinline__ void bwd_dq_body(const BwdParams& p) {
                 pr = keep_bits[kb] & (1u << (8 * (r >> 2) + (r & 3))) ? pr : 0.f;
             } else if (MASKED) {
                 const int key = key0 + 32 * kb + acc_row(r, h);
-                bool drop = (key >= klimit) | ((p.m.causal != 0) & (key > qrow));     // bitwise: selects, not branches
+                bool drop = (key >= klimit) | ((p.m.causal != 0) & (key > qrow + past));     // bitwise: selects, not branches
                 if (HASMASK) {
                     if (vec_mask) drop = drop || !mrow.keep(kb, r, h);
                     else if (!drop && qok) drop = !mask_attends(p.m, mbase, (int64_t)qrow * p.m.sq + (int64_t)key * p.m.sk);
@@ -1266,7 +1335,7 @@ __device__ __forceinline__ void bwd_dq_body(const BwdParams& p) {
     };
 
     int n_full = HASMASK ? 0 : KEYS ? kt.n_whole : klimit / BN;
-    if (p.m.causal) n_full = min(n_full, (q0 + 1) / BN);
+    if (p.m.causal) n_full = min(n_full, PACKED ? max(q0 + 1 + past, 0) / BN : (q0 + 1) / BN);
     n_full = min(n_full - t_lo, n_tiles);
     using IM = std::integral_constant<int, -1>;
     using I0 = std::integral_constant<int, 0>;
@@ -1304,8 +1373,8 @@ __device__ __forceinline__ void bwd_dq_body(const BwdParams& p) {
     }
 
     // ---- epilogue: fp32 partial sums for bwd_dq_merge_kernel, in accumulator order: [db][group of four][thread] ...
-    if (p.dq_parts > 1) {
-        float* dst = p.split_ws + ((size_t)wg * p.dq_parts + part) * (size_t)(BM * D);
+    if (parts > 1) {
+        float* dst = p.split_ws + (PACKED ? (size_t)wg : (size_t)wg * parts + part) * (size_t)(BM * D);
 #pragma unroll
         for (int db = 0; db < DB; ++db)
 #pragma unroll
@@ -1316,7 +1385,8 @@ __device__ __forceinline__ void bwd_dq_body(const BwdParams& p) {
         return;
     }
     // ... or dQ = scale * dQ^T, bf16 (every walk ended with a barrier: the tiles are free)
-    store_rows32<D>(lds_all + wave * 32 * RS, p.dq + b * p.dqs.b + hh * p.dqs.h + (int64_t)qw0 * p.dqs.n, p.dqs.n, p.Sq - qw0, p.d, [&](int db, int g) {
+    uint16_t* const dqbase = PACKED ? p.dq + u.q_at(p.dqs) : p.dq + b * p.dqs.b + hh * p.dqs.h;
+    store_rows32<D>(lds_all + wave * 32 * RS, dqbase + (int64_t)qw0 * p.dqs.n, p.dqs.n, Sq - qw0, p.d, [&](int db, int g) {
         const f32x16& a = dqacc[db];
         return u32x2{pack_bf16(a[4 * g] * p.scale, a[4 * g + 1] * p.scale), pack_bf16(a[4 * g + 2] * p.scale, a[4 * g + 3] * p.scale)};
     });

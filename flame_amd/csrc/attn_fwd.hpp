@@ -22,6 +22,7 @@
 #include <type_traits>
 
 #include "attn_common.hpp"
+#include "packed_units.hpp"
 
 namespace fattn {
 
@@ -43,6 +44,7 @@ struct FwdParams {
     int key_splits = 1;          // 1: O and LSE are written directly
     float* part_o = nullptr;     // [key_splits][B*H*Sq][dv]
     float* part_lse = nullptr;   // [key_splits][B*H*Sq], natural log, -inf for a slice without an attended key, NaN for one with a NaN
+    // (packed sequences: the unnormalised sums of a unit in part_o, and the maximum, in units of log 2, and sum of its rows in part_lse)
 };
 
 template <int D>
@@ -71,8 +73,10 @@ typedef uint16_t u16x8_any __attribute__((ext_vector_type(8), aligned(2)));
 // read once per workgroup.
 // AHEAD: a bias is requested a step earlier (see EARLY).
 // DEALT: the units come in the order of causal_order.hpp (deals_units, which the host asks).
-template <int D, int EXCL, int NW, int DROP, int KG, bool AHEAD, bool DEALT>
-__device__ __forceinline__ void fwd_body(const FwdParams& p) {
+// PACKED: the unit is a query tile of one of several sequences of different lengths (packed_units.hpp), `u`.
+template <int D, int EXCL, int NW, int DROP, int KG, bool AHEAD, bool DEALT, bool PACKED = false>
+__device__ __forceinline__ void fwd_body(const FwdParams& p, const PackedUnit& u = PackedUnit()) {
+    static_assert(!PACKED || (EXCL == kExNone && DROP == kDropNone && !AHEAD && !DEALT), "packed sequences: causal flag and lengths only");
     static_assert(KG == 1 || (KG == 2 && EXCL == kExNone), "key groups: nothing excluded but by causal flag and key lengths");
     static_assert(!DEALT || (KG == 1 && DROP == kDropNone), "more than one workgroup per compute unit, no dropout");
     using T = FwdTile<D>;
@@ -98,13 +102,19 @@ __device__ __forceinline__ void fwd_body(const FwdParams& p) {
     const int n = lane & 31, h = lane >> 5;
     uint16_t* lds = lds_all + (KG == 1 ? 0 : group * (T::LDS_BYTES / 2));
 
-    const int n_qt = (p.Sq + BM - 1) / BM;
+    const int Sq = PACKED ? u.Sq : p.Sq, Sk = PACKED ? u.Sk : p.Sk;
+    const int past = PACKED ? u.past : 0;             // under the causal flag query i attends to key j <= i + past
+    const int n_qt = (Sq + BM - 1) / BM;
     constexpr bool KNOWS_BIAS = EXCL == kExBiasF32 || EXCL == kExBiasBf16;       // no causal flag, no key lengths
     const bool falling = !KNOWS_BIAS && EXCL != kExKeys && p.m.causal && !p.m.kv_len;
     const bool by_batch = !KNOWS_BIAS && (p.m.kv_len || EXCL == kExKeys || EXCL == kExBits);
-    const int wg = p.wg_base + xcd_remap_heads<NW == 4 && KG == 1 && EXCL != kExBits>(blockIdx.x, gridDim.x, n_qt, by_batch, falling);
-    int qt = wg % n_qt, bh = wg / n_qt;
-    if constexpr (DEALT) {
+    int wg = 0, qt = u.tile, bh = 0;
+    if constexpr (!PACKED) {
+        wg = p.wg_base + xcd_remap_heads<NW == 4 && KG == 1 && EXCL != kExBits>(blockIdx.x, gridDim.x, n_qt, by_batch, falling);
+        qt = wg % n_qt, bh = wg / n_qt;
+    }
+    if constexpr (PACKED) {
+    } else if constexpr (DEALT) {
         int t, s;
         dealt_unit<NW == 4 && EXCL != kExBits>(blockIdx.x, n_qt, p.B, p.H, !falling, t, s);
         qt = __builtin_amdgcn_readfirstlane(falling ? n_qt - 1 - t : t);         // (the compiler divides in vector registers)
@@ -112,7 +122,7 @@ __device__ __forceinline__ void fwd_body(const FwdParams& p) {
     } else if (falling) {
         causal_longest_first<NW == 4 && KG == 1>(wg, n_qt, gridDim.x, qt, bh);
     }
-    if (EXCL == kExKeys || (p.m.kv_len && EXCL != kExBits)) bh = longest_batches_first<EXCL == kExKeys>(bh, p.B, p.H, p.Sk, p.m);
+    if (!PACKED && (EXCL == kExKeys || (p.m.kv_len && EXCL != kExBits))) bh = longest_batches_first<EXCL == kExKeys>(bh, p.B, p.H, p.Sk, p.m);
     // a bias that all batches share: its rows are read by the batches' workgroups one after the other on one XCD, from its L2
     if ((EXCL == kExBiasF32 || EXCL == kExBiasBf16) && p.m.bb == 0) {
         const int rest = wg / p.B;
@@ -124,18 +134,31 @@ __device__ __forceinline__ void fwd_body(const FwdParams& p) {
     const int qw0 = q0 + wave * 32;
     const int qi = qw0 + n;                           // this lane's query
 
-    const uint16_t* qbase = p.q + b * p.qs.b + hh * p.qs.h;
-    const uint16_t* kbase = p.k + b * p.ks.b + hh * p.ks.h;
-    const uint16_t* vbase = p.v + b * p.vs.b + hh * p.vs.h;
+    const uint16_t* qbase = PACKED ? p.q + u.q_at(p.qs) : p.q + b * p.qs.b + hh * p.qs.h;
+    const uint16_t* kbase = PACKED ? p.k + u.k_at(p.ks) : p.k + b * p.ks.b + hh * p.ks.h;
+    const uint16_t* vbase = PACKED ? p.v + u.k_at(p.vs) : p.v + b * p.vs.b + hh * p.vs.h;
 
-    int klimit = p.Sk;
-    if (p.m.kv_len) klimit = min(klimit, max(p.m.kv_len[b], 0));
+    int klimit = Sk;
+    if (!PACKED && p.m.kv_len) klimit = min(klimit, max(p.m.kv_len[b], 0));
     int kend = klimit;
-    if (p.m.causal) kend = min(kend, q0 + BM);
+    if (p.m.causal) kend = min(kend, q0 + BM + past);
+    if constexpr (PACKED) kend = max(kend, 0);
     int n_tiles = (kend + BN - 1) / BN;
     // The tiles of this wavefront's group become tiles 0 .. n_tiles - 1 of a walk that starts at key `key0`.
     const int n_first = (n_tiles + 1) / 2;            // of group 0
-    const int key0 = KG == 1 ? 0 : group * n_first * BN;
+    int key0 = KG == 1 ? 0 : group * n_first * BN;
+    const int parts = PACKED ? packed_parts(u, n_tiles) : 1;          // that share this walk, each leaving its sums
+    if constexpr (PACKED) {
+        if (u.part >= parts) return;
+        if (parts > 1) {
+            const int share = packed_uniform((n_tiles + parts - 1) / parts);
+            key0 = u.part * share * BN;
+            n_tiles = min(share, n_tiles - u.part * share);           // (not positive: nothing is left for this part)
+            klimit -= key0;
+            kbase += key0 * p.ks.n;
+            vbase += key0 * p.vs.n;
+        }
+    }
     if constexpr (KG == 2) {
         n_tiles = group ? n_tiles - n_first : n_first;
         klimit -= key0;
@@ -223,7 +246,7 @@ __device__ __forceinline__ void fwd_body(const FwdParams& p) {
     {
         static_assert(T::q_pass_bytes(NW) == 0 || (KG == 1 && !BIAS && !KEYS), "nothing else lies behind the stages");
         u32x4 w[DC];
-        load_rows32<D>(w, qbase + (int64_t)qw0 * p.qs.n, p.qs.n, p.Sq - qw0, p.d);
+        load_rows32<D>(w, qbase + (int64_t)qw0 * p.qs.n, p.qs.n, Sq - qw0, p.d);
         fragments_of_rows32<D>(lds + (T::q_pass_bytes(NW) ? 2 * T::STAGE_ELEMS : T::STAGE_ELEMS + T::TILE_ELEMS) + wave * 1024, w,
                                [&](auto dc, u32x4 f) { qf[decltype(dc)::value] = __builtin_bit_cast(bf16x8, f); });
     }
@@ -291,7 +314,7 @@ __device__ __forceinline__ void fwd_body(const FwdParams& p) {
             keep_bits[0] = (uint32_t)w >> (4 * h);
             keep_bits[1] = (uint32_t)(w >> 32) >> (4 * h);
         }
-        const int limit = (p.m.causal ? min(klimit, qi + 1 - key0) : klimit) - t * BN;
+        const int limit = (p.m.causal ? min(klimit, qi + 1 + past - key0) : klimit) - t * BN;
         lim = limit - 4 * h;
         if constexpr (EXCL == kExRows16) {
             // folded into the mask bytes where they cut the tile: the per-element test is then the mask byte alone
@@ -302,7 +325,7 @@ __device__ __forceinline__ void fwd_body(const FwdParams& p) {
     // Tiles below t_clean need no exclusions for any query of the workgroup; the rest (ragged tail, causal
     // diagonal, or everything under an explicit mask) carry per-element exclusions.
     int t_clean = KEYS ? kt.n_whole : (EXCL == kExNone || BIAS) ? klimit / BN : 0;
-    if (p.m.causal) t_clean = min(t_clean, (q0 + 1 - key0) / BN);
+    if (p.m.causal) t_clean = min(t_clean, (q0 + 1 + past - key0) / BN);
     t_clean = max(min(t_clean, n_tiles), 0);
     if constexpr (BITS) {
         const int first = t_clean == 0 ? 0 : (t_clean - 1) | 1;      // that a step with exclusions takes: steps go in pairs, see below
@@ -678,15 +701,36 @@ __device__ __forceinline__ void fwd_body(const FwdParams& p) {
     }
 
     // ---- epilogue: O through LDS where nobody reads any more (KG: the state of the second group this wavefront has joined)
+    if constexpr (PACKED) {
+        if (parts > 1) {           // sums in the accumulators' order, [db][group of four][thread], for fwd_packed_merge_kernel
+            const float l = l_run + xhalf(l_run);
+            float* const sums = p.part_o + (int64_t)u.unit * (BM * D);
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const f32x16& a = oacc[db];
+                    *reinterpret_cast<f32x4*>(sums + ((db * 4 + g) * 256 + tid) * 4) = f32x4{a[4 * g], a[4 * g + 1], a[4 * g + 2], a[4 * g + 3]};
+                }
+            if (h == 0) reinterpret_cast<f32x2*>(p.part_lse)[(int64_t)u.unit * BM + 32 * wave + n] = f32x2{m_run * c_log2, l};
+            return;
+        }
+    }
     if constexpr (KG == 1) __syncthreads();
     uint16_t* own = KG == 1 ? lds + wave * 32 * RS : lds_all + wave * (4 * DB + 1) * 64 * 8;
     const float l = l_run + xhalf(l_run);
     float inv = l > 0.f ? 1.0f / l : 0.f;
     if constexpr (DROP == kDropFlat || DROP == kDropRows64) inv *= p.m.drop_scale;
-    store_rows32<D>(own, p.o + b * p.os.b + hh * p.os.h + (int64_t)qw0 * p.os.n, p.os.n, p.Sq - qw0, p.dv, [&](int db, int g) {
+    uint16_t* const obase = PACKED ? p.o + u.q_at(p.os) : p.o + b * p.os.b + hh * p.os.h;
+    store_rows32<D>(own, obase + (int64_t)qw0 * p.os.n, p.os.n, Sq - qw0, p.dv, [&](int db, int g) {
         const f32x16& a = oacc[db];
         return u32x2{pack_bf16(a[4 * g] * inv, a[4 * g + 1] * inv), pack_bf16(a[4 * g + 2] * inv, a[4 * g + 3] * inv)};
     });
+    if constexpr (PACKED) {       // (the row from the lane's number: kept through the walk, it went to scratch memory)
+        const int at = (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0));
+        if (p.lse && at < 32 && qw0 + at < Sq) p.lse[u.stat_row() + qw0 + at] = l > 0.f ? (m_run * c_log2 + log2_fast(l)) * kLn2 : -INFINITY;
+        return;
+    }
     if (p.lse && h == 0 && qi < p.Sq) p.lse[(int64_t)bh * p.Sq + qi] = l > 0.f ? (m_run * c_log2 + log2_fast(l)) * kLn2 : -INFINITY;
 }
 

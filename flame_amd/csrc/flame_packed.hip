@@ -1,0 +1,198 @@
+// Entry points of the attention of packed sequences (attn_packed.hpp): argument checks and launches.
+#include <algorithm>
+#include <atomic>
+#include <climits>
+#include <cmath>
+
+#include "attn_packed.hpp"
+#include "../../include/flame_attn.h"
+
+using namespace fattn;
+
+namespace {
+
+// [rows, heads, D] element strides: D stride 1, the others multiples of 8 (16-byte rows)
+int check_rows(const void* base, const int64_t* st) {
+    if (!base || !st) return FLAME_ATTN_ERR_INVALID;
+    if (st[2] != 1) return FLAME_ATTN_ERR_UNSUPPORTED;
+    if ((st[0] | st[1]) & 7) return FLAME_ATTN_ERR_UNSUPPORTED;
+    if (st[0] < 0 || st[1] < 0 || st[0] >= (int64_t(1) << 24)) return FLAME_ATTN_ERR_UNSUPPORTED;   // row offsets inside a tile are kept in 32 bits
+    if (reinterpret_cast<uintptr_t>(base) & 15u) return FLAME_ATTN_ERR_UNSUPPORTED;
+    return FLAME_ATTN_OK;
+}
+Strides rows_of(const int64_t* st) { return Strides{0, st[1], st[0]}; }
+
+// an output whose rows or heads lie on each other would be written by several workgroups at once
+bool overlaps(const int64_t* st, int rows, int heads, int D) {
+    const int64_t n = st[0], h = st[1];
+    if ((rows > 1 && n < D) || (heads > 1 && h < D)) return true;
+    if (rows == 1 || heads == 1) return false;
+    return n >= h ? n < h * (heads - 1) + D : h < n * (rows - 1) + D;
+}
+
+int set_lds(const void* kern, int bytes, std::atomic<uint64_t>& done) {      // a kernel's dynamic LDS size, once per kernel and device
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess) return (int)hipErrorInvalidDevice;
+    const uint64_t bit = uint64_t(1) << (dev & 63);
+    if (done.load(std::memory_order_relaxed) & bit) return FLAME_ATTN_OK;
+    const hipError_t e = hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != hipSuccess) return (int)e;
+    done.fetch_or(bit, std::memory_order_relaxed);
+    return FLAME_ATTN_OK;
+}
+
+template <class P>
+int launch(void (*kern)(P, PackedArgs), int lds, std::atomic<uint64_t>& done, int64_t units, int heads, const P& p, const PackedArgs& a, hipStream_t s) {
+    if (units * heads > INT32_MAX) return FLAME_ATTN_ERR_UNSUPPORTED;
+    if (const int rc = set_lds(reinterpret_cast<const void*>(kern), lds, done)) return rc;
+    hipLaunchKernelGGL(kern, dim3((unsigned)(units * heads)), dim3(256), (size_t)lds, s, p, a);
+    return (int)hipGetLastError();
+}
+template <class P>
+int launch_merge(void (*kern)(P, PackedArgs), int64_t tiles, int heads, int blocks, const P& p, const PackedArgs& a, hipStream_t s) {
+    hipLaunchKernelGGL(kern, dim3((unsigned)(tiles * heads), (unsigned)blocks), dim3(256), 0, s, p, a);
+    return (int)hipGetLastError();
+}
+
+int padded(int D) { return D <= 64 ? 64 : D <= 96 ? 96 : 128; }
+size_t align256(size_t x) { return (x + 255) / 256 * 256; }
+
+// log2 of what the card holds of a kernel's workgroups, two per compute unit or one
+constexpr int kRoomQueries = 9, kRoomKeys = 8;
+// Whether the walks of a problem's tiles are cut into parts: not where whole walks fill the card, nor where the mean one is short.
+bool parts_pay(int64_t slots, int heads, int n_seqs, int walked_rows, int room_log2) {
+    return n_seqs <= 64 && walked_rows / n_seqs >= 1024 && slots * heads * 2 < 3 << room_log2;
+}
+
+struct Parts {
+    int64_t slots, units;          // per head: tiles, and units at most
+    int room_log2;                 // 0: whole walks
+    size_t bytes;                  // of the units' sums
+};
+Parts parts_of(int tile_rows, int walked_rows, int n_seqs, int heads, int room_log2, size_t unit_bytes) {
+    Parts z{packed_slots(tile_rows, n_seqs, 128), 0, 0, 0};
+    z.units = z.slots;
+    if (parts_pay(z.slots, heads, n_seqs, walked_rows, room_log2)) {
+        z.room_log2 = room_log2;
+        z.units = PackedCut::most(z.slots, heads, room_log2);
+        z.bytes = align256((size_t)z.units * heads * unit_bytes);
+    }
+    return z;
+}
+Parts fwd_parts(int n_seqs, int T_q, int T_kv, int H, int D) { return parts_of(T_q, T_kv, n_seqs, H, kRoomQueries, (size_t)128 * (padded(D) * sizeof(float) + sizeof(f32x2))); }
+Parts dq_parts(int n_seqs, int T_q, int T_kv, int H, int D) { return parts_of(T_q, T_kv, n_seqs, H, kRoomQueries, (size_t)128 * padded(D) * sizeof(float)); }
+Parts dkdv_parts(int n_seqs, int T_q, int T_kv, int H, int H_kv, int D) {
+    return parts_of(T_kv, (int)std::min<int64_t>((int64_t)T_q * (H / H_kv), INT32_MAX), n_seqs, H_kv, kRoomKeys, (size_t)2 * 128 * padded(D) * sizeof(float));
+}
+
+template <int D>
+int launch_fwd(FwdParams p, PackedArgs a, void* workspace, size_t bytes, hipStream_t s) {
+    static std::atomic<uint64_t> done{0};
+    Parts z = fwd_parts(a.n, a.total_q, a.total_k, a.H, D);
+    if (!workspace || bytes < z.bytes) z.room_log2 = 0, z.units = z.slots;
+    a.room_log2 = z.room_log2;
+    p.part_o = static_cast<float*>(workspace);
+    p.part_lse = p.part_o + z.units * a.H * 128 * D;
+    if (const int rc = launch(fwd_packed_kernel<D>, FwdTile<D>::LDS_BYTES + FwdTile<D>::q_pass_bytes(4), done, z.units, a.H, p, a, s)) return rc;
+    return z.room_log2 ? launch_merge(fwd_packed_merge_kernel<D>, z.slots, a.H, D / 32, p, a, s) : FLAME_ATTN_OK;
+}
+
+template <int D>
+int launch_bwd(BwdParams p, PackedArgs a, size_t part_bytes, hipStream_t s) {
+    static std::atomic<uint64_t> done_q{0}, done_kv{0};
+    Parts q = dq_parts(a.n, a.total_q, a.total_k, a.H, D), kv = dkdv_parts(a.n, a.total_q, a.total_k, a.H, a.Hkv, D);
+    if (part_bytes < std::max(q.bytes, kv.bytes)) q.room_log2 = kv.room_log2 = 0, q.units = q.slots, kv.units = kv.slots;
+    a.room_log2 = q.room_log2;
+    if (const int rc = launch(bwd_dq_packed_kernel<D>, BwdDqTile<D>::LDS_BYTES, done_q, q.units, a.H, p, a, s)) return rc;
+    if (q.room_log2)
+        if (const int rc = launch_merge(bwd_dq_packed_merge_kernel<D>, q.slots, a.H, D / 32, p, a, s)) return rc;
+    a.room_log2 = kv.room_log2;
+    if (const int rc = launch(bwd_dkdv_packed_kernel<D>, BwdTile<D>::LDS_BYTES, done_kv, kv.units, a.Hkv, p, a, s)) return rc;
+    return kv.room_log2 ? launch_merge(bwd_dkdv_packed_merge_kernel<D>, kv.slots, a.Hkv, D / 32, p, a, s) : FLAME_ATTN_OK;
+}
+
+bool head_dim_ok(int D) { return D > 0 && D % 8 == 0 && D <= 128; }
+size_t bwd_rows_bytes(int H, int T_q) { return 2 * align256((size_t)H * T_q * sizeof(float)); }
+
+int check_sizes(const void* cu_q, const void* cu_k, int n_seqs, int T_q, int T_kv, int H, int H_kv, int D, float scale) {
+    if (!cu_q || !cu_k || n_seqs <= 0 || T_q <= 0 || T_kv <= 0 || H <= 0 || H_kv <= 0 || D <= 0) return FLAME_ATTN_ERR_INVALID;
+    if (H % H_kv != 0 || !(scale > 0.f) || !std::isfinite(scale)) return FLAME_ATTN_ERR_INVALID;
+    return head_dim_ok(D) ? FLAME_ATTN_OK : FLAME_ATTN_ERR_UNSUPPORTED;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t flame_attn_packed_fwd_workspace_bytes(int n_seqs, int T_q, int T_kv, int H, int D) {
+    if (n_seqs <= 0 || T_q <= 0 || T_kv <= 0 || H <= 0 || !head_dim_ok(D)) return 0;
+    return fwd_parts(n_seqs, T_q, T_kv, H, D).bytes;
+}
+
+int flame_attn_packed_fwd_bf16(const void* Q, const void* K, const void* V, void* O, void* LSE, const int32_t* cu_q, const int32_t* cu_k,
+                               int n_seqs, int T_q, int T_kv, int H, int H_kv, int D, float scale, const int64_t* q_strides,
+                               const int64_t* k_strides, const int64_t* v_strides, const int64_t* o_strides, int causal, void* workspace,
+                               size_t workspace_bytes, void* stream) {
+    int rc;
+    if ((rc = check_sizes(cu_q, cu_k, n_seqs, T_q, T_kv, H, H_kv, D, scale))) return rc;
+    if ((rc = check_rows(Q, q_strides)) || (rc = check_rows(K, k_strides)) || (rc = check_rows(V, v_strides)) || (rc = check_rows(O, o_strides))) return rc;
+    if (overlaps(o_strides, T_q, H, D) || (reinterpret_cast<uintptr_t>(workspace) & 15u)) return FLAME_ATTN_ERR_UNSUPPORTED;
+    FwdParams p{};
+    p.q = static_cast<const uint16_t*>(Q);
+    p.k = static_cast<const uint16_t*>(K);
+    p.v = static_cast<const uint16_t*>(V);
+    p.o = static_cast<uint16_t*>(O);
+    p.lse = static_cast<float*>(LSE);
+    p.qs = rows_of(q_strides); p.ks = rows_of(k_strides); p.vs = rows_of(v_strides); p.os = rows_of(o_strides);
+    p.d = p.dv = D;
+    p.scale = scale;
+    p.m.causal = causal ? 1 : 0;
+    const PackedArgs a{cu_q, cu_k, n_seqs, T_q, T_kv, H, H_kv, p.m.causal, 0};
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    return D <= 64 ? launch_fwd<64>(p, a, workspace, workspace_bytes, s)
+                   : D <= 96 ? launch_fwd<96>(p, a, workspace, workspace_bytes, s) : launch_fwd<128>(p, a, workspace, workspace_bytes, s);
+}
+
+size_t flame_attn_packed_bwd_workspace_bytes(int n_seqs, int T_q, int T_kv, int H, int H_kv, int D) {
+    if (n_seqs <= 0 || T_q <= 0 || T_kv <= 0 || H <= 0 || H_kv <= 0 || H % H_kv != 0 || !head_dim_ok(D)) return 0;
+    return bwd_rows_bytes(H, T_q) + std::max(dq_parts(n_seqs, T_q, T_kv, H, D).bytes, dkdv_parts(n_seqs, T_q, T_kv, H, H_kv, D).bytes);
+}
+
+int flame_attn_packed_bwd_bf16(const void* Q, const void* K, const void* V, const void* O, const void* dO, const void* LSE, void* dQ, void* dK,
+                               void* dV, const int32_t* cu_q, const int32_t* cu_k, int n_seqs, int T_q, int T_kv, int H, int H_kv, int D,
+                               float scale, const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
+                               const int64_t* o_strides, const int64_t* do_strides, const int64_t* dq_strides, const int64_t* dk_strides,
+                               const int64_t* dv_strides, int causal, void* workspace, size_t workspace_bytes, void* stream) {
+    int rc;
+    if ((rc = check_sizes(cu_q, cu_k, n_seqs, T_q, T_kv, H, H_kv, D, scale))) return rc;
+    if (!LSE || !workspace || workspace_bytes < bwd_rows_bytes(H, T_q)) return FLAME_ATTN_ERR_INVALID;
+    if (reinterpret_cast<uintptr_t>(workspace) & 15u) return FLAME_ATTN_ERR_UNSUPPORTED;
+    if ((rc = check_rows(Q, q_strides)) || (rc = check_rows(K, k_strides)) || (rc = check_rows(V, v_strides)) || (rc = check_rows(O, o_strides)) ||
+        (rc = check_rows(dO, do_strides)) || (rc = check_rows(dQ, dq_strides)) || (rc = check_rows(dK, dk_strides)) || (rc = check_rows(dV, dv_strides)))
+        return rc;
+    if (overlaps(dq_strides, T_q, H, D) || overlaps(dk_strides, T_kv, H_kv, D) || overlaps(dv_strides, T_kv, H_kv, D)) return FLAME_ATTN_ERR_UNSUPPORTED;
+    BwdParams p{};
+    p.q = static_cast<const uint16_t*>(Q);
+    p.k = static_cast<const uint16_t*>(K);
+    p.v = static_cast<const uint16_t*>(V);
+    p.o = static_cast<const uint16_t*>(O);
+    p.dout = static_cast<const uint16_t*>(dO);
+    p.lse = static_cast<const float*>(LSE);
+    p.dq = static_cast<uint16_t*>(dQ);
+    p.dk = static_cast<uint16_t*>(dK);
+    p.dv = static_cast<uint16_t*>(dV);
+    p.ndelta = static_cast<float*>(workspace);
+    p.lse2 = reinterpret_cast<float*>(static_cast<char*>(workspace) + bwd_rows_bytes(H, T_q) / 2);
+    p.split_ws = reinterpret_cast<float*>(static_cast<char*>(workspace) + bwd_rows_bytes(H, T_q));
+    const size_t part_bytes = workspace_bytes - bwd_rows_bytes(H, T_q);
+    p.qs = rows_of(q_strides); p.ks = rows_of(k_strides); p.vs = rows_of(v_strides); p.os = rows_of(o_strides);
+    p.dos = rows_of(do_strides); p.dqs = rows_of(dq_strides); p.dks = rows_of(dk_strides); p.dvs = rows_of(dv_strides);
+    p.d = D;
+    p.scale = scale;
+    p.m.causal = causal ? 1 : 0;
+    const PackedArgs a{cu_q, cu_k, n_seqs, T_q, T_kv, H, H_kv, p.m.causal, 0};
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    return D <= 64 ? launch_bwd<64>(p, a, part_bytes, s) : D <= 96 ? launch_bwd<96>(p, a, part_bytes, s) : launch_bwd<128>(p, a, part_bytes, s);
+}
+
+}  // extern "C"

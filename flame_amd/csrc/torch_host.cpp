@@ -15,13 +15,16 @@
 
 #include <algorithm>
 #include <cmath>
+#include <vector>
 
 #include <ATen/ATen.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>      // this torch names its HIP devices "cuda"
 #include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 
@@ -38,6 +41,8 @@ using at::Tensor;
     X(flame_attn_bwd_bf16) X(flame_attn_bwd_workspace_bytes) X(flame_attn_fwd_dropout_tiled_bf16)                       \
     X(flame_attn_bwd_dropout_tiled_bf16) X(flame_attn_materialised_workspace_bytes) X(flame_attn_fwd_materialised_bf16) \
     X(flame_attn_bwd_materialised_bf16) X(flame_sage_quant_qk_int8_ks) X(flame_sage_attn_fwd_bias_int8)                 \
+    X(flame_attn_packed_fwd_bf16) X(flame_attn_packed_fwd_workspace_bytes) X(flame_attn_packed_bwd_bf16) X(flame_attn_packed_bwd_workspace_bytes)                \
+    X(flame_attn_paged_workspace_bytes) X(flame_attn_paged_fwd_bf16) X(flame_kv_store_bf16) X(flame_kv_copy_pages_bf16)  \
     X(flame_attn_prep_rmsnorm_rope_bf16) X(flame_bf16_to_fp8) X(flame_fp8_to_bf16) X(flame_attn_cast_qkv_f32_to_bf16) X(flame_attn_cast_bf16_to_f32)
 
 struct Api {
@@ -752,6 +757,373 @@ PyObject* py_fp8(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// ---------------------------------------------------------------- packed sequences
+// [rows, heads, D] tensors of sequences one behind the other, and the bounds of the sequences
+struct PackedSizes {
+    int Tq, Tk, n, H, Hkv, D;
+};
+void check_device(const Tensor& t, const Tensor& like, const char* what) { check_that(t.is_cuda() && t.device() == like.device(), what); }
+int size32(int64_t n) {
+    check_that(n <= INT32_MAX, "a size exceeds 2^31 - 1");
+    return (int)n;
+}
+void check_workspace(const Tensor& ws, const Tensor& like) {
+    check_that(ws.scalar_type() == at::kByte && ws.is_contiguous(), "the workspace is a contiguous uint8 tensor");
+    check_device(ws, like, "all tensors are on one GPU");
+}
+void check_bounds(const Tensor& cu, const Tensor& like) {
+    check_that(cu.dim() == 1 && cu.scalar_type() == at::kInt && cu.size(0) >= 2 && cu.stride(0) == 1, "the bounds of the sequences are a contiguous int32 [sequences + 1] tensor");
+    check_device(cu, like, "all tensors are on one GPU");
+}
+PackedSizes packed_sizes(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu_q, const Tensor& cu_k) {
+    if (q.dim() != 3 || k.dim() != 3 || v.dim() != 3) fail(PyExc_ValueError, "packed attention expects 3-D input [rows, heads, D]");
+    check_that(k.sizes() == v.sizes() && q.size(2) == k.size(2), "k and v have one shape, and the head dim of q");
+    check_that(q.numel() > 0 && k.numel() > 0, "packed attention needs at least one query row and one key row");
+    check_that(q.size(1) % k.size(1) == 0, "the number of heads is a multiple of the number of key heads");
+    check_bounds(cu_q, q);
+    check_bounds(cu_k, q);
+    check_that(cu_q.size(0) == cu_k.size(0), "as many sequences of keys as of queries");
+    check_device(q, q, "the tensors are on a GPU");
+    check_device(k, q, "all tensors are on one GPU");
+    check_device(v, q, "all tensors are on one GPU");
+    return {size32(q.size(0)), size32(k.size(0)), size32(cu_q.size(0) - 1), size32(q.size(1)), size32(k.size(1)), size32(q.size(2))};
+}
+PackedSizes checked_sizes(const Tensor& q, const Tensor& k, const Tensor& cu_q) {        // of tensors that packed_sizes has seen: raises nothing
+    return {(int)q.size(0), (int)k.size(0), (int)cu_q.size(0) - 1, (int)q.size(1), (int)k.size(1), (int)q.size(2)};
+}
+void check_bf16_like(const Tensor& t, const Tensor& like, const char* what) {
+    check_that(t.scalar_type() == at::kBFloat16 && t.sizes() == like.sizes(), what);
+    check_device(t, like, "all tensors are on one GPU");
+}
+Tensor packed_f32(const PackedSizes& z, const Tensor& like) { return empty({z.H, z.Tq}, at::kFloat, like); }
+void check_lse(const Tensor& lse, const PackedSizes& z, const Tensor& like) {
+    check_that(lse.scalar_type() == at::kFloat && lse.is_contiguous() && lse.dim() == 2 && lse.size(0) == z.H && lse.size(1) == z.Tq, "lse is a contiguous fp32 [heads, rows] tensor");
+    check_device(lse, like, "all tensors are on one GPU");
+}
+
+void call_packed_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu_q, const Tensor& cu_k, const PackedSizes& z, float scale,
+                     bool causal, bool want_lse, Tensor workspace, Tensor& o, Tensor& lse) {
+    if (!o.defined()) o = empty(q.sizes(), at::kBFloat16, q);
+    if (!lse.defined() && want_lse) lse = packed_f32(z, q);
+    if (!workspace.defined()) workspace = optional_bytes_like(g_api.flame_attn_packed_fwd_workspace_bytes(z.n, z.Tq, z.Tk, z.H, z.D), q);
+    check_rc(g_api.flame_attn_packed_fwd_bf16(ptr(q), ptr(k), ptr(v), ptr(o), ptr(lse), static_cast<const int32_t*>(ptr(cu_q)),
+                                              static_cast<const int32_t*>(ptr(cu_k)), z.n, z.Tq, z.Tk, z.H, z.Hkv, z.D, scale, strides4(q), strides4(k),
+                                              strides4(v), strides4(o), causal, ptr(workspace), workspace.defined() ? (size_t)workspace.numel() : 0, stream_of(q)),
+             "flame_attn_packed_fwd_bf16");
+}
+int call_packed_bwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o, const Tensor& d_o, const Tensor& lse, const Tensor& cu_q,
+                    const Tensor& cu_k, const PackedSizes& z, float scale, bool causal, Tensor workspace, Grads& g) {
+    if (!workspace.defined()) {        // with the part that the call is only faster with, where the device has it left
+        workspace = optional_bytes_like(g_api.flame_attn_packed_bwd_workspace_bytes(z.n, z.Tq, z.Tk, z.H, z.Hkv, z.D), q);
+        if (!workspace.defined()) workspace = bytes_like(((size_t)z.H * z.Tq * 4 + 255) / 256 * 512, q);
+    }
+    if (!g.dq.defined()) {
+        g.dq = empty(q.sizes(), at::kBFloat16, q);
+        g.dk = empty(k.sizes(), at::kBFloat16, q);
+        g.dv = empty(v.sizes(), at::kBFloat16, q);
+    }
+    return g_api.flame_attn_packed_bwd_bf16(ptr(q), ptr(k), ptr(v), ptr(o), ptr(d_o), ptr(lse), ptr(g.dq), ptr(g.dk), ptr(g.dv),
+                                            static_cast<const int32_t*>(ptr(cu_q)), static_cast<const int32_t*>(ptr(cu_k)), z.n, z.Tq, z.Tk, z.H, z.Hkv,
+                                            z.D, scale, strides4(q), strides4(k), strides4(v), strides4(o), strides4(d_o), strides4(g.dq), strides4(g.dk),
+                                            strides4(g.dv), causal, ptr(workspace), (size_t)workspace.numel(), stream_of(q));
+}
+// bf16 rows that the kernels load: the head dim contiguous, the others on 16 bytes (of axes of one element, too, whose strides a
+// contiguous tensor may have any of)
+Tensor packed_rows(const Tensor& x) {
+    const Tensor t = x.scalar_type() == at::kBFloat16 ? x : x.to(at::kBFloat16);
+    bool fits = t.stride(-1) == 1 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
+    for (int64_t ax = 0; ax + 1 < t.dim(); ++ax) fits = fits && (t.stride(ax) & 7) == 0;
+    return fits ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+struct SdpaPacked : public torch::autograd::Function<SdpaPacked> {
+    // saves O and the log-sum-exp only; the backward recomputes the probabilities
+    static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu_q, const Tensor& cu_k,
+                          bool causal, double scale) {
+        Tensor o, lse;
+        call_packed_fwd(q, k, v, cu_q, cu_k, checked_sizes(q, k, cu_q), (float)scale, causal, true, Tensor(), o, lse);
+        ctx->save_for_backward({q, k, v, o, lse, cu_q, cu_k});
+        ctx->saved_data["causal"] = causal;
+        ctx->saved_data["scale"] = scale;
+        return o;
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &o = saved[3], &lse = saved[4], &cu_q = saved[5], &cu_k = saved[6];
+        c10::OptionalDeviceGuard device(q.device());
+        at::NoGradGuard no_grad;
+        const PackedSizes z = checked_sizes(q, k, cu_q);
+        Grads g;
+        const int rc = call_packed_bwd(q, k, v, o, packed_rows(grads[0]), lse, cu_q, cu_k, z, (float)ctx->saved_data["scale"].toDouble(),
+                                       ctx->saved_data["causal"].toBool(), Tensor(), g);
+        if (rc != FLAME_ATTN_OK) throw_python({"flame_attn_packed_bwd_bf16", rc});
+        return {g.dq, g.dk, g.dv, Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+
+// A leaf whose gradients an earlier graph, still alive, accumulates on another stream: its backward would wait for that stream, which
+// in a capture is an error that the autograd engine does not survive.  Refused where the capture can still be told.
+void check_capture(const Tensor& t) {
+    if (!t.requires_grad() || !t.is_leaf()) return;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+    if (!node) return;
+    const auto stream = node->stream();
+    const c10::Stream now = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).unwrap();
+    TORCH_CHECK(!stream || *stream == now, "packed attention: a graph recorded on another stream holds one of the leaves; delete it before its backward is captured");
+}
+
+// sdpa_packed(q, k, v, cu_q, cu_k | None, causal, scale | None)
+PyObject* py_sdpa_packed(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        need_args(n, 7);
+        const Tensor &q = tensor_arg(a[0], "q"), &k = tensor_arg(a[1], "k"), &v = tensor_arg(a[2], "v"), &cu_q = tensor_arg(a[3], "cu_seqlens");
+        const Tensor& cu_k = a[4] == Py_None ? cu_q : tensor_arg(a[4], "cu_seqlens_k");
+        const PackedSizes z = packed_sizes(q, k, v, cu_q, cu_k);
+        for (const Tensor* t : {&q, &k, &v})
+            TORCH_CHECK_NOT_IMPLEMENTED(!t->_fw_grad(0).defined(), "packed attention has no forward-mode derivative: an input carries a tangent");
+        const bool causal = bool_arg(a[5]);
+        const double scale = a[6] == Py_None ? 1.0 / std::sqrt((double)z.D) : float_arg(a[6]);
+        Tensor out;
+        {
+            WithoutGil nogil;
+            c10::OptionalDeviceGuard device(q.device());
+            const at::ScalarType orig = q.scalar_type();
+            const bool graph = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad());
+            if (graph && c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None)
+                for (const Tensor* t : {&q, &k, &v}) check_capture(*t);
+            const Tensor qb = packed_rows(q), kb = packed_rows(k), vb = packed_rows(v);
+            Tensor lse;
+            if (graph) out = SdpaPacked::apply(qb, kb, vb, cu_q, cu_k, causal, scale);
+            else call_packed_fwd(qb, kb, vb, cu_q, cu_k, z, (float)scale, causal, false, Tensor(), out, lse);
+            if (orig != at::kBFloat16) out = out.to(orig);
+        }
+        return THPVariable_Wrap(out);
+    });
+}
+
+// attn_packed_fwd(q, k, v, cu_q, cu_k, scale, causal, want_lse, out, lse_out, workspace) -> (o, lse | None)
+PyObject* py_attn_packed_fwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        need_args(n, 11);
+        const Tensor &q = tensor_arg(a[0], "q"), &k = tensor_arg(a[1], "k"), &v = tensor_arg(a[2], "v"), &cu_q = tensor_arg(a[3], "cu_q"),
+                     &cu_k = tensor_arg(a[4], "cu_k");
+        const PackedSizes z = packed_sizes(q, k, v, cu_q, cu_k);
+        for (const Tensor* t : {&q, &k, &v}) check_that(t->scalar_type() == at::kBFloat16, "q, k and v are bf16");
+        const float scale = (float)float_arg(a[5]);
+        const bool causal = bool_arg(a[6]), want_lse = bool_arg(a[7]);
+        Tensor o = opt_tensor_arg(a[8], "out"), lse = opt_tensor_arg(a[9], "lse_out");
+        if (o.defined()) check_bf16_like(o, q, "out is a bf16 tensor of q's shape");
+        if (lse.defined()) check_lse(lse, z, q);
+        const Tensor ws = opt_tensor_arg(a[10], "workspace");
+        if (ws.defined()) check_workspace(ws, q);
+        {
+            WithoutGil nogil;
+            c10::OptionalDeviceGuard device(q.device());
+            call_packed_fwd(q, k, v, cu_q, cu_k, z, scale, causal, want_lse, ws, o, lse);
+        }
+        return pair(o, lse);
+    });
+}
+
+// attn_packed_bwd(q, k, v, o, do, lse, cu_q, cu_k, scale, causal, workspace, dq, dk, dv) -> (dq, dk, dv)
+PyObject* py_attn_packed_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        need_args(n, 14);
+        const Tensor &q = tensor_arg(a[0], "q"), &k = tensor_arg(a[1], "k"), &v = tensor_arg(a[2], "v"), &o = tensor_arg(a[3], "o"),
+                     &d_o = tensor_arg(a[4], "do"), &lse = tensor_arg(a[5], "lse"), &cu_q = tensor_arg(a[6], "cu_q"), &cu_k = tensor_arg(a[7], "cu_k");
+        const PackedSizes z = packed_sizes(q, k, v, cu_q, cu_k);
+        for (const Tensor* t : {&q, &k, &v}) check_that(t->scalar_type() == at::kBFloat16, "q, k and v are bf16");
+        check_bf16_like(o, q, "o is a bf16 tensor of q's shape");
+        check_bf16_like(d_o, q, "do is a bf16 tensor of q's shape");
+        check_lse(lse, z, q);
+        const float scale = (float)float_arg(a[8]);
+        const bool causal = bool_arg(a[9]);
+        const Tensor ws = opt_tensor_arg(a[10], "workspace");
+        if (ws.defined()) check_workspace(ws, q);
+        Grads g{opt_tensor_arg(a[11], "dq"), opt_tensor_arg(a[12], "dk"), opt_tensor_arg(a[13], "dv")};
+        if (g.dq.defined()) {
+            check_that(g.dk.defined() && g.dv.defined(), "all three gradients or none");
+            check_bf16_like(g.dq, q, "dq is a bf16 tensor of q's shape");
+            check_bf16_like(g.dk, k, "dk is a bf16 tensor of k's shape");
+            check_bf16_like(g.dv, v, "dv is a bf16 tensor of v's shape");
+        }
+        {
+            WithoutGil nogil;
+            c10::OptionalDeviceGuard device(q.device());
+            check_rc(call_packed_bwd(q, k, v, o, d_o, lse, cu_q, cu_k, z, scale, causal, ws, g), "flame_attn_packed_bwd_bf16");
+        }
+        return triple(g);
+    });
+}
+
+// ---------------------------------------------------------------- paged cache
+// [pages, Hkv, page, D], or with the layers in front for the copies
+void check_caches(const Tensor& kc, const Tensor& vc, int64_t dims, const char* what) {
+    if (kc.dim() != dims || vc.dim() != dims) fail(PyExc_ValueError, what);
+    check_that(kc.sizes() == vc.sizes() && kc.numel() > 0, "the two caches have one shape");
+    check_that(kc.scalar_type() == at::kBFloat16 && vc.scalar_type() == at::kBFloat16, "the caches are bf16");
+    check_device(kc, kc, "the tensors are on a GPU");
+    check_device(vc, kc, "all tensors are on one GPU");
+}
+void check_ints(const Tensor& t, int64_t n, const Tensor& like, const char* what) {
+    check_that(t.dim() == 1 && t.scalar_type() == at::kInt && t.size(0) == n && (n == 1 || t.stride(0) == 1), what);
+    check_device(t, like, "all tensors are on one GPU");
+}
+void check_table(const Tensor& t, int64_t n, const Tensor& like) {
+    check_that(t.dim() == 2 && t.scalar_type() == at::kInt && t.size(0) == n && t.size(1) > 0 && (t.size(1) == 1 || t.stride(1) == 1),
+               "the page table is an int32 [sequences, pages] tensor with contiguous rows");
+    check_device(t, like, "all tensors are on one GPU");
+}
+const int32_t* ints(const Tensor& t) { return static_cast<const int32_t*>(ptr(t)); }
+
+struct PagedCall {
+    Tensor table, kv_len, prefix_table, prefix_len;
+};
+// checks of everything but q's dtype and layout
+void check_paged(const Tensor& q, const Tensor& kc, const Tensor& vc, const PagedCall& c) {
+    check_4d(q);
+    check_caches(kc, vc, 4, "the caches are 4-D [pages, key heads, page, D]");
+    check_device(kc, q, "all tensors are on one GPU");
+    check_that(q.numel() > 0 && q.size(3) == kc.size(3) && q.size(1) % kc.size(1) == 0, "q is [B, H, N, D] with the caches' head dim and a multiple of their heads");
+    check_table(c.table, q.size(0), q);
+    check_ints(c.kv_len, q.size(0), q, "kv_len is an int32 [B] tensor");
+    check_that(c.prefix_table.defined() == c.prefix_len.defined(), "a prefix has a table and a length");
+    if (c.prefix_table.defined()) {
+        check_that(c.prefix_table.numel() > 0, "a prefix has at least one page");
+        check_ints(c.prefix_table, c.prefix_table.numel(), q, "the prefix table is a contiguous int32 [pages] tensor");
+        check_ints(c.prefix_len, 1, q, "prefix_len is an int32 [1] tensor");
+    }
+    for (const Tensor* t : {&q, &kc, &c.table})
+        for (int64_t n : t->sizes()) size32(n);
+    if (c.prefix_table.defined()) size32(c.prefix_table.numel());
+}
+void call_paged(const Tensor& q, const Tensor& kc, const Tensor& vc, const PagedCall& c, float scale, bool want_lse, Tensor workspace, Tensor& o, Tensor& lse) {
+    const int B = (int)q.size(0), H = (int)q.size(1), N = (int)q.size(2), D = (int)q.size(3), Hkv = (int)kc.size(1), page = (int)kc.size(2);
+    const int pages = (int)c.table.size(1), prefix = c.prefix_table.defined() ? (int)c.prefix_table.numel() : 0;
+    if (!o.defined()) o = empty(q.sizes(), at::kBFloat16, q);
+    if (want_lse) lse = empty({(int64_t)B * H, N}, at::kFloat, q);
+    if (!workspace.defined())
+        if (const size_t need = g_api.flame_attn_paged_workspace_bytes(B, H, Hkv, N, D, page, pages, prefix)) workspace = bytes_like(need, q);
+    check_rc(g_api.flame_attn_paged_fwd_bf16(ptr(q), ptr(kc), ptr(vc), ptr(o), ptr(lse), ints(c.table), c.table.stride(0), pages, ints(c.kv_len),
+                                             ints(c.prefix_table), prefix, ints(c.prefix_len), B, H, Hkv, N, D, (int)kc.size(0), page, scale, strides4(q),
+                                             strides4(kc), strides4(vc), strides4(o), ptr(workspace), workspace.defined() ? (size_t)workspace.numel() : 0, stream_of(q)),
+             "flame_attn_paged_fwd_bf16");
+}
+
+// sdpa_paged(q, k_cache, v_cache, page_table, kv_len, prefix_table | None, prefix_len | None, scale | None) -> o
+PyObject* py_sdpa_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        need_args(n, 8);
+        const Tensor &q = tensor_arg(a[0], "q"), &kc = tensor_arg(a[1], "k_cache"), &vc = tensor_arg(a[2], "v_cache");
+        const PagedCall c{tensor_arg(a[3], "page_table"), tensor_arg(a[4], "kv_len"), opt_tensor_arg(a[5], "prefix_table"), opt_tensor_arg(a[6], "prefix_len")};
+        check_paged(q, kc, vc, c);
+        TORCH_CHECK(!at::GradMode::is_enabled() || !(q.requires_grad() || kc.requires_grad() || vc.requires_grad()),
+                    "paged attention has no backward and an input requires a gradient: call it under torch.no_grad()");
+        const float scale = (float)(a[7] == Py_None ? 1.0 / std::sqrt((double)q.size(3)) : float_arg(a[7]));
+        Tensor o, lse;
+        {
+            WithoutGil nogil;
+            c10::OptionalDeviceGuard device(q.device());
+            const at::ScalarType orig = q.scalar_type();
+            call_paged(packed_rows(q), kc, vc, c, scale, false, Tensor(), o, lse);
+            if (orig != at::kBFloat16) o = o.to(orig);
+        }
+        return THPVariable_Wrap(o);
+    });
+}
+
+// attn_paged_fwd(q, k_cache, v_cache, page_table, kv_len, scale, prefix_table, prefix_len, want_lse, out, workspace) -> (o, lse | None)
+PyObject* py_attn_paged_fwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        need_args(n, 11);
+        const Tensor &q = tensor_arg(a[0], "q"), &kc = tensor_arg(a[1], "k_cache"), &vc = tensor_arg(a[2], "v_cache");
+        const PagedCall c{tensor_arg(a[3], "page_table"), tensor_arg(a[4], "kv_len"), opt_tensor_arg(a[6], "prefix_table"), opt_tensor_arg(a[7], "prefix_len")};
+        check_paged(q, kc, vc, c);
+        check_that(q.scalar_type() == at::kBFloat16, "q is bf16");
+        const float scale = (float)float_arg(a[5]);
+        const bool want_lse = bool_arg(a[8]);
+        Tensor o = opt_tensor_arg(a[9], "out"), lse;
+        if (o.defined()) check_bf16_like(o, q, "out is a bf16 tensor of q's shape");
+        const Tensor ws = opt_tensor_arg(a[10], "workspace");
+        if (ws.defined()) check_workspace(ws, q);
+        {
+            WithoutGil nogil;
+            c10::OptionalDeviceGuard device(q.device());
+            call_paged(q, kc, vc, c, scale, want_lse, ws, o, lse);
+        }
+        return pair(o, lse);
+    });
+}
+
+// kv_store(k, v, k_cache, v_cache, page_table, cu, start)
+PyObject* py_kv_store(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        need_args(n, 7);
+        const Tensor &k = tensor_arg(a[0], "k"), &v = tensor_arg(a[1], "v"), &kc = tensor_arg(a[2], "k_cache"), &vc = tensor_arg(a[3], "v_cache"),
+                     &table = tensor_arg(a[4], "page_table"), &cu = tensor_arg(a[5], "cu"), &start = tensor_arg(a[6], "start");
+        if (k.dim() != 3) fail(PyExc_ValueError, "k and v are 3-D [rows, key heads, D]");
+        check_caches(kc, vc, 4, "the caches are 4-D [pages, key heads, page, D]");
+        check_that(k.sizes() == v.sizes() && k.numel() > 0 && k.size(1) == kc.size(1) && k.size(2) == kc.size(3), "k and v have one shape, with the caches' heads and head dim");
+        check_that(k.scalar_type() == at::kBFloat16 && v.scalar_type() == at::kBFloat16, "k and v are bf16");
+        check_device(k, kc, "all tensors are on one GPU");
+        check_device(v, kc, "all tensors are on one GPU");
+        check_bounds(cu, kc);
+        check_table(table, cu.size(0) - 1, kc);
+        check_ints(start, cu.size(0) - 1, kc, "start is an int32 [sequences] tensor");
+        for (const Tensor* t : {&k, &kc, &table})
+            for (int64_t s : t->sizes()) size32(s);
+        {
+            WithoutGil nogil;
+            c10::OptionalDeviceGuard device(kc.device());
+            check_rc(g_api.flame_kv_store_bf16(ptr(k), ptr(v), ptr(kc), ptr(vc), ints(table), table.stride(0), (int)table.size(1), ints(cu), ints(start),
+                                               (int)table.size(0), (int)k.size(0), (int)k.size(1), (int)k.size(2), (int)kc.size(0), (int)kc.size(2), strides4(k),
+                                               strides4(v), strides4(kc), strides4(vc), stream_of(kc)),
+                     "flame_kv_store_bf16");
+        }
+        return Py_NewRef(Py_None);
+    });
+}
+
+std::vector<int32_t> int_list(PyObject* o) {
+    PyObject* seq = PySequence_Fast(o, "src and dst are sequences of page numbers");
+    if (!seq) throw PyErrorSet{};
+    std::vector<int32_t> out;
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(seq);
+    out.reserve((size_t)n);
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        const long v = PyLong_AsLong(PySequence_Fast_GET_ITEM(seq, i));
+        if (PyErr_Occurred() || v < INT32_MIN || v > INT32_MAX) {
+            Py_DECREF(seq);
+            if (!PyErr_Occurred()) PyErr_SetString(PyExc_OverflowError, "a page number exceeds 32 bits");
+            throw PyErrorSet{};
+        }
+        out.push_back((int32_t)v);
+    }
+    Py_DECREF(seq);
+    return out;
+}
+// kv_copy_pages(k_cache, v_cache, src, dst): caches [pages, Hkv, page, D] or [layers, pages, Hkv, page, D]
+PyObject* py_kv_copy_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        need_args(n, 4);
+        Tensor kc = tensor_arg(a[0], "k_cache"), vc = tensor_arg(a[1], "v_cache");
+        if (kc.dim() == 4 && vc.dim() == 4) kc = kc.unsqueeze(0), vc = vc.unsqueeze(0);
+        check_caches(kc, vc, 5, "the caches are [pages, key heads, page, D], with the layers in front or without");
+        const std::vector<int32_t> src = int_list(a[2]), dst = int_list(a[3]);
+        check_that(src.size() == dst.size(), "as many sources as destinations");
+        size32((int64_t)src.size());
+        for (int64_t s : kc.sizes()) size32(s);
+        {
+            WithoutGil nogil;
+            c10::OptionalDeviceGuard device(kc.device());
+            check_rc(g_api.flame_kv_copy_pages_bf16(ptr(kc), ptr(vc), (int)kc.size(0), (int)kc.size(1), (int)kc.size(2), (int)kc.size(3), (int)kc.size(4),
+                                                    strides4(kc), strides4(vc), src.data(), dst.data(), (int)src.size(), stream_of(kc)),
+                     "flame_kv_copy_pages_bf16");
+        }
+        return Py_NewRef(Py_None);
+    });
+}
+
 // bind(dlopen handle of the library, the exception class)
 PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
@@ -788,6 +1160,13 @@ PyMethodDef g_methods[] = {FLAME_HOST_METHOD("bind", py_bind),
                            FLAME_HOST_METHOD("sage_fwd", py_sage_fwd),
                            FLAME_HOST_METHOD("prep_rmsnorm_rope", py_prep),
                            FLAME_HOST_METHOD("fp8", py_fp8),
+                           FLAME_HOST_METHOD("sdpa_packed", py_sdpa_packed),
+                           FLAME_HOST_METHOD("sdpa_paged", py_sdpa_paged),
+                           FLAME_HOST_METHOD("attn_paged_fwd", py_attn_paged_fwd),
+                           FLAME_HOST_METHOD("kv_store", py_kv_store),
+                           FLAME_HOST_METHOD("kv_copy_pages", py_kv_copy_pages),
+                           FLAME_HOST_METHOD("attn_packed_fwd", py_attn_packed_fwd),
+                           FLAME_HOST_METHOD("attn_packed_bwd", py_attn_packed_bwd),
                            {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_flame_torch_host", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -35,3 +35,28 @@ def sdpa_with_bias(q, k, v, bias=None, scale=None):
     if bias is None:
         return sdpa(q, k, v, scale=scale)
     return capi.host().sdpa_with_bias(q, k, v, bias, scale)
+
+
+def sdpa_packed(q, k, v, cu_seqlens, cu_seqlens_k=None, is_causal=None, scale=None):
+    """Attention of sequences of different lengths packed one behind the other: q [rows, H, D], k/v [key rows, H_kv, D],
+    H a multiple of H_kv (head h reads key head h // (H // H_kv)).  Differentiable.
+
+    cu_seqlens (and cu_seqlens_k where the keys have other lengths): int32 [sequences + 1] on the device, the rows of
+    sequence i being cu_seqlens[i] .. cu_seqlens[i + 1] - 1; a recorded graph holds them, so they may not be refilled before
+    its backward.  is_causal=True: query i of a sequence attends to keys j <= i + (keys - queries), the last query to
+    all of them.  Queries without a key and rows behind the last sequence come out as zeros, with zero gradients.
+    Inputs of another dtype are promoted to bf16 and the result is cast back.
+    Its backward may be captured into a graph; a leaf that an eager graph recorded on another stream still holds is refused
+    in the capture."""
+    return capi.host().sdpa_packed(q, k, v, cu_seqlens, cu_seqlens_k, is_causal is not None and bool(is_causal), scale)
+
+
+def sdpa_paged(q, k_cache, v_cache, page_table, kv_len, prefix_table=None, prefix_len=None, scale=None):
+    """Attention of the last N tokens of every sequence, q [B, H, N, D], against a paged cache, bf16 [pages, H_kv, page, D]
+    (inference only; flame_amd.paged_cache keeps such a cache).
+
+    page_table: int32 [B, pages], the pages of a sequence's own keys in their order; kv_len: int32 [B], how many own keys,
+    the N new ones among them.  prefix_table (int32 [pages]) and prefix_len (int32 [1]): keys that all sequences have in
+    front of their own, read once for the batch.  Token i attends to the prefix and to own keys j <= kv_len - N + i.
+    q of another dtype is promoted to bf16 and the result is cast back."""
+    return capi.host().sdpa_paged(q, k_cache, v_cache, page_table, kv_len, prefix_table, prefix_len, scale)

@@ -230,6 +230,91 @@ int flame_attn_bwd_bf16_noalloc(const void* Q, const void* K, const void* V, con
                                 const uint8_t* keep_mask, const int64_t* mask_strides, void* stream);
 
 /* ------------------------------------------------------------------------------------------------
+ * Packed sequences: n_seqs sequences of different lengths one behind the other in [rows, heads, D] tensors, without padding.
+ * No counterpart in the reference, whose batches are padded to one length.
+ *   - Q, O [T_q, H, D], K, V [T_kv, H_kv, D], bf16; H a multiple of H_kv, head h reads key head h / (H / H_kv).  Strides: three
+ *     ELEMENT strides in (row, head, D) order under the rules of the [B,H,N,D] views above (D stride 1, the others multiples of 8,
+ *     row strides below 2^24, 16-byte aligned base); D any multiple of 8 up to 128.  Rows or heads of an output must not overlap.
+ *   - cu_q, cu_k: int32 [n_seqs + 1] on the device; sequence i has the query rows cu_q[i] .. cu_q[i + 1] - 1 and the key rows
+ *     cu_k[i] .. cu_k[i + 1] - 1.  They rise from 0 and end at or before T_q / T_kv; a sequence may have no rows.  (They are read on
+ *     the device and cannot be refused: values that fall or lead outside are cut to the tensors, and the result is of no use.)
+ *   - causal: query i of a sequence attends to its keys j <= i + (keys - queries), i.e. the last query to all of them.  A query
+ *     without a key has O = 0, LSE = -inf and a zero gradient.
+ *   - Rows behind the last sequence: O, dQ, dK and dV are 0 there, LSE is -inf; their values in the inputs are not used.
+ *   - An excluded key's V enters its tile's products with the weight 0: infinities and NaN in V rows of the same sequence reach
+ *     the queries of their 64-key tile that do not attend to them, as in the other causal calls.  Rows of other sequences and
+ *     rows behind the last one are never read into a sequence's tiles.
+ *   - LSE: fp32, contiguous [H, T_q], otherwise as above; may be null in the forward.
+ * The results do not depend on the order in which workgroups finish.
+ * ---------------------------------------------------------------------------------------------- */
+/* `workspace` (device memory, 16-byte aligned, used only during the call; null or too small is accepted): where the tiles of the
+ * queries leave compute units idle, their walks over the keys are cut into parts that leave fp32 partial sums there.  0 bytes
+ * where that would not be faster.  Calls that overlap (other streams, captured graphs that run at once) need one each. */
+size_t flame_attn_packed_fwd_workspace_bytes(int n_seqs, int T_q, int T_kv, int H, int D);
+int flame_attn_packed_fwd_bf16(const void* Q, const void* K, const void* V, void* O, void* LSE, const int32_t* cu_q,
+                               const int32_t* cu_k, int n_seqs, int T_q, int T_kv, int H, int H_kv, int D, float scale,
+                               const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
+                               const int64_t* o_strides, int causal, void* workspace, size_t workspace_bytes, void* stream);
+/* Recommended bytes of device scratch for the backward (16-byte aligned, used only during the call): two fp32 values per query
+ * row and head (required), and the partial sums of walks in parts (optional, as in the forward). */
+size_t flame_attn_packed_bwd_workspace_bytes(int n_seqs, int T_q, int T_kv, int H, int H_kv, int D);
+/* dQ [T_q, H, D], dK, dV [T_kv, H_kv, D] from the saved O and LSE; dK and dV are summed over the heads that share a key head, in
+ * fp32 within one workgroup. */
+int flame_attn_packed_bwd_bf16(const void* Q, const void* K, const void* V, const void* O, const void* dO, const void* LSE,
+                               void* dQ, void* dK, void* dV, const int32_t* cu_q, const int32_t* cu_k, int n_seqs, int T_q,
+                               int T_kv, int H, int H_kv, int D, float scale, const int64_t* q_strides,
+                               const int64_t* k_strides, const int64_t* v_strides, const int64_t* o_strides,
+                               const int64_t* do_strides, const int64_t* dq_strides, const int64_t* dk_strides,
+                               const int64_t* dv_strides, int causal, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * A paged cache of keys and values: attention of one or a few new tokens per sequence, stores into the pages, page copies.
+ * No counterpart in the reference, which keeps no keys between calls.
+ *   - The caches are bf16 [n_pages, H_kv, page, D] tensors through four ELEMENT strides in (page, head, token, D) order, the rules
+ *     those of the [B,H,N,D] views above; `page`, the tokens of a page, is a power of two from 16 to 65536.
+ *   - page_table: int32 on the device, row b (table_stride elements apart, table_pages entries) lists the pages of sequence b in
+ *     the order of its tokens: token t lies on page page_table[b][t / page], place t % page.
+ *   - Lengths and page numbers are read on the device and cannot be refused.  Nothing outside the caches and tables is read or
+ *     written whatever they say: in the attention a page number outside [0, n_pages) or a length past the table makes every row
+ *     that would read there NaN; a store to such a place is left out.  Negative lengths count as 0.  Entries behind a
+ *     sequence's last token, and what a page holds behind it, are not used.
+ * ---------------------------------------------------------------------------------------------- */
+
+/* O [B,H,N,D] = attention of the last N tokens of every sequence (N = 1: one new token; more: drafted tokens) to the keys that all
+ * sequences share, then their own: softmax over both.  The shared prefix has prefix_len[0] tokens (one int32 on the device) on the pages
+ * prefix_table[0 .. prefix_pages - 1] and is read once for the batch; null, null and 0 pages: none.  kv_len [B]: the keys of a sequence's own pages,
+ * its N new tokens among them (stored before the call).  Token i of the N attends to the whole prefix and to own keys
+ * j <= kv_len[b] - N + i.  A row without a key has O = 0 and LSE = -inf.  H a multiple of H_kv: head h reads key head
+ * h / (H / H_kv).  D any multiple of 8 up to 128.  LSE: fp32, contiguous [B*H, N], or null.
+ * `workspace`: device memory, 16-byte aligned, of at least flame_attn_paged_workspace_bytes(...) bytes (0: none is needed, or the
+ * call would be refused), used only during the call; nothing in it has to start at any value.  Calls that overlap (other streams,
+ * captured graphs that run at once) need one each.
+ * The results do not depend on the order in which workgroups finish.  Inference only. */
+size_t flame_attn_paged_workspace_bytes(int B, int H, int H_kv, int N, int D, int page, int table_pages, int prefix_pages);
+int flame_attn_paged_fwd_bf16(const void* Q, const void* K_cache, const void* V_cache, void* O, void* LSE,
+                              const int32_t* page_table, int64_t table_stride, int table_pages, const int32_t* kv_len,
+                              const int32_t* prefix_table, int prefix_pages, const int32_t* prefix_len, int B, int H, int H_kv,
+                              int N, int D, int n_pages, int page, float scale, const int64_t* q_strides,
+                              const int64_t* k_strides, const int64_t* v_strides, const int64_t* o_strides, void* workspace,
+                              size_t workspace_bytes, void* stream);
+
+/* Rows K, V [T, H_kv, D] (three element strides in (row, head, D) order) of n_seqs sequences, sequence b having the rows
+ * cu[b] .. cu[b + 1] - 1 (int32 [n_seqs + 1] on the device, rising from 0), to the places start[b], start[b] + 1, ... of their pages.
+ * Rows behind the last sequence are not stored.  Two rows for one place leave either of them.  D any multiple of 8. */
+int flame_kv_store_bf16(const void* K, const void* V, void* K_cache, void* V_cache, const int32_t* page_table,
+                        int64_t table_stride, int table_pages, const int32_t* cu, const int32_t* start, int n_seqs, int T, int H_kv,
+                        int D, int n_pages, int page, const int64_t* k_strides, const int64_t* v_strides,
+                        const int64_t* kc_strides, const int64_t* vc_strides, void* stream);
+
+/* Copies page src[i] to page dst[i], i < n, in every layer of both caches [layers, n_pages, H_kv, page, D] (five element strides;
+ * here `page` is any number).  src and dst are HOST arrays, read before the call returns and, in a captured graph, kept by value.
+ * A number outside the cache, a page that is written twice, or one that is both read and written, is FLAME_ATTN_ERR_INVALID and
+ * nothing is copied.  One launch for every 400 pairs. */
+int flame_kv_copy_pages_bf16(void* K_cache, void* V_cache, int layers, int n_pages, int H_kv, int page, int D,
+                             const int64_t* k_strides, const int64_t* v_strides, const int32_t* src, const int32_t* dst, int n,
+                             void* stream);
+
+/* ------------------------------------------------------------------------------------------------
  * The materialised path: every shape the fused kernels refuse.  Any head dim D >= 1 (no multiple-of-8 rule, no
  * upper limit, D stride 1 and non-negative strides as the only layout rules), a value head dim Dv of its own,
  * causal flag, key lengths, keep-mask and (forward) additive bias as in the primary entry points, and the

@@ -45,23 +45,27 @@ fn main() {
         .map(|s| s.trim().to_string())
         .unwrap_or_else(|| "?".to_string());
 
-    let obj = out.join("flame_attn.o");
-    let mut cc = Command::new(&hipcc);
-    cc.args(["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC"])
-        // packed fp32 vector operations stay off for every HIP source of this library
-        .args(["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"])
-        .args(["-Wall", "-Wno-unused-function", "-Wno-inline-asm"])
-        .arg(format!("-DFLAME_ATTN_HIPCC_VERSION=\"{hip} (cargo)\""))
-        .arg("-c")
-        .arg(csrc.join("flame_attn.hip"))
-        .arg("-o")
-        .arg(&obj);
-    run(&mut cc, "hipcc flame_attn.hip");
+    let mut objects = Vec::new();
+    for name in ["flame_attn", "flame_packed", "flame_paged"] {
+        let obj = out.join(format!("{name}.o"));
+        let mut cc = Command::new(&hipcc);
+        cc.args(["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC"])
+            // packed fp32 vector operations stay off for every HIP source of this library
+            .args(["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"])
+            .args(["-Wall", "-Wno-unused-function", "-Wno-inline-asm"])
+            .arg(format!("-DFLAME_ATTN_HIPCC_VERSION=\"{hip} (cargo)\""))
+            .arg("-c")
+            .arg(csrc.join(format!("{name}.hip")))
+            .arg("-o")
+            .arg(&obj);
+        run(&mut cc, name);
+        objects.push(obj);
+    }
 
     let lib = out.join("libflame_attn_hip.a");
     let _ = std::fs::remove_file(&lib);
     let mut ar = Command::new("ar");
-    ar.arg("rcs").arg(&lib).arg(&obj);
+    ar.arg("rcs").arg(&lib).args(&objects);
     run(&mut ar, "ar");
 
     println!("cargo:rustc-link-search=native={}", out.display());

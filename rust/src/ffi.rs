@@ -168,6 +168,47 @@ extern "C" {
         dq_off: i64, dk_off: i64, dv_off: i64, causal: c_int, kv_len: *const i32, keep_mask: *const u8,
         mask_strides: *const i64, stream: *mut c_void
     ) -> c_int;
+    pub fn flame_attn_packed_fwd_bf16(
+        q: *const c_void, k: *const c_void, v: *const c_void, o: *mut c_void, lse: *mut c_void, cu_q: *const i32,
+        cu_k: *const i32, n_seqs: c_int, t_q: c_int, t_kv: c_int, h: c_int, h_kv: c_int, d: c_int, scale: f32,
+        q_strides: *const i64, k_strides: *const i64, v_strides: *const i64, o_strides: *const i64, causal: c_int,
+        workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void
+    ) -> c_int;
+    pub fn flame_attn_packed_fwd_workspace_bytes(
+        n_seqs: c_int, t_q: c_int, t_kv: c_int, h: c_int, d: c_int
+    ) -> usize;
+    pub fn flame_attn_packed_bwd_workspace_bytes(
+        n_seqs: c_int, t_q: c_int, t_kv: c_int, h: c_int, h_kv: c_int, d: c_int
+    ) -> usize;
+    pub fn flame_attn_packed_bwd_bf16(
+        q: *const c_void, k: *const c_void, v: *const c_void, o: *const c_void, d_o: *const c_void,
+        lse: *const c_void, dq: *mut c_void, dk: *mut c_void, dv: *mut c_void, cu_q: *const i32, cu_k: *const i32,
+        n_seqs: c_int, t_q: c_int, t_kv: c_int, h: c_int, h_kv: c_int, d: c_int, scale: f32, q_strides: *const i64,
+        k_strides: *const i64, v_strides: *const i64, o_strides: *const i64, do_strides: *const i64,
+        dq_strides: *const i64, dk_strides: *const i64, dv_strides: *const i64, causal: c_int,
+        workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void
+    ) -> c_int;
+    pub fn flame_attn_paged_workspace_bytes(
+        b: c_int, h: c_int, h_kv: c_int, n: c_int, d: c_int, page: c_int, table_pages: c_int, prefix_pages: c_int
+    ) -> usize;
+    pub fn flame_attn_paged_fwd_bf16(
+        q: *const c_void, k_cache: *const c_void, v_cache: *const c_void, o: *mut c_void, lse: *mut c_void,
+        page_table: *const i32, table_stride: i64, table_pages: c_int, kv_len: *const i32, prefix_table: *const i32,
+        prefix_pages: c_int, prefix_len: *const i32, b: c_int, h: c_int, h_kv: c_int, n: c_int, d: c_int,
+        n_pages: c_int, page: c_int, scale: f32, q_strides: *const i64, k_strides: *const i64, v_strides: *const i64,
+        o_strides: *const i64, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void
+    ) -> c_int;
+    pub fn flame_kv_store_bf16(
+        k: *const c_void, v: *const c_void, k_cache: *mut c_void, v_cache: *mut c_void, page_table: *const i32,
+        table_stride: i64, table_pages: c_int, cu: *const i32, start: *const i32, n_seqs: c_int, t: c_int,
+        h_kv: c_int, d: c_int, n_pages: c_int, page: c_int, k_strides: *const i64, v_strides: *const i64,
+        kc_strides: *const i64, vc_strides: *const i64, stream: *mut c_void
+    ) -> c_int;
+    pub fn flame_kv_copy_pages_bf16(
+        k_cache: *mut c_void, v_cache: *mut c_void, layers: c_int, n_pages: c_int, h_kv: c_int, page: c_int,
+        d: c_int, k_strides: *const i64, v_strides: *const i64, src: *const i32, dst: *const i32, n: c_int,
+        stream: *mut c_void
+    ) -> c_int;
     pub fn flame_attn_materialised_workspace_bytes(
         b: c_int, h: c_int, n_q: c_int, n_kv: c_int, d: c_int, dv: c_int, backward: c_int
     ) -> usize;
