@@ -59,9 +59,15 @@ size_t align256(size_t x) { return (x + 255) / 256 * 256; }
 
 // log2 of what the card holds of a kernel's workgroups, two per compute unit or one
 constexpr int kRoomQueries = 9, kRoomKeys = 8;
-// Whether the walks of a problem's tiles are cut into parts: not where whole walks fill the card, nor where the mean one is short.
-bool parts_pay(int64_t slots, int heads, int n_seqs, int walked_rows, int room_log2) {
-    return n_seqs <= 64 && walked_rows / n_seqs >= 1024 && slots * heads * 2 < 3 << room_log2;
+// Whether a problem gets room for walks in parts, which the device then cuts or not by the lengths (PackedCut): not where whole walks fill the
+// 256 compute units one and a half times, nor where the mean walk is short, nor where no lengths of these sums would be cut (the fewest
+// steps: a causal self-attention's).
+// (Whole -> in parts, us.  Forward: D = 128, 8 heads of 2000 34.8 -> 28.4, 4 of 8192 117 -> 89, 32 of 128 rows on 8192 keys 115 -> 33; D = 64, 2 of
+// 4096 41 -> 21.  Backward, two heads to a key head and more: 8 of 2000 207 -> 94, 4 of 8192 439 -> 267.  Left whole: 24 heads of 1200 24.7 (in parts 30.7),
+// backward 68 (86); D = 64, 12 heads of twice 2000 25.8 (34).)
+bool parts_pay(int64_t slots, int heads, int n_seqs, int walked_rows) {
+    if (n_seqs > 64 || walked_rows / n_seqs < 1024 || slots * heads * 2 >= 3 << PackedCut::kUnits_log2) return false;
+    return PackedCut::pays((walked_rows + 63) / 64, (slots - n_seqs) * heads * (walked_rows / n_seqs / 128));
 }
 
 struct Parts {
@@ -72,7 +78,7 @@ struct Parts {
 Parts parts_of(int tile_rows, int walked_rows, int n_seqs, int heads, int room_log2, size_t unit_bytes) {
     Parts z{packed_slots(tile_rows, n_seqs, 128), 0, 0, 0};
     z.units = z.slots;
-    if (parts_pay(z.slots, heads, n_seqs, walked_rows, room_log2)) {
+    if (parts_pay(z.slots, heads, n_seqs, walked_rows)) {
         z.room_log2 = room_log2;
         z.units = PackedCut::most(z.slots, heads, room_log2);
         z.bytes = align256((size_t)z.units * heads * unit_bytes);

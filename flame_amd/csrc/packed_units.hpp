@@ -48,16 +48,20 @@ struct PackedArgs {
 
 inline int64_t packed_slots(int total, int n, int tile) { return (int64_t)total / tile + n + 1; }
 
-// The walks of all tiles together have `steps` steps; a part has as many as gives 1 << room_log2 parts, but not so few that it spends its time
-// on loading its rows and leaving its sums.
+// How walks are cut.  The walks of all `units` tiles together have `steps` steps; the parts are to fill the 1 << room_log2 workgroups that
+// the card holds at once, of which the last part of every tile takes half a place on average.  A part has not so few steps that it spends its
+// time on loading its rows and leaving its sums, and nothing is cut where the longest walk is hardly longer than what each of the
+// 256 compute units has to do anyway: joining the parts costs about kGain steps.
 struct PackedCut {
-    static constexpr int kLeast = 8;
-    static __host__ __device__ int share(int64_t steps, int room_log2) {
-        const int64_t n = (steps + (1 << room_log2) - 1) >> room_log2;
-        return n < kLeast ? kLeast : n > (1 << 30) ? 1 << 30 : (int)n;
+    static constexpr int kLeast = 16, kGain = 16, kUnits_log2 = 8, kWhole = 1 << 30;
+    static __host__ __device__ bool pays(int longest, int64_t steps) { return longest - (int)(steps >> kUnits_log2) > kGain; }
+    static __host__ __device__ int share(int64_t steps, int units, int room_log2) {
+        const int room = 1 << room_log2, places = room - units / 2 > room / 4 ? room - units / 2 : room / 4;
+        const float n = (float)steps / (float)places;
+        return n < (float)kLeast ? kLeast : n > 1e9f ? 1000000000 : (int)n + 1;
     }
-    // units per head, at most, of `slots` tiles: a sequence's longest walk is at most twice the mean that `steps` counts
-    static int64_t most(int64_t slots, int heads, int room_log2) { return slots + ((2 << room_log2) + heads - 1) / heads; }
+    // units per head, at most, of `slots` tiles: a sequence's longest walk is at most twice the mean that `steps` counts (one more for the rounding of `n`)
+    static int64_t most(int64_t slots, int heads, int room_log2) { return slots + ((2 << room_log2) + heads - 1) / heads + 1; }
 };
 
 enum PackedWork : int { kPackedIdle = 0, kPackedTile = 1, kPackedBehind = 2 };
@@ -135,18 +139,22 @@ __device__ __forceinline__ PackedWork packed_unit(const PackedArgs& a, int block
         const int end = packed_uniform(packed_bound(cu, a.n, total));
         const int tiles = ((KEYS ? Sk : Sq) + TILE - 1) / TILE;
         const int walk = ((KEYS ? Sq : Sk) + STEP - 1) / STEP * (KEYS ? rep : 1);
-        int parts = 1, share = 1 << 30;
+        int parts = 1, share = PackedCut::kWhole;
         if (a.room_log2) {
             // steps of the batch, every sequence's by its mean walk (the causal flag leaves its first tiles little): at least half the longest
             const float cut = a.causal ? 0.5f * (float)min(Sq, Sk) / (float)max(max(Sq, Sk), 1) : 0.f;
             const int64_t mine = (int64_t)tiles * max((walk + 1) / 2, (int)((float)walk * (1.0f - cut)));
             const int low = __builtin_amdgcn_readlane(wave_scan((int)(mine & 0xffffff)), 63), high = __builtin_amdgcn_readlane(wave_scan((int)(mine >> 24)), 63);
-            share = PackedCut::share((((int64_t)high << 24) + low) * heads, a.room_log2);
+            const int64_t steps = (((int64_t)high << 24) + low) * heads;
+            int longest = 0;
+            for (int j = 0; j < a.n; ++j) longest = max(longest, __builtin_amdgcn_readlane(walk, j));
+            if (PackedCut::pays(longest, steps)) share = packed_uniform(PackedCut::share(steps, __builtin_amdgcn_readlane(wave_scan(tiles), 63) * heads, a.room_log2));
             parts = max((walk + share - 1) / share, 1);
         }
+        if (MERGE && share == PackedCut::kWhole) return kPackedIdle;
         const int units = tiles * parts;
         int i, at;                 // the lane that has the unit, and the slots before the lane's (whole walks under the causal flag: t itself)
-        if (a.causal && !a.room_log2) {
+        if (a.causal && share == PackedCut::kWhole) {
             // Every tile of a sequence walks one step of TILE rows less than the one before it, so the t-th of a sequence has the
             // level `longest` - t, and the tiles of all sequences come in the order of falling levels, those of one level by lanes.
             // The level of a slot is found by halving: fewer than slot + 1 tiles lie above it.

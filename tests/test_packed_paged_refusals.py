@@ -71,8 +71,10 @@ def cut(lens_tile, lens_walk, heads, rep, causal, room_log2):
         tiles, walk = -(-t // 128), -(-w // 64) * rep
         less = 0.5 * min(t, w) / max(t, w, 1) if causal else 0.0
         rows.append((tiles, walk, max((walk + 1) // 2, int(walk * (1 - less) + 1e-3))))
-    steps = sum(t * m for t, _, m in rows) * heads
-    share = max(8, -(-steps // (1 << room_log2)))
+    steps, units, room = sum(t * m for t, _, m in rows) * heads, sum(t for t, _, _ in rows) * heads, 1 << room_log2
+    if max(w for _, w, _ in rows) - steps // 256 <= 16:
+        return sum(t for t, _, _ in rows)
+    share = max(16, int(steps / max(room - units // 2, room // 4)) + 1)
     return sum(t * max(1, -(-w // share)) for t, w, _ in rows)
 
 
@@ -89,7 +91,8 @@ def test_workspaces_hold_every_part(lib, lens_q, lens_k, H, Hkv, causal):
     more = lib.flame_attn_packed_bwd_workspace_bytes(n, Tq, Tk, H, Hkv, D) - 2 * -(-H * Tq * 4 // 256) * 256
     assert more >= 0
     slots = Tk // 128 + n + 1
-    if Tq * (H // Hkv) >= 1024 and slots * Hkv * 2 < 3 * 256:
+    walked = Tq * (H // Hkv)
+    if walked // n >= 1024 and slots * Hkv * 2 < 3 * 256 and -(-walked // 64) - (slots - n) * Hkv * (walked // n // 128) // 256 > 16:
         assert more >= cut(lens_k, lens_q, Hkv, H // Hkv, causal, 8) * Hkv * 2 * 128 * D * 4
 
 
