@@ -259,7 +259,7 @@ int flame_attn_packed_fwd_bf16(const void* Q, const void* K, const void* V, void
  * row and head (required), and the partial sums of walks in parts (optional, as in the forward). */
 size_t flame_attn_packed_bwd_workspace_bytes(int n_seqs, int T_q, int T_kv, int H, int H_kv, int D);
 /* dQ [T_q, H, D], dK, dV [T_kv, H_kv, D] from the saved O and LSE; dK and dV are summed over the heads that share a key head, in
- * fp32 within one workgroup. */
+ * fp32 and always in the same order. */
 int flame_attn_packed_bwd_bf16(const void* Q, const void* K, const void* V, const void* O, const void* dO, const void* LSE,
                                void* dQ, void* dK, void* dV, const int32_t* cu_q, const int32_t* cu_k, int n_seqs, int T_q,
                                int T_kv, int H, int H_kv, int D, float scale, const int64_t* q_strides,

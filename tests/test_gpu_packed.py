@@ -131,6 +131,26 @@ def test_many_sequences(n):
     run(n, lens, lens, 2, 1, 64, True)
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("lens,H,Hkv", [([100, 70, 130], 4, 2), ([1500, 40, 1700], 2, 1), ([3] * 40 + [20, 33] + [5] * 40, 4, 4)])
+def test_neighbours_stay_apart(lens, H, Hkv, value, causal):
+    """Infinities and NaN all over one sequence leave the others' results, to the bit, as they are without them."""
+    from flame_amd import capi
+    mid = len(lens) // 2
+    lo, hi = sum(lens[:mid]), sum(lens[:mid + 1])
+    q, k, v, do, cq, _ = (t.cuda() for t in make(5, lens, lens, H, Hkv, 128))
+    got = []
+    for _ in range(2):
+        o, lse = capi.attn_packed_fwd(q, k, v, cq, cq, 0.1, causal=causal)
+        grads = capi.attn_packed_bwd(q, k, v, o, do, lse, cq, cq, 0.1, causal=causal)
+        got.append([torch.cat([t[:lo], t[hi:]]) for t in (o, lse.t(), *grads)])
+        for t in (q, k, v, do):
+            t[lo:hi] = value
+    for a, b in zip(*got):
+        assert torch.equal(a, b) and torch.isfinite(a).all()
+
+
 def test_long_sequence():
     run(77, [2500, 40], [2500, 40], 8, 2, 128, True)
 
