@@ -12,7 +12,10 @@
 // copies; two workgroups per compute unit.  A wavefront owns one K and one V tile of 32 keys in LDS and requests the next K tile as
 // soon as the fragments of the present one are in registers, V likewise, so that one of the two is always on its way.
 // What bounds the prefix of a large batch is the way from L2: read by every 32 rows for themselves (as the own keys are) it moved at
-// 13 TB/s and no faster.  So there the four wavefronts have 32 rows each and share the tiles, of which four are in LDS.
+// 13 TB/s and no faster.  So there the four wavefronts have 32 rows each and share the tiles, of which four are in LDS; what is left is
+// the issue of one wavefront per SIMD, 0.75 us a tile.
+// Measured, D = 128, 32 heads on 8: 64 sequences of 4000 keys 189 us, 5.5 TB/s, 256 of 4000 700 us, 6.0 TB/s, one of 131072 104 us, 5.2 TB/s, 8 of 32000
+// 187 us, 5.6 TB/s; 64 of 1 to 509 keys on a prefix of 8192 38.5 us.  (Reads alone reach 5.7 TB/s on this card, more from its last level of cache.)
 //
 // The number of keys is known on the device only.  The units are therefore cut there: every workgroup sums the tiles of the batch
 // and takes the unit length that gives about as many units as the device holds workgroups.
@@ -48,20 +51,35 @@ struct PagedParams {
     int2* plan;                    // [B] first unit and units per (head, row tile) of a sequence, then the splits of the prefix
 };
 
-// How the keys are cut.  A unit of fewer tiles than kLeast would leave wavefronts without work; up to kFill units run at once (two
-// per compute unit), and beyond kLong tiles per unit there are more, shorter units, so that sequences of different lengths level out.
-// The prefix: kShared units, at least kSharedLeast tiles each (the partial results of a unit's 128 rows weigh as much as two tiles).
+// How the keys are cut.  A walk (one sequence, key head and tile of rows, or the prefix in place of the sequence) has a tile for every 32 keys; a
+// unit of fewer than kLeast tiles would leave wavefronts without work.
+//   Fewer walks than half of the kFill workgroups that run at once: units so long that all of them run at once, the last one of every walk
+//   taking a place whatever is left for it.  (Against units of 32 tiles, some to a second round, us: 8 sequences of 16k to 40k keys,
+//   4 key heads, D = 128 105 -> 97; 16 of 500 to 5000, 8 key heads 46 -> 40.)
+//   More: whole walks up to kLong tiles, as a unit's start costs what about ten tiles do; longer ones in even units, kMany in all.
+//   (64 sequences of 2000 101 -> 97, 256 of 400 to 4000 439 -> 402, 64 of 1600 to 16000 416 -> 404; 48 of 1500 to 3000 91 -> 104.)
+// The prefix of more than 64 rows has units of 128 rows, up to kShared of them, with at least kSharedMost tiles each once there are half as
+// many: the partial results of a unit's rows weigh as much as two tiles.  (One key head with 512 rows on 4096 keys, D = 64, at kSharedMost
+// tiles throughout 21.8 us, so 16.5.  Rows or keys apart, 8 key heads, prefix of 8192: 96 rows each 29.5 and 35.2 us, 48 rows 28.2 and 24.8.)
 struct PagedCut {
-    static constexpr int kTile = 32, kLeast = 4, kFill = 512, kLong = 32, kMost = 2048, kShared = 256, kSharedLeast = 16;
-    // tiles per unit for `total` tiles of all rows
-    static __host__ __device__ int unit(int total) {
-        const int one_round = (total + kFill - 1) / kFill, more = (total + kMost - 1) / kMost;
-        const int n = one_round < kLong ? one_round : more > kLong ? more : kLong;
-        return n < kLeast ? kLeast : (n + kLeast - 1) / kLeast * kLeast;       // (no tiles: a divisor all the same)
+    static constexpr int kTile = 32, kLeast = 4, kFill = 512, kMany = 2048, kLong = 64, kShared = 256, kSharedMost = 16;
+    // tiles per unit for `total` tiles of `walks` walks
+    static __host__ __device__ int places(int walks) { return walks < kFill / 2 ? kFill - walks : walks < kMany - kFill / 2 ? kMany - walks : kFill / 2; }
+    static __host__ __device__ int least(int walks) { return walks < kFill / 2 ? kLeast : kLong; }
+    static __host__ __device__ int unit(int total, int walks) {
+        const int n = (total + places(walks) - 1) / places(walks);
+        return n < least(walks) ? least(walks) : (n + kLeast - 1) / kLeast * kLeast;       // (no tiles: a divisor all the same)
     }
+    // tiles per unit of a walk of `tiles` tiles, at most `unit`, and how many units that makes
+    static __host__ __device__ int even(int tiles, int unit, int walks) {
+        if (walks < kFill / 2 || tiles <= unit) return unit;
+        const int n = (tiles + unit - 1) / unit, each = (tiles + n - 1) / n;
+        return (each + kLeast - 1) / kLeast * kLeast;
+    }
+    static __host__ __device__ int splits(int tiles, int unit, int walks) { return (tiles + even(tiles, unit, walks) - 1) / even(tiles, unit, walks); }
     static __host__ __device__ int shared_unit(int total) {
-        const int n = (total + kShared - 1) / kShared;
-        return n < kSharedLeast ? kSharedLeast : n;
+        const int n = (total + kShared - 1) / kShared, half = 2 * n < kSharedMost ? 2 * n : kSharedMost;
+        return n > half ? n : half < kLeast ? kLeast : half;
     }
     // rows of a prefix unit: of up to 64 rows the wavefronts take the keys apart, not the rows
     static __host__ __device__ bool shared(int rows) { return rows > 64; }
@@ -125,11 +143,11 @@ __device__ __forceinline__ PagedPlan paged_plan(const PagedParams& p, int* sums)
     if (lane == 63) sums[wave] = tiles;
     __syncthreads();
     const int rows = p.N * (p.H / p.Hkv);
-    const int own = packed_uniform(sums[0] + sums[1] + sums[2] + sums[3]) * p.Hkv * PagedCut::row_tiles(rows);
-    c.own_unit = PagedCut::unit(own);
+    const int heads = p.Hkv * PagedCut::row_tiles(rows), own = packed_uniform(sums[0] + sums[1] + sums[2] + sums[3]) * heads;
+    c.own_unit = packed_uniform(PagedCut::unit(own, p.B * heads));
     c.prefix_tiles = paged_tiles(c.prefix_keys);
     const int all = p.B * rows, per_split = p.Hkv * PagedCut::prefix_row_tiles(all), total = c.prefix_tiles * per_split;
-    c.prefix_unit = PagedCut::shared(all) ? PagedCut::shared_unit(total) : PagedCut::unit(total);
+    c.prefix_unit = PagedCut::shared(all) ? PagedCut::shared_unit(total) : PagedCut::unit(total, per_split);
     c.prefix_splits = packed_uniform((c.prefix_tiles + c.prefix_unit - 1) / c.prefix_unit);
     c.prefix_units = c.prefix_splits * per_split;
     return c;
@@ -145,7 +163,7 @@ __device__ __forceinline__ void paged_own_units(const PagedParams& p, const Page
     for (int b0 = 0; b0 < p.B; b0 += 256) {
         const int b = b0 + tid;
         const int len = b0 == 0 ? c.len : b < p.B ? p.kv_len[b] : 0;
-        const int splits = (paged_tiles(min(max(len, 0), most)) + c.own_unit - 1) / c.own_unit;
+        const int splits = PagedCut::splits(paged_tiles(min(max(len, 0), most)), c.own_unit, p.B * per_split);
         const int through = wave_scan(splits * per_split);
         __syncthreads();                               // the sums are free
         if (lane == 63) sums[wave] = through;
@@ -535,7 +553,7 @@ __device__ __forceinline__ void paged_shared_body(const PagedParams& p, const Pa
 
 // The units are dealt to the workgroups in turn, as the host does not know how many there are and a workgroup without one would cost as
 // much as the summing of the batch: those of the prefix first, then the own ones, of which the first go to the workgroups that have
-// none of the prefix, a few each while the others are at theirs.
+// none of the prefix, a few each while the others are at theirs (24 sequences on a prefix of 8192 34.5 -> 29.8 us, D = 64 35.5 -> 27.0).
 template <int D>
 __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void paged_fwd_kernel(const PagedParams p) {
     extern __shared__ __attribute__((aligned(1024))) uint16_t lds[];
@@ -569,11 +587,11 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void paged_fwd_kernel(const P
             else paged_unit_body<D, 4, false>(p, u, lds, c.prefix_bad, false, p.part_o + slot * p.d, p.part_ml + slot);
             at += (int)gridDim.x;
         } else {
-            const int unit = taken < ahead ? spare + taken * free : ahead * free + (int)blockIdx.x + (taken - ahead) * (int)gridDim.x;
+            const int number = taken < ahead ? spare + taken * free : ahead * free + (int)blockIdx.x + (taken - ahead) * (int)gridDim.x;
             ++taken;
             if (threadIdx.x == 0) found[0] = -1;
             paged_own_units(p, c, sums, [&](int b, int len, int first, int splits) {
-                if (unit >= first && unit < first + splits * p.Hkv * rt) {
+                if (number >= first && number < first + splits * p.Hkv * rt) {
                     found[0] = b;
                     found[1] = first;
                     found[2] = splits;
@@ -585,7 +603,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void paged_fwd_kernel(const P
             __syncthreads();
             const int b = packed_uniform(found[0]);
             if (b < 0) return;                         // past the last unit: nobody has one any more
-            const int in_b = unit - packed_uniform(found[1]), splits = packed_uniform(found[2]), len = packed_uniform(found[3]);
+            const int in_b = number - packed_uniform(found[1]), splits = packed_uniform(found[2]), len = packed_uniform(found[3]);
             const int pair = packed_uniform(in_b / splits), split = in_b - pair * splits, most = p.table_pages << p.page_shift;
             u.own = true;
             u.table = p.table + b * p.table_stride;
@@ -596,9 +614,10 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void paged_fwd_kernel(const P
             u.rows = min(32, rows - u.row0);
             u.b0 = b;
             u.lag = p.N - 1;
-            u.tile0 = split * c.own_unit;
-            u.tiles = min(c.own_unit, paged_tiles(u.keys) - u.tile0);
-            const int64_t slot = p.own_slot + (int64_t)unit * slot_rows;
+            const int unit = packed_uniform(PagedCut::even(paged_tiles(u.keys), c.own_unit, p.B * p.Hkv * rt));
+            u.tile0 = split * unit;
+            u.tiles = min(unit, paged_tiles(u.keys) - u.tile0);
+            const int64_t slot = p.own_slot + (int64_t)number * slot_rows;
             paged_unit_body<D, 4, false>(p, u, lds, len > most, splits == 1 && c.prefix_tiles == 0, p.part_o + slot * p.d, p.part_ml + slot);
         }
     }
@@ -626,7 +645,8 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? (D <= 64 ? 3 : 2) : 2) void page
     paged_unit_body<D, NW, true>(p, u, lds, bad, true, nullptr, nullptr);
 }
 
-// Joins the units of a row: SHARE wavefronts take a share of the units each (4: a workgroup per row, 1: a workgroup for four rows).
+// Joins the units of a row: SHARE wavefronts take a share of the units each (4: a workgroup per row, 1: a workgroup for four rows).  Bound by the
+// latency of plan, maxima and sums one behind the other, about 6 us with its launch.
 template <int SHARE>
 __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams p) {
     __shared__ f32x2 quarter[4][64];

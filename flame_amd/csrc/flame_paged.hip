@@ -61,11 +61,10 @@ int set_lds(const void* kern, int bytes, std::atomic<uint64_t>& done) {      // 
 // Most units that PagedCut makes of `tiles` tiles that `groups` walks (sequences, heads, row tiles) have together at most.
 int64_t most_units(int64_t tiles, int64_t groups) {
     if (tiles <= 0) return 0;
-    const int64_t whole = tiles <= (int64_t)PagedCut::kFill * PagedCut::kLong ? PagedCut::kFill : PagedCut::kMost;
-    return std::min(whole, (tiles + PagedCut::kLeast - 1) / PagedCut::kLeast) + groups;
+    return std::min<int64_t>(PagedCut::places((int)groups), (tiles + PagedCut::least((int)groups) - 1) / PagedCut::least((int)groups)) + groups;
 }
 int64_t most_shared_units(int64_t tiles, int64_t groups) {
-    return tiles <= 0 ? 0 : std::min<int64_t>(PagedCut::kShared, (tiles + PagedCut::kSharedLeast - 1) / PagedCut::kSharedLeast) + groups;
+    return tiles <= 0 ? 0 : std::min<int64_t>(PagedCut::kShared, (tiles + PagedCut::kLeast - 1) / PagedCut::kLeast) + groups;
 }
 
 struct PagedSizes {
@@ -84,7 +83,7 @@ bool paged_sizes(int B, int H, int H_kv, int N, int D, int page, int pages, int 
     const double own = (double)(((int64_t)pages * page + 31) / 32) * B * H_kv * rt, prefix = (double)(((int64_t)prefix_pages * page + 31) / 32) * H_kv * prefix_rt;
     if (own > INT32_MAX / 2 || prefix > INT32_MAX / 2 || (double)pages * page > INT32_MAX / 2 || (double)prefix_pages * page > INT32_MAX / 2) return false;
     const bool shared = PagedCut::shared((int)(B * rows));
-    z->direct = prefix_pages == 0 && (int64_t)pages * page <= kDirectKeys;
+    z->direct = prefix_pages == 0 && (int64_t)pages * page <= (B * H_kv * rt < PagedCut::kFill / 2 ? kDirectKeys : PagedCut::kLong * PagedCut::kTile);
     z->own_units = most_units((int64_t)own, B * H_kv * rt);
     z->prefix_units = shared ? most_shared_units((int64_t)prefix, H_kv * prefix_rt) : most_units((int64_t)prefix, H_kv * prefix_rt);
     z->prefix_rows = z->prefix_units * (shared ? 128 : 32);
@@ -101,7 +100,7 @@ int launch_paged(const PagedParams& p, const PagedSizes& z, hipStream_t s) {
     const int rows = p.N * (p.H / p.Hkv);
     if (z.direct) {
         const int64_t grid = (int64_t)p.B * p.Hkv * PagedCut::row_tiles(rows);
-        const bool wide = grid < 512;                  // a workgroup of eight wavefronts has its compute unit to itself, of four there are two
+        const bool wide = grid <= 256;                 // a workgroup of eight wavefronts has its compute unit to itself, of four there are two
         const auto kern = wide ? paged_direct_kernel<D, 8> : paged_direct_kernel<D, 4>;
         const int lds = PagedTile<D>::lds_bytes(wide ? 8 : 4);
         if (const int rc = set_lds(reinterpret_cast<const void*>(kern), lds, wide ? done8 : done4)) return rc;
@@ -212,7 +211,7 @@ int flame_kv_store_bf16(const void* K, const void* V, void* K_cache, void* V_cac
     p.d = D;
     p.n_pages = n_pages;
     p.page_shift = page_shift(page);
-    p.rows_per_wave = std::max(1, std::min(8, T / 4096));
+    p.rows_per_wave = std::max(1, 64 / (H_kv * (D / 8)));
     const int64_t grid = ((int64_t)T + 4 * p.rows_per_wave - 1) / (4 * p.rows_per_wave);
     hipLaunchKernelGGL(kv_store_kernel, dim3((unsigned)grid), dim3(256), 0, static_cast<hipStream_t>(stream), p);
     return (int)hipGetLastError();

@@ -86,8 +86,8 @@ def run(seed, lens, H, Hkv, N, D, page, prefix=0, **kw):
     torch.cuda.synchronize()
     want = reference(q, keys, D ** -0.5)
     check(o, lse, want)
-    if not prefix and page * table.shape[1] <= 1024:           # short tables go to kernels of their own; a wider one goes the long way
-        wider = torch.cat([table, torch.full((len(lens), 1024 // page + 1), -1, dtype=torch.int32)], 1).cuda()
+    if not prefix and page * table.shape[1] <= 2048:           # short tables go to kernels of their own; a wider one goes the long way
+        wider = torch.cat([table, torch.full((len(lens), 2048 // page + 1), -1, dtype=torch.int32)], 1).cuda()
         o2, l2 = capi.attn_paged_fwd(*args[:3], wider, args[4], D ** -0.5, want_lse=True)
         check(o2, l2, want)
     return args, extra, o, lse
@@ -142,6 +142,15 @@ def test_shared_prefix_of_many_sequences():
 def test_long_sequences():
     run(2, [9000, 3, 4097], 8, 2, 1, 128, 64, wide=40)
     run(3, [20001], 4, 4, 2, 64, 16)
+
+
+@pytest.mark.parametrize("prefix", [0, 300])
+@pytest.mark.parametrize("longest", [2000, 2049, 4500, 9000])
+def test_many_walks(longest, prefix):
+    """256 heads and sequences and more: tables that one workgroup walks, and long walks in even pieces among short ones."""
+    lens = [longest] + [(997 * i) % longest for i in range(17)]
+    run(longest, lens, 16, 16, 1, 64, 16, prefix=prefix)
+    run(longest + 1, lens[:10], 30, 30, 1, 40, 32, prefix=prefix)
 
 
 def test_more_pages_than_a_wavefront_holds():

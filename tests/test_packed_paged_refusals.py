@@ -124,23 +124,31 @@ def test_paged_workspace(lib):
     assert paged(lib, pages=100, ws_bytes=need - 1) == INVALID
 
 
-def units(tiles):
-    """Lengths of units as the kernels cut `tiles` tiles (32 keys each)."""
-    one, more = -(-tiles // 512), -(-tiles // 2048)
-    n = one if one < 32 else max(more, 32)
-    return max(4, -(-n // 4) * 4)
+def units(tiles, walks):
+    """Most tiles of a unit, as the kernels cut `tiles` tiles (32 keys each) of `walks` walks."""
+    if walks < 256:
+        return max(4, -(-tiles // (512 - walks)) + 3 & ~3)
+    return max(64, -(-tiles // max(2048 - walks, 256)) + 3 & ~3)
 
 
-@pytest.mark.parametrize("lens", [[1], [31, 32, 33], [4096] * 7, [100000, 3], [7] * 500, [60000] * 64, [0, 0, 5]])
+def splits(tiles, unit, walks):
+    """Units of a walk: as even as they come if there are many walks."""
+    if walks >= 256 and tiles > unit:
+        n = -(-tiles // unit)
+        unit = -(-tiles // n) + 3 & ~3
+    return -(-tiles // unit)
+
+
+@pytest.mark.parametrize("lens", [[1], [31, 32, 33], [4096] * 7, [100000, 3], [7] * 500, [60000] * 64, [0, 0, 5], [9000, 1, 4000] * 30, [2100] * 300])
 @pytest.mark.parametrize("H,Hkv,N", [(32, 8, 1), (4, 4, 1), (8, 1, 5)])
-def test_workspace_holds_every_unit(lib, lens, H, Hkv, N):
+@pytest.mark.parametrize("wider", [1, 3])
+def test_workspace_holds_every_unit(lib, lens, H, Hkv, N, wider):
     """The units that the device cuts lie within the room that the host asks for, whatever the lengths under a table's width."""
     rows = N * (H // Hkv)
     rt, D, page = -(-rows // 32), 64, 16
-    pages = max(65, max(-(-n // page) for n in lens))              # (of at most 64 pages there are no units)
-    tiles = [-(-n // 32) for n in lens]
-    unit = units(sum(tiles) * Hkv * rt)
-    made = sum(-(-t // unit) for t in tiles) * Hkv * rt
+    pages = wider * max(129, max(-(-n // page) for n in lens))     # (of at most 128 pages there may be no units)
+    tiles, walks = [-(-n // 32) for n in lens], len(lens) * Hkv * rt
+    made = sum(splits(t, units(sum(tiles) * Hkv * rt, walks), walks) for t in tiles) * Hkv * rt
     have = lib.flame_attn_paged_workspace_bytes(len(lens), H, Hkv, N, D, page, pages, 0)
     assert have >= made * min(32, rows) * (4 * D + 8)
     all_rows = len(lens) * rows
@@ -148,10 +156,11 @@ def test_workspace_holds_every_unit(lib, lens, H, Hkv, N):
         t = -(-prefix // 32)
         if all_rows > 64:          # units of 128 rows
             per_split, height = Hkv * -(-all_rows // 128), 128
-            unit = max(16, -(-t * per_split // 256))
+            n = -(-t * per_split // 256)
+            unit = max(n, min(16, 2 * n), 4)
         else:
             per_split, height = Hkv * -(-all_rows // 32), 32
-            unit = units(t * per_split)
+            unit = units(t * per_split, per_split)
         more = lib.flame_attn_paged_workspace_bytes(len(lens), H, Hkv, N, D, page, pages, -(-prefix // page)) - have
         assert more >= -(-t // unit) * per_split * height * (4 * D + 8) - 512
 
