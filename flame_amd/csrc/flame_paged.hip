@@ -72,7 +72,9 @@ struct PagedSizes {
     bool direct;                                                   // one workgroup takes all keys
     size_t plan_bytes, ml_bytes, bytes;                            // of the workspace
 };
-// Up to so many keys of a table one workgroup takes all of a sequence's: 10.9 us instead of 14.2 in two launches (D = 128, 8 key heads, 4 sequences of up to 1024).
+// Up to so many keys of a table one workgroup takes all of a sequence's, in one launch and without the summing of the batch; with as many walks as
+// the cut leaves whole, up to as many keys as it leaves whole.  (In two launches -> in one, us, D = 128, 8 key heads: one sequence of 500 12.0 -> 8.2, 4 of
+// 1000 13.0 -> 11.4, 64 of 1000 48 -> 42, 64 of 2000 97 -> 92, 64 of 200 to 2000 57 -> 52.  4 of 2000 15.4, one workgroup each 17.9.)
 constexpr int64_t kDirectKeys = 1024;
 
 // false: too large
@@ -100,7 +102,9 @@ int launch_paged(const PagedParams& p, const PagedSizes& z, hipStream_t s) {
     const int rows = p.N * (p.H / p.Hkv);
     if (z.direct) {
         const int64_t grid = (int64_t)p.B * p.Hkv * PagedCut::row_tiles(rows);
-        const bool wide = grid <= 256;                 // a workgroup of eight wavefronts has its compute unit to itself, of four there are two
+        // a workgroup of eight wavefronts has its compute unit to itself, of four there are two (four -> eight, us, D = 128, keys 1000: 8
+        // workgroups 14.1 -> 11.1, 64 15.1 -> 11.9, 256 22.6 -> 23.1, D = 64 13.8 -> 13.2, 504 40.4 -> 42.2)
+        const bool wide = grid <= 256;
         const auto kern = wide ? paged_direct_kernel<D, 8> : paged_direct_kernel<D, 4>;
         const int lds = PagedTile<D>::lds_bytes(wide ? 8 : 4);
         if (const int rc = set_lds(reinterpret_cast<const void*>(kern), lds, wide ? done8 : done4)) return rc;
@@ -109,9 +113,10 @@ int launch_paged(const PagedParams& p, const PagedSizes& z, hipStream_t s) {
     }
     constexpr int lds = PagedTile<D>::lds_bytes(4);
     if (const int rc = set_lds(reinterpret_cast<const void*>(paged_fwd_kernel<D>), lds, done)) return rc;
-    const int64_t room = D <= 64 ? 768 : 512;          // workgroups that the card holds
+    const int64_t room = D <= 64 ? 768 : 512;          // workgroups that the card holds (D = 64, 64 sequences of 4000: 512 of them 105.4 us, 768 102.8)
     hipLaunchKernelGGL(paged_fwd_kernel<D>, dim3((unsigned)std::min(room, z.prefix_units + z.own_units)), dim3(256), lds, s, p);
     if (const hipError_t e = hipGetLastError()) return (int)e;
+    // (a workgroup for four rows -> per row, us: 32 rows of 500 units 101 -> 92, 256 rows 21.1 -> 20.4, 992 46.9 -> 47.5, 2048 101.6 -> 104.4)
     const int all = p.B * p.H * p.N;                   // rows
     if (all >= 1024) hipLaunchKernelGGL(paged_merge_kernel<1>, dim3((unsigned)((all + 3) / 4)), dim3(256), 0, s, p);
     else hipLaunchKernelGGL(paged_merge_kernel<4>, dim3((unsigned)all), dim3(256), 0, s, p);

@@ -23,7 +23,8 @@ struct KvStoreParams {
 // A wavefront takes one row, all heads of K and V, or as many rows as make 64 granules of 16 bytes.  A row whose place lies outside its
 // sequence's pages, or on a page outside the cache, is left out.
 // Bound by memory: 32768 rows of 8 heads, D = 128, 41 us, 6.5 TB/s of what is read and written (with eight rows one behind the other in
-// a wavefront 48: the search is short against the latency of a row's chain of table and copy); 65536 rows of one head, D = 64, STORE_SMALL.
+// a wavefront 48: the search is short against the latency of a row's chain of table and copy); 65536 rows of one
+// head, D = 64, 6.7 us, 5.0 TB/s (with a row per wavefront 28).
 static __global__ __launch_bounds__(256) void kv_store_kernel(const KvStoreParams p) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r0 = ((int)blockIdx.x * 4 + wave) * p.rows_per_wave;
@@ -76,7 +77,8 @@ struct KvCopyParams {
 
 constexpr int kKvCopyPerThread = 4;
 
-// blockIdx.x: chunk of a page, of K or V; y: layer; z: pair.
+// blockIdx.x: chunk of a page, of K or V; y: layer; z: pair.  Bound by memory: 600 pages of 16 tokens, 8 heads, D = 128 in 24 layers 386 us,
+// 4.9 TB/s of what is read and written, as fast as a large copy.  Four granules per thread are requested before the first is stored.
 static __global__ __launch_bounds__(256) void kv_copy_kernel(const KvCopyParams p, const KvCopyPairs pairs) {
     const int which = (int)blockIdx.x / p.chunks, chunk = (int)blockIdx.x - which * p.chunks;
     uint16_t* const layer = p.c[which] + (int)blockIdx.y * p.layer[which];
