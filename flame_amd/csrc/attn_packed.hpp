@@ -5,6 +5,13 @@
 //   backward  dS = P (dO V^T - delta),  dQ = scale dS K,  dK = scale sum over the heads of a key head of dS^T Q,  dV = the same of P^T dO
 //
 // The sums over the heads that share a key head are one walk of one workgroup: no atomics, no partial gradients per head.
+//
+// What bounds them is what bounds the dense kernels, at their rates: the matrix instructions and the exponentials between them.  Forward,
+// eight prompts of 1 to 4096, 32 heads on 8, D = 128: 292 us, 1.0 PFLOP/s (as much as the dense causal one on 4096); training on six documents of
+// 333 to 4608, the same heads: forward 370, dQ 520, dK/dV 680 us.  Small batches: the longest walk, one step of 64 keys after the other at 0.6 to 1 us.
+// Roundings to 16 bits, which the matrix instructions' operands take: P before it meets V and dO, dS before it meets K and Q, O as it is saved,
+// from which delta is formed; all sums are fp32.  dQ and dK are therefore off by 0.0025 of their root mean square against 0.0017 of one
+// rounded result: 0.0017 from dS, 0.0013 from P and O in delta.
 #pragma once
 #include "attn_bwd.hpp"
 #include "attn_fwd.hpp"

@@ -196,6 +196,7 @@ int flame_kv_store_bf16(const void* K, const void* V, void* K_cache, void* V_cac
         return rc;
     const int64_t size[4] = {n_pages, H_kv, page, D};
     if (overlaps(kc_strides, size, 4) || overlaps(vc_strides, size, 4)) return FLAME_ATTN_ERR_UNSUPPORTED;
+    if (K_cache == V_cache) return FLAME_ATTN_ERR_INVALID;             // both would be written to the same places
     KvStoreParams p{};
     p.k = static_cast<const uint16_t*>(K);
     p.v = static_cast<const uint16_t*>(V);

@@ -4,8 +4,9 @@
 // Sequence i has the rows [cu[i], cu[i + 1]) (int32 on the device, n + 1 of them, cu[0] taken as 0).  The host knows the number of
 // rows and of sequences, not the lengths, so it launches as many workgroups as there can be tiles, and every workgroup finds its own.
 //   Up to 64 sequences: a lane holds one.  The tiles come in the order of falling walks, so that the longest start first and what
-//   is left at the end is short: under the causal flag tile by tile over all sequences, else sequence by sequence.  On grids that
-//   leave compute units idle the walks are cut into parts (PackedCut) whose partial sums a second launch joins.
+//   is left at the end is short: under the causal flag tile by tile over all sequences (training on six documents of 333 to 4608, us:
+//   sequence by sequence 1543, tile by tile 1515), else sequence by sequence.  On grids that leave compute units idle the walks are cut
+//   into parts (PackedCut) whose partial sums a second launch joins.
 //   More: in their own order.  Every sequence gets the slots [slot(i), slot(i + 1)) with slot(i) = cu[i] / tile + i, at least as many as
 //   it has tiles and at most one more, so that a search finds it without a sum over the lengths.
 // The rows behind the last sequence are the last tiles of that numbering: their workgroups write zeros.

@@ -177,6 +177,8 @@ class PagedCache:
         """Rows k, v [new tokens of the batch, kv_heads, head_dim], sequence after sequence, to their places."""
         if k.shape[0] != sum(batch.counts):
             raise ValueError("as many rows as the batch has new tokens")
+        if not k.shape[0]:
+            return
         capi.kv_store(k, v, self.k[layer], self.v[layer], batch.page_table, batch.cu, batch.start)
 
     def attend(self, layer, q, batch, scale=None):

@@ -300,7 +300,8 @@ int flame_attn_paged_fwd_bf16(const void* Q, const void* K_cache, const void* V_
 
 /* Rows K, V [T, H_kv, D] (three element strides in (row, head, D) order) of n_seqs sequences, sequence b having the rows
  * cu[b] .. cu[b + 1] - 1 (int32 [n_seqs + 1] on the device, rising from 0), to the places start[b], start[b] + 1, ... of their pages.
- * Rows behind the last sequence are not stored.  Two rows for one place leave either of them.  D any multiple of 8. */
+ * Rows behind the last sequence are not stored.  Two rows for one place leave either of them.  D any multiple of 8.  K_cache and
+ * V_cache are different tensors (one pointer for both is FLAME_ATTN_ERR_INVALID). */
 int flame_kv_store_bf16(const void* K, const void* V, void* K_cache, void* V_cache, const int32_t* page_table,
                         int64_t table_stride, int table_pages, const int32_t* cu, const int32_t* start, int n_seqs, int T, int H_kv,
                         int D, int n_pages, int page, const int64_t* k_strides, const int64_t* v_strides,

@@ -1,6 +1,6 @@
 // UNVERIFIED SOURCE: never compiled (no Rust toolchain in the image the library is developed in).
 //
-// Build script of the crate: one hipcc compilation of the attention library for gfx950 and nothing else, archived
+// Build script of the crate: hipcc compilations of the attention library for gfx950 and nothing else, archived
 // and linked statically, with the HIP runtime as the only dynamic dependency.  It takes the place of the part of
 // flame-core's build.rs that loops nvcc over the CUDA sources and links cudart / cuBLAS / cuDNN
 // (build.rs:251-347 there; the cuDNN discovery at :53-86 has no counterpart: nothing is discovered, nothing is

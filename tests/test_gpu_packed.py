@@ -192,6 +192,29 @@ def test_strided_views():
         check(name, t.cpu(), *z[name])
 
 
+def test_rows_far_apart():
+    """Row strides just below their limit, elements past 2^32: the results of the same rows close together, to the bit."""
+    from flame_amd import capi
+    lens, H, Hkv, D, far = [1, 170, 129], 4, 2, 64, (1 << 24) - 8
+    q, k, v, do, cq, ck = (t.cuda() for t in make(8, lens, lens, H, Hkv, D))
+    o, lse = capi.attn_packed_fwd(q, k, v, cq, ck, 0.125)
+    near = (o, *capi.attn_packed_bwd(q, k, v, o, do, lse, cq, ck, 0.125))
+    memory = torch.empty(len(q) * far, dtype=torch.bfloat16, device="cuda")
+    assert memory.numel() > 2 ** 32
+    at, views = 0, []
+    for t in (q, k, v, do, o, q, k, v):
+        views.append(memory.as_strided(t.shape, (far, D, 1), at))
+        at += t.shape[1] * D
+    for view, t in zip(views, (q, k, v, do)):
+        view.copy_(t)
+    fq, fk, fv, fdo, fo, *grads = views
+    _, far_lse = capi.attn_packed_fwd(fq, fk, fv, cq, ck, 0.125, out=fo)
+    capi.attn_packed_bwd(fq, fk, fv, fo, fdo, far_lse, cq, ck, 0.125, grads=tuple(grads))
+    assert torch.equal(lse, far_lse)
+    for a, b in zip(near, (fo, *grads)):
+        assert torch.equal(a, b)
+
+
 def test_same_result_every_time():
     dev, o, l, g = run(5, [700, 300, 64], [700, 300, 64], 8, 2, 128, True)
     for _ in range(3):

@@ -26,6 +26,7 @@ def i64(*v):
 
 
 P = ctypes.c_void_p(4096)            # never dereferenced: the checks come first
+P2 = ctypes.c_void_p(1 << 20)
 ODD = ctypes.c_void_p(4104)          # not on 16 bytes
 NULL = ctypes.c_void_p(0)
 
@@ -165,14 +166,14 @@ def test_workspace_holds_every_unit(lib, lens, H, Hkv, N, wider):
         assert more >= -(-t // unit) * per_split * height * (4 * D + 8) - 512
 
 
-def store(lib, k=P, kc=P, table=P, cu=P, start=P, n=2, T=10, H_kv=2, D=64, n_pages=20, page=16, pages=4, ks=(128, 64, 1), kcs=(2048, 1024, 64, 1)):
-    return lib.flame_kv_store_bf16(k, P, kc, P, table, ctypes.c_int64(4), pages, cu, start, n, T, H_kv, D, n_pages, page, i64(*ks), i64(*ks), i64(*kcs), i64(*kcs), NULL)
+def store(lib, k=P, kc=P, vc=P2, table=P, cu=P, start=P, n=2, T=10, H_kv=2, D=64, n_pages=20, page=16, pages=4, ks=(128, 64, 1), kcs=(2048, 1024, 64, 1)):
+    return lib.flame_kv_store_bf16(k, P, kc, vc, table, ctypes.c_int64(4), pages, cu, start, n, T, H_kv, D, n_pages, page, i64(*ks), i64(*ks), i64(*kcs), i64(*kcs), NULL)
 
 
 @pytest.mark.parametrize("bad,code", [
     (dict(k=NULL), INVALID), (dict(kc=NULL), INVALID), (dict(table=NULL), INVALID), (dict(cu=NULL), INVALID), (dict(start=NULL), INVALID), (dict(n=0), INVALID),
     (dict(T=0), INVALID), (dict(n_pages=0), INVALID), (dict(pages=0), INVALID), (dict(page=12), UNSUPPORTED), (dict(D=4), UNSUPPORTED), (dict(k=ODD), UNSUPPORTED),
-    (dict(ks=(128, 64, 2)), UNSUPPORTED), (dict(kcs=(0, 1024, 64, 1)), UNSUPPORTED), (dict(kcs=(2048, 1024, 32, 1)), UNSUPPORTED)])
+    (dict(ks=(128, 64, 2)), UNSUPPORTED), (dict(kcs=(0, 1024, 64, 1)), UNSUPPORTED), (dict(kcs=(2048, 1024, 32, 1)), UNSUPPORTED), (dict(vc=P), INVALID)])
 def test_store(lib, bad, code):
     assert store(lib, **bad) == code
 
