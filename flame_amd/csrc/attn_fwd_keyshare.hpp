@@ -34,8 +34,10 @@ struct FwdKeyShareTile {
 // DROP (DropMode) as in fwd_kernel.  At D = 64 four wavefronts per SIMD, two workgroups of eight per unit; the draw by tiles takes 184 registers
 // and keeps to two: within 128 it spilled 56 bytes per lane (us, that -> this: 4 heads of 512 11.8 -> 10.1, 8 of 1024 19.5 -> 15.4, 16 of 1024 33.3 -> 26.4, 2 of 4096
 // 57.7 -> 45.7, 64 heads, 20 queries, 2000 keys 36.4 -> 25.3).
+// `all`: number of this workgroup's query tile (and slice of its keys).  Under the causal flag query i attends to key j <= i + past.
+// (p by value: through a reference the kernel at D = 64 had 24 instructions more and was 1 % slower.)
 template <int D, int NW_, int DROP>
-__global__ __launch_bounds__(64 * NW_, D == 64 && DROP != kDropTiled ? 4 : 2) void fwd_keyshare_kernel(const FwdParams p) {
+__device__ __forceinline__ void fwd_keyshare_body(const FwdParams p, const int all, const int past) {
     using T = FwdKeyShareTile<D, NW_>;
     constexpr int BN = T::BN, NW = T::NW, RS = T::RS, DC = D / 16, DB = D / 32, GPR = RS / 8, NDMA = T::NDMA;
 
@@ -47,7 +49,6 @@ __global__ __launch_bounds__(64 * NW_, D == 64 && DROP != kDropTiled ? 4 : 2) vo
     const int n = lane & 31, h = lane >> 5;
 
     const int n_qt = (p.Sq + T::BQ - 1) / T::BQ;
-    const int all = xcd_remap(blockIdx.x, gridDim.x);            // the workgroups of a (batch, head) share an L2
     const int slice = all % p.key_splits, wg = p.wg_base + all / p.key_splits;
     const int bh = wg / n_qt, qi = (wg % n_qt) * T::BQ + n, q0 = (wg % n_qt) * T::BQ;     // qi: this lane's query
     const int b = bh / p.H, hh = bh % p.H;
@@ -58,7 +59,7 @@ __global__ __launch_bounds__(64 * NW_, D == 64 && DROP != kDropTiled ? 4 : 2) vo
     int klimit = p.Sk;
     if (p.m.kv_len) klimit = min(klimit, max(p.m.kv_len[b], 0));
     int kend = klimit;
-    if (p.m.causal) kend = min(kend, q0 + T::BQ);
+    if (p.m.causal) kend = min(kend, q0 + T::BQ + past);         // (not positive: no tile is walked)
     const int n_tiles_all = (kend + BN - 1) / BN;
     const int per = (n_tiles_all + p.key_splits - 1) / p.key_splits;
     const int t_lo = slice * per, t_hi = min(n_tiles_all, t_lo + per);
@@ -150,7 +151,7 @@ __global__ __launch_bounds__(64 * NW_, D == 64 && DROP != kDropTiled ? 4 : 2) vo
         for (int r = 0; r < 16; ++r) s[r] = 0.f;
 #pragma unroll
         for (int dc = 0; dc < DC; ++dc) s = mfma32(kf[dc], qf[dc], s);
-        const int lim = (p.m.causal ? min(klimit, qi + 1) : klimit) - t * BN - 4 * h;
+        const int lim = (p.m.causal ? min(klimit, qi + 1 + past) : klimit) - t * BN - 4 * h;
         if (__any(lim < BN))
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = 8 * (r >> 2) + (r & 3) >= lim ? -INFINITY : s[r];
@@ -258,6 +259,11 @@ __global__ __launch_bounds__(64 * NW_, D == 64 && DROP != kDropTiled ? 4 : 2) vo
             if (p.lse && g == 0) p.lse[r] = lse;
         }
     }
+}
+
+template <int D, int NW, int DROP>
+__global__ __launch_bounds__(64 * NW, D == 64 && DROP != kDropTiled ? 4 : 2) void fwd_keyshare_kernel(const FwdParams p) {
+    fwd_keyshare_body<D, NW, DROP>(p, xcd_remap(blockIdx.x, gridDim.x), 0);        // the workgroups of a (batch, head) share an L2
 }
 
 }  // namespace fattn

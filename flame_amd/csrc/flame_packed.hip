@@ -42,10 +42,10 @@ int set_lds(const void* kern, int bytes, std::atomic<uint64_t>& done) {      // 
 }
 
 template <class P>
-int launch(void (*kern)(P, PackedArgs), int lds, std::atomic<uint64_t>& done, int64_t units, int heads, const P& p, const PackedArgs& a, hipStream_t s) {
+int launch(void (*kern)(P, PackedArgs), int lds, std::atomic<uint64_t>& done, int64_t units, int heads, const P& p, const PackedArgs& a, hipStream_t s, int threads = 256) {
     if (units * heads > INT32_MAX) return FLAME_ATTN_ERR_UNSUPPORTED;
     if (const int rc = set_lds(reinterpret_cast<const void*>(kern), lds, done)) return rc;
-    hipLaunchKernelGGL(kern, dim3((unsigned)(units * heads)), dim3(256), (size_t)lds, s, p, a);
+    hipLaunchKernelGGL(kern, dim3((unsigned)(units * heads)), dim3(threads), (size_t)lds, s, p, a);
     return (int)hipGetLastError();
 }
 template <class P>
@@ -57,64 +57,96 @@ int launch_merge(void (*kern)(P, PackedArgs), int64_t tiles, int heads, int bloc
 int padded(int D) { return D <= 64 ? 64 : D <= 96 ? 96 : 128; }
 size_t align256(size_t x) { return (x + 255) / 256 * 256; }
 
-// log2 of what the card holds of a kernel's workgroups, two per compute unit or one
-constexpr int kRoomQueries = 9, kRoomKeys = 8;
+// Two workgroups of queries per compute unit, one of keys (at D = 64 a second one fits).  The backward's steps are longer, so shorter parts pay
+// there (at least 16 steps each -> 8, us: 8 heads on 2 of 612 65 -> 51, 4 of 2000 72 -> 58, D = 64, 4 of 2000 50 -> 42; forward, 8 of 100 rows on 30000 keys
+// 37 -> 46).
+constexpr PackedCut kCutFwd{9, 16, 16, 1.6f}, kCutDq{9, 8, 12, 1.6f};
+PackedCut cut_dkdv(int D) { return PackedCut{8, 8, 12, D <= 64 ? 0.65f : 1.6f}; }
 // Whether a problem gets room for walks in parts, which the device then cuts or not by the lengths (PackedCut): not where whole walks fill the
 // 256 compute units one and a half times, nor where the mean walk is short, nor where no lengths of these sums would be cut (the fewest
 // steps: a causal self-attention's).
-// (Whole -> in parts, us.  Forward: D = 128, 8 heads of 2000 34.8 -> 28.4, 4 of 8192 117 -> 89, 32 of 128 rows on 8192 keys 115 -> 33; D = 64, 2 of
-// 4096 41 -> 21.  Backward, two heads to a key head and more: 8 of 2000 207 -> 94, 4 of 8192 439 -> 267.  Left whole: 24 heads of 1200 24.7 (in parts 30.7),
-// backward 68 (86); D = 64, 12 heads of twice 2000 25.8 (34).)
-bool parts_pay(int64_t slots, int heads, int n_seqs, int walked_rows) {
-    if (n_seqs > 64 || walked_rows / n_seqs < 1024 || slots * heads * 2 >= 3 << PackedCut::kUnits_log2) return false;
-    return PackedCut::pays((walked_rows + 63) / 64, (slots - n_seqs) * heads * (walked_rows / n_seqs / 128));
+// (Whole -> in parts, us, D = 128.  Forward: 4 heads of 8192 117 -> 88, 32 of 128 rows on 8192 keys 115 -> 32, 8 of 100 rows on 30000 400 -> 37.  Backward: 4 of
+// 1024 53 -> 48, 8 on 2 of 612 67 -> 52, of 2000 207 -> 82, 4 on 2 of 8192 439 -> 263.  Left whole: 24 of 1200 23 and 64, in parts 35 and 94.)
+bool parts_pay(const PackedCut& cut, int64_t slots, int heads, int n_seqs, int walked_rows) {
+    if (n_seqs > 64 || walked_rows / n_seqs < 64 * cut.gain || slots * heads * 2 >= 3 << PackedCut::kUnits_log2) return false;
+    return cut.pays((walked_rows + 63) / 64, (slots - n_seqs) * heads * (walked_rows / n_seqs / 128));
 }
 
 struct Parts {
     int64_t slots, units;          // per head: tiles, and units at most
-    int room_log2;                 // 0: whole walks
+    PackedCut cut;
     size_t bytes;                  // of the units' sums
 };
-Parts parts_of(int tile_rows, int walked_rows, int n_seqs, int heads, int room_log2, size_t unit_bytes) {
-    Parts z{packed_slots(tile_rows, n_seqs, 128), 0, 0, 0};
-    z.units = z.slots;
-    if (parts_pay(z.slots, heads, n_seqs, walked_rows)) {
-        z.room_log2 = room_log2;
-        z.units = PackedCut::most(z.slots, heads, room_log2);
+Parts whole(int64_t slots) { return Parts{slots, slots, PackedCut{0, 0, 0, 0.f}, 0}; }
+Parts parts_of(const PackedCut& cut, int tile_rows, int walked_rows, int n_seqs, int heads, size_t unit_bytes) {
+    Parts z = whole(packed_slots(tile_rows, n_seqs, 128));
+    if (parts_pay(cut, z.slots, heads, n_seqs, walked_rows)) {
+        z.cut = cut;
+        z.units = cut.most(z.slots, heads);
         z.bytes = align256((size_t)z.units * heads * unit_bytes);
     }
     return z;
 }
-Parts fwd_parts(int n_seqs, int T_q, int T_kv, int H, int D) { return parts_of(T_q, T_kv, n_seqs, H, kRoomQueries, (size_t)128 * (padded(D) * sizeof(float) + sizeof(f32x2))); }
-Parts dq_parts(int n_seqs, int T_q, int T_kv, int H, int D) { return parts_of(T_q, T_kv, n_seqs, H, kRoomQueries, (size_t)128 * padded(D) * sizeof(float)); }
+// Workgroups of 32 queries whose wavefronts share the keys, in place of 128 queries per workgroup: where two fit a compute unit, or four at D = 64, all
+// at once, the second half of them for walks that are not the shortest; and where no walk is so long that parts of it (above) are better.
+// (128 queries -> 32, us.  D = 128: 24 heads of 77 7.7 -> 6.5, 4 of 1024 19.7 -> 12.8, 4 of 2000 25.6 -> 18.5, 8 of 1200 24.5 -> 17.6, 16 of four pieces of 100 on
+// 900 keys 19.5 -> 14.9; beyond: 24 of 1024 21.5 -> 26.1, 32 of 700 15.7 -> 21.0, 8 of 4000 53.5 -> 60; short: 24 of eight times 32 6.9 -> 7.4.  D = 64: 8 of 612 11.3 -> 7.8, 12 of
+// 2000 24.3 -> 18.4, 16 of 2000 26.9 -> 20.2; beyond: 24 of 2000 25.6 -> 29.7.  8 heads of 100 on 4000 keys: 23.6 -> 25.5, D = 64 18.6 -> 17.9.)
+bool keyshare_pays(int n_seqs, int T_q, int T_kv, int H, int D) {
+    const int64_t grid = packed_slots(T_q, n_seqs, 32) * H, most = D <= 64 ? 1024 : 512;
+    return grid <= (T_kv / n_seqs >= 256 ? most : most / 2) && (n_seqs < 4 ? T_kv : 4 * (int64_t)T_kv / n_seqs) <= 4096;
+}
+// ... eight wavefronts while a compute unit gets one workgroup at most (two at D = 64 with long walks), else four
+bool keyshare_wide(int n_seqs, int T_q, int T_kv, int H, int D) {
+    const int64_t grid = packed_slots(T_q, n_seqs, 32) * H;
+    return grid <= 256 || (D <= 64 && grid <= 512 && T_kv / n_seqs >= 2048);
+}
+Parts fwd_parts(int n_seqs, int T_q, int T_kv, int H, int D) {
+    if (keyshare_pays(n_seqs, T_q, T_kv, H, D)) return whole(packed_slots(T_q, n_seqs, 32));
+    return parts_of(kCutFwd, T_q, T_kv, n_seqs, H, (size_t)128 * (padded(D) * sizeof(float) + sizeof(f32x2)));
+}
+Parts dq_parts(int n_seqs, int T_q, int T_kv, int H, int D) { return parts_of(kCutDq, T_q, T_kv, n_seqs, H, (size_t)128 * padded(D) * sizeof(float)); }
 Parts dkdv_parts(int n_seqs, int T_q, int T_kv, int H, int H_kv, int D) {
-    return parts_of(T_kv, (int)std::min<int64_t>((int64_t)T_q * (H / H_kv), INT32_MAX), n_seqs, H_kv, kRoomKeys, (size_t)2 * 128 * padded(D) * sizeof(float));
+    return parts_of(cut_dkdv(D), T_kv, (int)std::min<int64_t>((int64_t)T_q * (H / H_kv), INT32_MAX), n_seqs, H_kv, (size_t)2 * 128 * padded(D) * sizeof(float));
+}
+
+// One launch for the sums of the parts: with few tiles a workgroup per eight columns, with more one per 32.  (Per 32 -> per eight, us: 8 tiles of 30
+// parts each 45.8 -> 37.0, backward, D = 64, 8 heads on 2 of 1024 47.5 -> 43.8; 192 tiles of two or three parts 39.9 -> 44.7.)
+template <class P>
+int merge_parts_of(const Parts& z, int heads, int D, void (*eight)(P, PackedArgs), void (*wide)(P, PackedArgs), const P& p, const PackedArgs& a, hipStream_t s) {
+    if (!z.cut.room_log2) return FLAME_ATTN_OK;
+    return z.slots * heads <= 96 ? launch_merge(eight, z.slots, heads, D / 8, p, a, s) : launch_merge(wide, z.slots, heads, D / 32, p, a, s);
 }
 
 template <int D>
 int launch_fwd(FwdParams p, PackedArgs a, void* workspace, size_t bytes, hipStream_t s) {
-    static std::atomic<uint64_t> done{0};
+    static std::atomic<uint64_t> done{0}, done4{0}, done8{0};
+    if (keyshare_pays(a.n, a.total_q, a.total_k, a.H, D)) {
+        const int64_t slots = packed_slots(a.total_q, a.n, 32);
+        return keyshare_wide(a.n, a.total_q, a.total_k, a.H, D)
+                   ? launch(fwd_packed_keyshare_kernel<D, 8>, FwdKeyShareTile<D, 8>::LDS_BYTES, done8, slots, a.H, p, a, s, 512)
+                   : launch(fwd_packed_keyshare_kernel<D, 4>, FwdKeyShareTile<D, 4>::LDS_BYTES, done4, slots, a.H, p, a, s);
+    }
     Parts z = fwd_parts(a.n, a.total_q, a.total_k, a.H, D);
-    if (!workspace || bytes < z.bytes) z.room_log2 = 0, z.units = z.slots;
-    a.room_log2 = z.room_log2;
+    if (!workspace || bytes < z.bytes) z = whole(z.slots);
+    a.cut = z.cut;
     p.part_o = static_cast<float*>(workspace);
     p.part_lse = p.part_o + z.units * a.H * 128 * D;
     if (const int rc = launch(fwd_packed_kernel<D>, FwdTile<D>::LDS_BYTES + FwdTile<D>::q_pass_bytes(4), done, z.units, a.H, p, a, s)) return rc;
-    return z.room_log2 ? launch_merge(fwd_packed_merge_kernel<D>, z.slots, a.H, D / 32, p, a, s) : FLAME_ATTN_OK;
+    return merge_parts_of(z, a.H, D, fwd_packed_merge_kernel<D, 1>, fwd_packed_merge_kernel<D, 4>, p, a, s);
 }
 
 template <int D>
 int launch_bwd(BwdParams p, PackedArgs a, size_t part_bytes, hipStream_t s) {
     static std::atomic<uint64_t> done_q{0}, done_kv{0};
     Parts q = dq_parts(a.n, a.total_q, a.total_k, a.H, D), kv = dkdv_parts(a.n, a.total_q, a.total_k, a.H, a.Hkv, D);
-    if (part_bytes < std::max(q.bytes, kv.bytes)) q.room_log2 = kv.room_log2 = 0, q.units = q.slots, kv.units = kv.slots;
-    a.room_log2 = q.room_log2;
+    if (part_bytes < std::max(q.bytes, kv.bytes)) q = whole(q.slots), kv = whole(kv.slots);
+    a.cut = q.cut;
     if (const int rc = launch(bwd_dq_packed_kernel<D>, BwdDqTile<D>::LDS_BYTES, done_q, q.units, a.H, p, a, s)) return rc;
-    if (q.room_log2)
-        if (const int rc = launch_merge(bwd_dq_packed_merge_kernel<D>, q.slots, a.H, D / 32, p, a, s)) return rc;
-    a.room_log2 = kv.room_log2;
+    if (const int rc = merge_parts_of(q, a.H, D, bwd_dq_packed_merge_kernel<D, 1>, bwd_dq_packed_merge_kernel<D, 4>, p, a, s)) return rc;
+    a.cut = kv.cut;
     if (const int rc = launch(bwd_dkdv_packed_kernel<D>, BwdTile<D>::LDS_BYTES, done_kv, kv.units, a.Hkv, p, a, s)) return rc;
-    return kv.room_log2 ? launch_merge(bwd_dkdv_packed_merge_kernel<D>, kv.slots, a.Hkv, D / 32, p, a, s) : FLAME_ATTN_OK;
+    return merge_parts_of(kv, a.Hkv, D, bwd_dkdv_packed_merge_kernel<D, 1>, bwd_dkdv_packed_merge_kernel<D, 4>, p, a, s);
 }
 
 bool head_dim_ok(int D) { return D > 0 && D % 8 == 0 && D <= 128; }
@@ -153,7 +185,7 @@ int flame_attn_packed_fwd_bf16(const void* Q, const void* K, const void* V, void
     p.d = p.dv = D;
     p.scale = scale;
     p.m.causal = causal ? 1 : 0;
-    const PackedArgs a{cu_q, cu_k, n_seqs, T_q, T_kv, H, H_kv, p.m.causal, 0};
+    const PackedArgs a{cu_q, cu_k, n_seqs, T_q, T_kv, H, H_kv, p.m.causal, PackedCut{0, 0, 0, 0.f}};
     hipStream_t s = static_cast<hipStream_t>(stream);
     return D <= 64 ? launch_fwd<64>(p, a, workspace, workspace_bytes, s)
                    : D <= 96 ? launch_fwd<96>(p, a, workspace, workspace_bytes, s) : launch_fwd<128>(p, a, workspace, workspace_bytes, s);
@@ -196,7 +228,7 @@ int flame_attn_packed_bwd_bf16(const void* Q, const void* K, const void* V, cons
     p.d = D;
     p.scale = scale;
     p.m.causal = causal ? 1 : 0;
-    const PackedArgs a{cu_q, cu_k, n_seqs, T_q, T_kv, H, H_kv, p.m.causal, 0};
+    const PackedArgs a{cu_q, cu_k, n_seqs, T_q, T_kv, H, H_kv, p.m.causal, PackedCut{0, 0, 0, 0.f}};
     hipStream_t s = static_cast<hipStream_t>(stream);
     return D <= 64 ? launch_bwd<64>(p, a, part_bytes, s) : D <= 96 ? launch_bwd<96>(p, a, part_bytes, s) : launch_bwd<128>(p, a, part_bytes, s);
 }

@@ -37,6 +37,28 @@ struct PackedUnit {
     __device__ __forceinline__ int64_t k_at(const S& st) const { return k_row * st.n + kv_head * st.h; }
 };
 
+// How walks are cut.  The walks of all `units` tiles together have `steps` steps; the parts are to fill the workgroups that the card holds at
+// once, of which the last part of every tile takes half a place on average.  Parts of fewer than 16 steps are `scale` times as long as that
+// gives: longer, to leave places for the workgroups of parts that a tile with a shorter walk does not have; shorter, where a compute unit takes a
+// second workgroup and has little to do.  At least `least`: a part should not spend its time on loading its rows and leaving its sums.
+// Nothing is cut where the longest walk is hardly longer than what each of the 256 compute units has to do anyway: joining the parts
+// costs about `gain` steps.
+struct PackedCut {
+    int room_log2, least, gain;    // log2 of the workgroups that the card holds, 0: whole walks
+    float scale;
+    static constexpr int kUnits_log2 = 8, kWhole = 1 << 30;
+    __host__ __device__ bool pays(int longest, int64_t steps) const { return longest - (int)(steps >> kUnits_log2) > gain; }
+    __host__ __device__ int share(int64_t steps, int units) const {
+        const int room = 1 << room_log2, places = room - units / 2 > room / 4 ? room - units / 2 : room / 4;
+        const float n = (float)steps / (float)places;
+        if (n < 16.f) return scale * n < (float)least ? least : scale * n > 16.f ? 16 : (int)(scale * n);
+        return n > 1e9f ? 1000000000 : (int)n + 1;
+    }
+    // units per head, at most, of `slots` tiles: a sequence's longest walk is at most twice the mean that `steps` counts, a part at least half
+    // as long as the places give (one more for the rounding of `n`)
+    int64_t most(int64_t slots, int heads) const { return slots + (((scale < 1.f ? 4 : 2) << room_log2) + heads - 1) / heads + 1; }
+};
+
 struct PackedArgs {
     const int32_t* cu_q;
     const int32_t* cu_k;
@@ -44,26 +66,10 @@ struct PackedArgs {
     int total_q, total_k;          // rows of the tensors
     int H, Hkv;
     int causal;
-    int room_log2;                 // log2 of the workgroups that the parts of the walks are to fill, 0: whole walks
+    PackedCut cut;
 };
 
 inline int64_t packed_slots(int total, int n, int tile) { return (int64_t)total / tile + n + 1; }
-
-// How walks are cut.  The walks of all `units` tiles together have `steps` steps; the parts are to fill the 1 << room_log2 workgroups that
-// the card holds at once, of which the last part of every tile takes half a place on average.  A part has not so few steps that it spends its
-// time on loading its rows and leaving its sums, and nothing is cut where the longest walk is hardly longer than what each of the
-// 256 compute units has to do anyway: joining the parts costs about kGain steps.
-struct PackedCut {
-    static constexpr int kLeast = 16, kGain = 16, kUnits_log2 = 8, kWhole = 1 << 30;
-    static __host__ __device__ bool pays(int longest, int64_t steps) { return longest - (int)(steps >> kUnits_log2) > kGain; }
-    static __host__ __device__ int share(int64_t steps, int units, int room_log2) {
-        const int room = 1 << room_log2, places = room - units / 2 > room / 4 ? room - units / 2 : room / 4;
-        const float n = (float)steps / (float)places;
-        return n < (float)kLeast ? kLeast : n > 1e9f ? 1000000000 : (int)n + 1;
-    }
-    // units per head, at most, of `slots` tiles: a sequence's longest walk is at most twice the mean that `steps` counts (one more for the rounding of `n`)
-    static int64_t most(int64_t slots, int heads, int room_log2) { return slots + ((2 << room_log2) + heads - 1) / heads + 1; }
-};
 
 enum PackedWork : int { kPackedIdle = 0, kPackedTile = 1, kPackedBehind = 2 };
 
@@ -141,7 +147,7 @@ __device__ __forceinline__ PackedWork packed_unit(const PackedArgs& a, int block
         const int tiles = ((KEYS ? Sk : Sq) + TILE - 1) / TILE;
         const int walk = ((KEYS ? Sq : Sk) + STEP - 1) / STEP * (KEYS ? rep : 1);
         int parts = 1, share = PackedCut::kWhole;
-        if (a.room_log2) {
+        if (a.cut.room_log2) {
             // steps of the batch, every sequence's by its mean walk (the causal flag leaves its first tiles little): at least half the longest
             const float cut = a.causal ? 0.5f * (float)min(Sq, Sk) / (float)max(max(Sq, Sk), 1) : 0.f;
             const int64_t mine = (int64_t)tiles * max((walk + 1) / 2, (int)((float)walk * (1.0f - cut)));
@@ -149,7 +155,7 @@ __device__ __forceinline__ PackedWork packed_unit(const PackedArgs& a, int block
             const int64_t steps = (((int64_t)high << 24) + low) * heads;
             int longest = 0;
             for (int j = 0; j < a.n; ++j) longest = max(longest, __builtin_amdgcn_readlane(walk, j));
-            if (PackedCut::pays(longest, steps)) share = packed_uniform(PackedCut::share(steps, __builtin_amdgcn_readlane(wave_scan(tiles), 63) * heads, a.room_log2));
+            if (a.cut.pays(longest, steps)) share = packed_uniform(a.cut.share(steps, __builtin_amdgcn_readlane(wave_scan(tiles), 63) * heads));
             parts = max((walk + share - 1) / share, 1);
         }
         if (MERGE && share == PackedCut::kWhole) return kPackedIdle;

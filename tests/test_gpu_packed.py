@@ -96,8 +96,18 @@ def run(seed, lq, lk, H, Hkv, D, causal, behind=0, behind_k=0, poison=False):
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("D", [64, 96, 128])
 @pytest.mark.parametrize("lens", [[1], [64], [65, 1, 127, 128, 129], [300, 7, 513], [0, 33, 0, 0, 200, 0]])
-def test_self_attention(lens, D, causal):
-    run(len(lens) * D, lens, lens, 4, 2, D, causal)
+@pytest.mark.parametrize("H,behind", [(4, 0), (20, 0), (8, 2200)])
+def test_self_attention(lens, D, causal, H, behind):
+    """Few rows, whose keys the wavefronts of a workgroup share; room for many, which have 128 to a workgroup."""
+    run(len(lens) * D, lens, lens, H, 2, D, causal, behind)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("D", [64, 72, 96, 128])
+@pytest.mark.parametrize("lens,H", [([700, 1, 400], 10), ([1100, 900], 2), ([3000], 4), ([1, 2, 3] * 10 + [50], 5), ([31] * 70 + [700], 2)])
+def test_shared_keys(lens, H, D, causal):
+    """Grids of the kernels whose wavefronts share the keys, eight and four of them, more than 64 sequences, rows behind."""
+    run(H, lens, lens, H, H // 2 if H % 2 == 0 else 1, D, causal, 40, 9)
 
 
 @pytest.mark.parametrize("H,Hkv", [(1, 1), (3, 1), (8, 8), (6, 3), (16, 8), (24, 8), (8, 1), (5, 5)])
@@ -117,6 +127,7 @@ def test_other_key_lengths(lq, lk, causal):
     """More keys than queries (earlier keys), fewer (queries without a key), and none of either."""
     run(len(lq), lq, lk, 6, 2, 64, causal)
     run(len(lq), lq, lk, 2, 2, 128, causal)
+    run(len(lq), lq, lk, 10, 2, 96, causal, 1700)
 
 
 @pytest.mark.parametrize("behind", [1, 127, 128, 500])
@@ -157,7 +168,7 @@ def test_long_sequence():
 
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("D", [64, 96, 128])
-@pytest.mark.parametrize("lq,lk", [([100, 5, 129], [5000, 1300, 129]), ([2000], [2000]), ([1, 0, 1], [3000, 700, 0]), ([1500, 40, 1700], [1500, 40, 1600])])
+@pytest.mark.parametrize("lq,lk", [([100, 5, 129], [5000, 1300, 129]), ([4200], [4200]), ([1, 0, 1], [5000, 700, 0]), ([2500, 40, 1700], [2500, 40, 1600])])
 def test_walks_in_parts(lq, lk, D, causal):
     """Few tiles and long walks: the parts' sums are joined by a second launch.  Without room for them the walks stay whole."""
     from flame_amd import capi

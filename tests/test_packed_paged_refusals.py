@@ -65,17 +65,18 @@ def test_packed_workspace(lib):
     assert f(0, 10, 10, 8, 2, 64) == f(1, 10, 10, 8, 3, 64) == f(1, 10, 10, 8, 2, 63) == 0
 
 
-def cut(lens_tile, lens_walk, heads, rep, causal, room_log2):
+def cut(lens_tile, lens_walk, heads, rep, causal, room, least, gain, scale):
     """Units per head as the packed kernels make them: (tiles, longest walk, mean walk) of every sequence, parts of the longest."""
     rows = []
     for t, w in zip(lens_tile, lens_walk):
         tiles, walk = -(-t // 128), -(-w // 64) * rep
         less = 0.5 * min(t, w) / max(t, w, 1) if causal else 0.0
         rows.append((tiles, walk, max((walk + 1) // 2, int(walk * (1 - less) + 1e-3))))
-    steps, units, room = sum(t * m for t, _, m in rows) * heads, sum(t for t, _, _ in rows) * heads, 1 << room_log2
-    if max(w for _, w, _ in rows) - steps // 256 <= 16:
+    steps, units = sum(t * m for t, _, m in rows) * heads, sum(t for t, _, _ in rows) * heads
+    if max(w for _, w, _ in rows) - steps // 256 <= gain:
         return sum(t for t, _, _ in rows)
-    share = max(16, int(steps / max(room - units // 2, room // 4)) + 1)
+    n = steps / max(room - units // 2, room // 4)
+    share = int(n) + 1 if n >= 16 else max(least, min(16, int(scale * n)))
     return sum(t * max(1, -(-w // share)) for t, w, _ in rows)
 
 
@@ -88,13 +89,16 @@ def test_workspaces_hold_every_part(lib, lens_q, lens_k, H, Hkv, causal):
     Tq, Tk, n, D = sum(lens_q), sum(lens_k), len(lens_q), 64
     have = lib.flame_attn_packed_fwd_workspace_bytes(n, Tq, Tk, H, D)
     if have:
-        assert have >= cut(lens_q, lens_k, H, 1, causal, 9) * H * 128 * (4 * D + 8)
+        assert have >= cut(lens_q, lens_k, H, 1, causal, 512, 16, 16, 1.6) * H * 128 * (4 * D + 8)
     more = lib.flame_attn_packed_bwd_workspace_bytes(n, Tq, Tk, H, Hkv, D) - 2 * -(-H * Tq * 4 // 256) * 256
     assert more >= 0
     slots = Tk // 128 + n + 1
     walked = Tq * (H // Hkv)
-    if walked // n >= 1024 and slots * Hkv * 2 < 3 * 256 and -(-walked // 64) - (slots - n) * Hkv * (walked // n // 128) // 256 > 16:
-        assert more >= cut(lens_k, lens_q, Hkv, H // Hkv, causal, 8) * Hkv * 2 * 128 * D * 4
+    if walked // n >= 768 and slots * Hkv * 2 < 3 * 256 and -(-walked // 64) - (slots - n) * Hkv * (walked // n // 128) // 256 > 12:
+        assert more >= cut(lens_k, lens_q, Hkv, H // Hkv, causal, 256, 8, 12, 0.65) * Hkv * 2 * 128 * D * 4
+    slots = Tq // 128 + n + 1
+    if Tk // n >= 768 and slots * H * 2 < 3 * 256 and -(-Tk // 64) - (slots - n) * H * (Tk // n // 128) // 256 > 12:
+        assert more >= cut(lens_q, lens_k, H, 1, causal, 512, 8, 12, 1.6) * H * 128 * D * 4
 
 
 def paged(lib, q=P, kc=P, o=P, table=P, stride=8, pages=8, kv_len=P, prefix=NULL, prefix_pages=0, prefix_len=NULL, B=2, H=4, H_kv=2, N=1, D=64, n_pages=20,
