@@ -170,6 +170,12 @@ def test_more_pages_than_a_wavefront_holds():
     assert ((lse[:, 0].double() - torch.logsumexp(s, 1)).abs() <= 1e-4).all()
 
 
+def test_the_largest_pages():
+    """65536 tokens in a page: one page, a page and a bit, part of one."""
+    run(12, [65536, 65537, 300], 2, 1, 1, 8, 65536, spare=1)
+    run(13, [1000, 1], 2, 1, 3, 8, 65536, prefix=65000, spare=1)
+
+
 def test_offsets_past_32_bits():
     """Pages whose first element lies more than 2^32 elements into the cache."""
     from flame_amd import capi
