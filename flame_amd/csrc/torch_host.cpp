@@ -850,6 +850,7 @@ struct SdpaPacked : public torch::autograd::Function<SdpaPacked> {
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
         const auto saved = ctx->get_saved_variables();
         const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &o = saved[3], &lse = saved[4], &cu_q = saved[5], &cu_k = saved[6];
+        TORCH_CHECK(!at::GradMode::is_enabled(), "packed attention has no second derivative: its gradients would count as constants (create_graph=True)");
         c10::OptionalDeviceGuard device(q.device());
         at::NoGradGuard no_grad;
         const PackedSizes z = checked_sizes(q, k, cu_q);

@@ -39,7 +39,8 @@ def sdpa_with_bias(q, k, v, bias=None, scale=None):
 
 def sdpa_packed(q, k, v, cu_seqlens, cu_seqlens_k=None, is_causal=None, scale=None):
     """Attention of sequences of different lengths packed one behind the other: q [rows, H, D], k/v [key rows, H_kv, D],
-    H a multiple of H_kv (head h reads key head h // (H // H_kv)).  Differentiable.
+    H a multiple of H_kv (head h reads key head h // (H // H_kv)).  Differentiable, once: a backward with create_graph=True is
+    refused.
 
     cu_seqlens (and cu_seqlens_k where the keys have other lengths): int32 [sequences + 1] on the device, the rows of
     sequence i being cu_seqlens[i] .. cu_seqlens[i + 1] - 1; a recorded graph holds them, so they may not be refilled before

@@ -160,6 +160,18 @@ def test_graph_of_autograd():
     del eager
 
 
+def test_a_second_derivative_is_refused():
+    from flame_amd import functional
+    _, (q, k, v, do, cq, ck) = inputs()
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    o = functional.sdpa_packed(*leaves, cq, is_causal=True)
+    first = torch.autograd.grad(o, leaves, do, retain_graph=True)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(o, leaves, do, create_graph=True)
+    again = torch.autograd.grad(o, leaves, do)
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
 def test_another_stream():
     from flame_amd import functional
     _, (q, k, v, do, cq, ck) = inputs(4, lens=(500, 300))
