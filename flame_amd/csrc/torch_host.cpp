@@ -15,6 +15,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <unordered_set>
 #include <vector>
 
 #include <ATen/ATen.h>
@@ -865,12 +866,20 @@ struct SdpaPacked : public torch::autograd::Function<SdpaPacked> {
 // A leaf whose gradients an earlier graph, still alive, accumulates on another stream: its backward would wait for that stream, which
 // in a capture is an error that the autograd engine does not survive.  Refused where the capture can still be told.
 void check_capture(const Tensor& t) {
-    if (!t.requires_grad() || !t.is_leaf()) return;
-    const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
-    if (!node) return;
-    const auto stream = node->stream();
+    if (!t.requires_grad()) return;
     const c10::Stream now = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).unwrap();
-    TORCH_CHECK(!stream || *stream == now, "packed attention: a graph recorded on another stream holds one of the leaves; delete it before its backward is captured");
+    const auto first = t.is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(t) : t.grad_fn();
+    std::vector<torch::autograd::Node*> todo{first.get()};
+    std::unordered_set<torch::autograd::Node*> seen;
+    while (!todo.empty()) {
+        torch::autograd::Node* const node = todo.back();
+        todo.pop_back();
+        if (!node || !seen.insert(node).second) continue;
+        for (const auto& edge : node->next_edges()) todo.push_back(edge.function.get());
+        if (!dynamic_cast<torch::autograd::AccumulateGrad*>(node)) continue;
+        const auto stream = node->stream();
+        TORCH_CHECK(!stream || *stream == now, "packed attention: a graph recorded on another stream holds one of the leaves; delete it before its backward is captured");
+    }
 }
 
 // sdpa_packed(q, k, v, cu_q, cu_k | None, causal, scale | None)

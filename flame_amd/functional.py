@@ -47,8 +47,8 @@ def sdpa_packed(q, k, v, cu_seqlens, cu_seqlens_k=None, is_causal=None, scale=No
     its backward.  is_causal=True: query i of a sequence attends to keys j <= i + (keys - queries), the last query to
     all of them.  Queries without a key and rows behind the last sequence come out as zeros, with zero gradients.
     Inputs of another dtype are promoted to bf16 and the result is cast back.
-    Its backward may be captured into a graph; a leaf that an eager graph recorded on another stream still holds is refused
-    in the capture."""
+    Its backward may be captured into a graph; a leaf that q, k or v come from and that an eager graph recorded on another
+    stream still holds is refused in the capture."""
     return capi.host().sdpa_packed(q, k, v, cu_seqlens, cu_seqlens_k, is_causal is not None and bool(is_causal), scale)
 
 

@@ -158,6 +158,15 @@ def test_graph_of_autograd():
         with pytest.raises(RuntimeError, match="another stream"):
             functional.sdpa_packed(*held, cq, is_causal=True)
     del eager
+    both = torch.cat([q, k, v], 1).requires_grad_(True)                # one leaf, seen by views
+    parts = lambda: (both[:, :4], both[:, 4:4 + k.shape[1]], both[:, 4 + k.shape[1]:])
+    eager = functional.sdpa_packed(*parts(), cq, is_causal=True)
+    torch.cuda.synchronize()
+    other = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(other, stream=side):
+        with pytest.raises(RuntimeError, match="another stream"):
+            functional.sdpa_packed(*parts(), cq, is_causal=True)
+    del eager
 
 
 def test_a_second_derivative_is_refused():
