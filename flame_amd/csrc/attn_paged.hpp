@@ -19,7 +19,7 @@
 //
 // The number of keys is known on the device only.  The units are therefore cut there: every workgroup sums the tiles of the batch
 // and takes the unit length that gives about as many units as the device holds workgroups.
-// Short tables (PagedDirect) need none of this: one workgroup per sequence, key head and 32 rows takes all keys and writes O itself.
+// Short tables (paged_direct_kernel) need none of this: one workgroup per sequence, key head and 32 rows takes all keys and writes O itself.
 #pragma once
 #include "attn_common.hpp"
 #include "packed_units.hpp"
