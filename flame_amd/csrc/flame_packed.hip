@@ -43,7 +43,6 @@ int set_lds(const void* kern, int bytes, std::atomic<uint64_t>& done) {      // 
 
 template <class P>
 int launch(void (*kern)(P, PackedArgs), int lds, std::atomic<uint64_t>& done, int64_t units, int heads, const P& p, const PackedArgs& a, hipStream_t s, int threads = 256) {
-    if (units * heads > INT32_MAX) return FLAME_ATTN_ERR_UNSUPPORTED;
     if (const int rc = set_lds(reinterpret_cast<const void*>(kern), lds, done)) return rc;
     hipLaunchKernelGGL(kern, dim3((unsigned)(units * heads)), dim3(threads), (size_t)lds, s, p, a);
     return (int)hipGetLastError();
@@ -56,6 +55,12 @@ int launch_merge(void (*kern)(P, PackedArgs), int64_t tiles, int heads, int bloc
 
 int padded(int D) { return D <= 64 ? 64 : D <= 96 ? 96 : 128; }
 size_t align256(size_t x) { return (x + 255) / 256 * 256; }
+
+// Rows of a tensor.  The kernels and the rules here count tiles and steps of up to 128 rows in 32 bits, from sums such as T + 127 and, under the
+// causal flag, Sk + 255: a number of tiles that has become negative would be a place in front of the tensor.
+constexpr int kMostRows = INT32_MAX - 1023;
+// ... and a launch has fewer than 2^32 threads: 256 for every tile of every head
+bool grid_fits(int rows, int n_seqs, int heads) { return (double)packed_slots(rows, n_seqs, 128) * heads * 256.0 <= (double)UINT32_MAX; }
 
 // Two workgroups of queries per compute unit, one of keys (at D = 64 a second one fits).  The backward's steps are longer, so shorter parts pay
 // there (at least 16 steps each -> 8, us: 8 heads on 2 of 612 65 -> 51, 4 of 2000 72 -> 58, D = 64, 4 of 2000 50 -> 42; forward, 8 of 100 rows on 30000 keys
@@ -107,7 +112,7 @@ Parts fwd_parts(int n_seqs, int T_q, int T_kv, int H, int D) {
 }
 Parts dq_parts(int n_seqs, int T_q, int T_kv, int H, int D) { return parts_of(kCutDq, T_q, T_kv, n_seqs, H, (size_t)128 * padded(D) * sizeof(float)); }
 Parts dkdv_parts(int n_seqs, int T_q, int T_kv, int H, int H_kv, int D) {
-    return parts_of(cut_dkdv(D), T_kv, (int)std::min<int64_t>((int64_t)T_q * (H / H_kv), INT32_MAX), n_seqs, H_kv, (size_t)2 * 128 * padded(D) * sizeof(float));
+    return parts_of(cut_dkdv(D), T_kv, (int)std::min<int64_t>((int64_t)T_q * (H / H_kv), kMostRows), n_seqs, H_kv, (size_t)2 * 128 * padded(D) * sizeof(float));
 }
 
 // One launch for the sums of the parts: with few tiles a workgroup per eight columns, with more one per 32.  (Per 32 -> per eight, us: 8 tiles of 30
@@ -155,7 +160,7 @@ size_t bwd_rows_bytes(int H, int T_q) { return 2 * align256((size_t)H * T_q * si
 int check_sizes(const void* cu_q, const void* cu_k, int n_seqs, int T_q, int T_kv, int H, int H_kv, int D, float scale) {
     if (!cu_q || !cu_k || n_seqs <= 0 || T_q <= 0 || T_kv <= 0 || H <= 0 || H_kv <= 0 || D <= 0) return FLAME_ATTN_ERR_INVALID;
     if (H % H_kv != 0 || !(scale > 0.f) || !std::isfinite(scale)) return FLAME_ATTN_ERR_INVALID;
-    return head_dim_ok(D) ? FLAME_ATTN_OK : FLAME_ATTN_ERR_UNSUPPORTED;
+    return head_dim_ok(D) && T_q <= kMostRows && T_kv <= kMostRows && grid_fits(T_q, n_seqs, H) ? FLAME_ATTN_OK : FLAME_ATTN_ERR_UNSUPPORTED;
 }
 
 }  // namespace
@@ -163,7 +168,7 @@ int check_sizes(const void* cu_q, const void* cu_k, int n_seqs, int T_q, int T_k
 extern "C" {
 
 size_t flame_attn_packed_fwd_workspace_bytes(int n_seqs, int T_q, int T_kv, int H, int D) {
-    if (n_seqs <= 0 || T_q <= 0 || T_kv <= 0 || H <= 0 || !head_dim_ok(D)) return 0;
+    if (n_seqs <= 0 || T_q <= 0 || T_kv <= 0 || T_q > kMostRows || T_kv > kMostRows || H <= 0 || !head_dim_ok(D)) return 0;
     return fwd_parts(n_seqs, T_q, T_kv, H, D).bytes;
 }
 
@@ -192,7 +197,7 @@ int flame_attn_packed_fwd_bf16(const void* Q, const void* K, const void* V, void
 }
 
 size_t flame_attn_packed_bwd_workspace_bytes(int n_seqs, int T_q, int T_kv, int H, int H_kv, int D) {
-    if (n_seqs <= 0 || T_q <= 0 || T_kv <= 0 || H <= 0 || H_kv <= 0 || H % H_kv != 0 || !head_dim_ok(D)) return 0;
+    if (n_seqs <= 0 || T_q <= 0 || T_kv <= 0 || T_q > kMostRows || T_kv > kMostRows || H <= 0 || H_kv <= 0 || H % H_kv != 0 || !head_dim_ok(D)) return 0;
     return bwd_rows_bytes(H, T_q) + std::max(dq_parts(n_seqs, T_q, T_kv, H, D).bytes, dkdv_parts(n_seqs, T_q, T_kv, H, H_kv, D).bytes);
 }
 
@@ -203,6 +208,7 @@ int flame_attn_packed_bwd_bf16(const void* Q, const void* K, const void* V, cons
                                const int64_t* dv_strides, int causal, void* workspace, size_t workspace_bytes, void* stream) {
     int rc;
     if ((rc = check_sizes(cu_q, cu_k, n_seqs, T_q, T_kv, H, H_kv, D, scale))) return rc;
+    if (!grid_fits(T_kv, n_seqs, H_kv)) return FLAME_ATTN_ERR_UNSUPPORTED;
     if (!LSE || !workspace || workspace_bytes < bwd_rows_bytes(H, T_q)) return FLAME_ATTN_ERR_INVALID;
     if (reinterpret_cast<uintptr_t>(workspace) & 15u) return FLAME_ATTN_ERR_UNSUPPORTED;
     if ((rc = check_rows(Q, q_strides)) || (rc = check_rows(K, k_strides)) || (rc = check_rows(V, v_strides)) || (rc = check_rows(O, o_strides)) ||

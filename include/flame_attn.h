@@ -235,6 +235,8 @@ int flame_attn_bwd_bf16_noalloc(const void* Q, const void* K, const void* V, con
  *   - Q, O [T_q, H, D], K, V [T_kv, H_kv, D], bf16; H a multiple of H_kv, head h reads key head h / (H / H_kv).  Strides: three
  *     ELEMENT strides in (row, head, D) order under the rules of the [B,H,N,D] views above (D stride 1, the others multiples of 8,
  *     row strides below 2^24, 16-byte aligned base); D any multiple of 8 up to 128.  Rows or heads of an output must not overlap.
+ *     At most 2^31 - 1024 rows, and fewer than 2^24 tiles of 128 rows: (T_q / 128 + n_seqs + 1) * H, in the backward also
+ *     (T_kv / 128 + n_seqs + 1) * H_kv.
  *   - cu_q, cu_k: int32 [n_seqs + 1] on the device; sequence i has the query rows cu_q[i] .. cu_q[i + 1] - 1 and the key rows
  *     cu_k[i] .. cu_k[i + 1] - 1.  They rise from 0 and end at or before T_q / T_kv; a sequence may have no rows.  (They are read on
  *     the device and cannot be refused: values that fall or lead outside are cut to the tensors, and the result is of no use.)
