@@ -77,6 +77,9 @@ struct PagedSizes {
 // 1000 13.0 -> 11.4, 64 of 1000 48 -> 42, 64 of 2000 97 -> 92, 64 of 200 to 2000 57 -> 52.  4 of 2000 15.4, one workgroup each 17.9.)
 constexpr int64_t kDirectKeys = 1024;
 
+// A launch has fewer than 2^32 threads.
+bool grid_fits(int64_t groups) { return groups * 256 <= (int64_t)UINT32_MAX; }
+
 // false: too large
 bool paged_sizes(int B, int H, int H_kv, int N, int D, int page, int pages, int prefix_pages, PagedSizes* z) {
     const int64_t rows = (int64_t)N * (H / H_kv), rt = (rows + 31) / 32;
@@ -86,6 +89,7 @@ bool paged_sizes(int B, int H, int H_kv, int N, int D, int page, int pages, int 
     if (own > INT32_MAX / 2 || prefix > INT32_MAX / 2 || (double)pages * page > INT32_MAX / 2 || (double)prefix_pages * page > INT32_MAX / 2) return false;
     const bool shared = PagedCut::shared((int)(B * rows));
     z->direct = prefix_pages == 0 && (int64_t)pages * page <= (B * H_kv * rt < PagedCut::kFill / 2 ? kDirectKeys : PagedCut::kLong * PagedCut::kTile);
+    if (!grid_fits(z->direct ? B * H_kv * rt : ((int64_t)B * H * N + 3) / 4)) return false;          // as launch_paged launches
     z->own_units = most_units((int64_t)own, B * H_kv * rt);
     z->prefix_units = shared ? most_shared_units((int64_t)prefix, H_kv * prefix_rt) : most_units((int64_t)prefix, H_kv * prefix_rt);
     z->prefix_rows = z->prefix_units * (shared ? 128 : 32);
@@ -191,6 +195,10 @@ int flame_kv_store_bf16(const void* K, const void* V, void* K_cache, void* V_cac
     if (!page_table || !cu || !start || n_seqs <= 0 || T <= 0 || H_kv <= 0 || D <= 0 || n_pages <= 0 || page <= 0 || table_pages <= 0 || table_stride < 0)
         return FLAME_ATTN_ERR_INVALID;
     if (D % 8 != 0 || (int64_t)H_kv * D > INT32_MAX / 2 || page_shift(page) < 0) return FLAME_ATTN_ERR_UNSUPPORTED;
+    // (a workgroup's rows are counted in 32 bits, also those past T)
+    const int rows_per_wave = std::max(1, 64 / (H_kv * (D / 8)));
+    const int64_t grid = ((int64_t)T + 4 * rows_per_wave - 1) / (4 * rows_per_wave);
+    if (T > INT32_MAX - 1023 || !grid_fits(grid)) return FLAME_ATTN_ERR_UNSUPPORTED;
     int rc;
     if ((rc = check_view(K, k_strides, 3)) || (rc = check_view(V, v_strides, 3)) || (rc = check_view(K_cache, kc_strides, 4)) || (rc = check_view(V_cache, vc_strides, 4)))
         return rc;
@@ -217,8 +225,7 @@ int flame_kv_store_bf16(const void* K, const void* V, void* K_cache, void* V_cac
     p.d = D;
     p.n_pages = n_pages;
     p.page_shift = page_shift(page);
-    p.rows_per_wave = std::max(1, 64 / (H_kv * (D / 8)));
-    const int64_t grid = ((int64_t)T + 4 * p.rows_per_wave - 1) / (4 * p.rows_per_wave);
+    p.rows_per_wave = rows_per_wave;
     hipLaunchKernelGGL(kv_store_kernel, dim3((unsigned)grid), dim3(256), 0, static_cast<hipStream_t>(stream), p);
     return (int)hipGetLastError();
 }

@@ -290,7 +290,8 @@ int flame_attn_packed_bwd_bf16(const void* Q, const void* K, const void* V, cons
  * h / (H / H_kv).  D any multiple of 8 up to 128.  LSE: fp32, contiguous [B*H, N], or null.
  * `workspace`: device memory, 16-byte aligned, of at least flame_attn_paged_workspace_bytes(...) bytes (0: none is needed, or the
  * call would be refused), used only during the call; nothing in it has to start at any value.  Calls that overlap (other streams,
- * captured graphs that run at once) need one each.
+ * captured graphs that run at once) need one each.  At most 2^26 - 4 rows of O, B * H * N (short tables, which need no
+ * workspace: at most 2^24 - 1 times one sequence, key head and 32 of its N * H / H_kv rows).
  * The results do not depend on the order in which workgroups finish.  Inference only. */
 size_t flame_attn_paged_workspace_bytes(int B, int H, int H_kv, int N, int D, int page, int table_pages, int prefix_pages);
 int flame_attn_paged_fwd_bf16(const void* Q, const void* K_cache, const void* V_cache, void* O, void* LSE,
@@ -303,7 +304,8 @@ int flame_attn_paged_fwd_bf16(const void* Q, const void* K_cache, const void* V_
 /* Rows K, V [T, H_kv, D] (three element strides in (row, head, D) order) of n_seqs sequences, sequence b having the rows
  * cu[b] .. cu[b + 1] - 1 (int32 [n_seqs + 1] on the device, rising from 0), to the places start[b], start[b] + 1, ... of their pages.
  * Rows behind the last sequence are not stored.  Two rows for one place leave either of them.  D any multiple of 8.  K_cache and
- * V_cache are different tensors (one pointer for both is FLAME_ATTN_ERR_INVALID). */
+ * V_cache are different tensors (one pointer for both is FLAME_ATTN_ERR_INVALID).  At most 2^31 - 1024 rows; rows of more
+ * than 256 elements (H_kv * D): at most 2^26 - 4. */
 int flame_kv_store_bf16(const void* K, const void* V, void* K_cache, void* V_cache, const int32_t* page_table,
                         int64_t table_stride, int table_pages, const int32_t* cu, const int32_t* start, int n_seqs, int T, int H_kv,
                         int D, int n_pages, int page, const int64_t* k_strides, const int64_t* v_strides,

@@ -43,3 +43,27 @@ def test_packed_grids(lib):  # noqa: F811
         assert packed_bwd(lib, null=True, T_kv=T + more, H=heads, H_kv=heads) == code
     assert packed_fwd(lib, q=NULL, n=2 ** 23, H=1, H_kv=1) == INVALID and packed_fwd(lib, q=NULL, n=2 ** 24, H=1, H_kv=1) == UNSUPPORTED
     assert packed_fwd(lib, q=NULL, T_kv=T + 128, H=heads, H_kv=heads) == INVALID          # the forward has no tiles of keys
+
+
+@pytest.mark.parametrize("H_kv,D,rows", [(1, 8, 64), (1, 64, 8), (3, 40, 4), (8, 128, 1), (2, 256, 1)])
+def test_stored_rows(lib, H_kv, D, rows):  # noqa: F811
+    """`rows` rows in a wavefront, four of these in a workgroup of 256 threads."""
+    size = dict(H_kv=H_kv, D=D, k=NULL)
+    most = min(MOST, (2 ** 24 - 1) * 4 * rows)
+    assert store(lib, T=most, **size) == INVALID
+    for T in (most + 1, 2 ** 31 - 1):
+        assert store(lib, T=T, **size) == UNSUPPORTED
+
+
+def test_paged_grids(lib):  # noqa: F811
+    """One workgroup of 256 threads for every sequence, key head and 32 rows where a table is short; else one for four rows of the result."""
+    assert paged(lib, B=2 ** 18, H=64, H_kv=64, D=8, pages=1) == UNSUPPORTED
+    one = dict(H=2 ** 10, H_kv=1, D=8, qs=(2 ** 13, 8, 8, 1), os_=(2 ** 13, 8, 8, 1), pages=129, ws=NULL)
+    assert paged(lib, B=2 ** 16 - 1, **one) == INVALID and paged(lib, B=2 ** 16, **one) == UNSUPPORTED
+    f = lib.flame_attn_paged_workspace_bytes
+    assert f(2 ** 16 - 1, 2 ** 10, 1, 1, 8, 16, 129, 0) > 0 and f(2 ** 16, 2 ** 10, 1, 1, 8, 16, 129, 0) == 0
+
+
+def test_copied_pages(lib):  # noqa: F811
+    """Pages of up to 2^30 elements, 65535 layers: their grids are within the limits."""
+    assert copies(lib, [0], [1], kc=NULL, layers=65535) == INVALID and copies(lib, [0], [1], kc=NULL, layers=65536) == UNSUPPORTED
