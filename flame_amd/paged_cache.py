@@ -117,7 +117,8 @@ class PagedCache:
 
         A last page that is partly filled and shared is copied first (all copies of the call in one launch per 400).  With
         share_prefix, whole pages that all sequences have in common at their beginning, before every new token, are listed
-        once as the batch's prefix.  Without enough free pages: MemoryError, and nothing has changed."""
+        once as the batch's prefix.  Without enough free pages: MemoryError.  Where this or anything else is raised, the book is
+        as it was."""
         seqs, counts = list(seqs), [int(n) for n in counts]
         if not seqs or len(seqs) != len(counts) or min(counts) < 0 or len(set(seqs)) < len(seqs):
             raise ValueError("different sequences, each with a number of new tokens")
@@ -136,36 +137,48 @@ class PagedCache:
             shared.append(copy)
         if sum(need) + sum(shared) > len(self._free):
             raise MemoryError(f"the cache has {len(self._free)} free pages and needs {sum(need) + sum(shared)}")
-        src, dst = [], []
-        for seq, n, more, copy in zip(seqs, counts, need, shared):
-            pages = self._pages[seq]
-            if copy:
-                src.append(pages[-1])
-                self._users[pages[-1]] -= 1
-                pages[-1] = heapq.heappop(self._free)
-                self._users[pages[-1]] = 1
-                dst.append(pages[-1])
-            for _ in range(more):
-                pages.append(heapq.heappop(self._free))
-                self._users[pages[-1]] = 1
+        taken, src, dst, lists = [], [], [], []
+        try:
+            for seq, more, copy in zip(seqs, need, shared):
+                pages, new = self._pages[seq], []
+                for _ in range(copy + more):
+                    taken.append(heapq.heappop(self._free))
+                    new.append(taken[-1])
+                if copy:
+                    src.append(pages[-1])
+                    dst.append(new[0])
+                    pages = pages[:-1]
+                lists.append(pages + new if new else pages)
+            if src:
+                capi.kv_copy_pages(self.k, self.v, src, dst)
+            batch = self._batch(lists, [self._len[s] + n for s, n in zip(seqs, counts)], counts, share_prefix)
+        except BaseException:
+            for p in taken:
+                heapq.heappush(self._free, p)
+            raise
+        # the copies and the upload were accepted: the book follows
+        for p in src:
+            self._users[p] -= 1
+        for p in taken:
+            self._users[p] = 1
+        for seq, n, pages in zip(seqs, counts, lists):
+            self._pages[seq] = pages
             self._len[seq] += n
-        if src:
-            capi.kv_copy_pages(self.k, self.v, src, dst)
-        return self._batch(seqs, counts, share_prefix)
+        return batch
 
-    def _batch(self, seqs, counts, share_prefix) -> PagedBatch:
-        lists = [self._pages[s] for s in seqs]
+    def _batch(self, lists, lens, counts, share_prefix) -> PagedBatch:
+        """Tables of sequences with these pages and lengths, the last counts[i] tokens of which are new."""
         common = 0
-        if share_prefix and len(seqs) > 1:
-            most = min(self._len[s] - n for s, n in zip(seqs, counts)) // self.page
+        if share_prefix and len(lists) > 1:
+            most = min(m - n for m, n in zip(lens, counts)) // self.page
             first = lists[0]
             common = next((i for i in range(most) if any(x[i] != first[i] for x in lists)), most)
-        B, width, held = len(seqs), max(1, max(len(x) for x in lists) - common), common * self.page
+        B, width, held = len(lists), max(1, max(len(x) for x in lists) - common), common * self.page
         data = lists[0][:common] + [held]
         for x in lists:
             row = x[common:]
             data += row + [0] * (width - len(row))
-        data += [self._len[s] - held for s in seqs] + [self._len[s] - n - held for s, n in zip(seqs, counts)]
+        data += [m - held for m in lens] + [m - n - held for m, n in zip(lens, counts)]
         at = [0]
         for n in counts:
             at.append(at[-1] + n)
