@@ -205,13 +205,15 @@ def attn_paged_fwd(q, k_cache, v_cache, page_table, kv_len, scale, prefix_table=
 
 def kv_store(k, v, k_cache, v_cache, page_table, cu, start):
     """flame_kv_store_bf16(...): rows k, v [rows, H_kv, D] of the sequences that cu (int32 [sequences + 1]) bounds to the
-    places start[b], start[b] + 1, ... (int32 [sequences]) of their pages."""
+    places start[b], start[b] + 1, ... (int32 [sequences]) of their pages.  Autograd records nothing: inputs that require a gradient
+    are refused while it is enabled, and a graph that saved a view of the caches raises in its backward."""
     host().kv_store(k, v, k_cache, v_cache, page_table, cu, start)
 
 
 def kv_copy_pages(k_cache, v_cache, src, dst):
     """flame_kv_copy_pages_bf16(...): page src[i] to page dst[i] (sequences of ints) in both caches, [pages, H_kv, page, D]
-    or [layers, pages, H_kv, page, D], in all layers.  A page that is written twice, or read and written, is refused."""
+    or [layers, pages, H_kv, page, D], in all layers.  A page that is written twice, or read and written, is refused.
+    Autograd is told what kv_store tells it."""
     host().kv_copy_pages(k_cache, v_cache, src, dst)
 
 

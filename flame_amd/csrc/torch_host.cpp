@@ -986,6 +986,21 @@ void check_table(const Tensor& t, int64_t n, const Tensor& like) {
 }
 const int32_t* ints(const Tensor& t) { return static_cast<const int32_t*>(ptr(t)); }
 
+// Inputs of a call that autograd knows nothing of: what they carry would be lost without a word.
+void check_no_derivative(std::initializer_list<const Tensor*> inputs, const char* call) {
+    for (const Tensor* t : inputs) TORCH_CHECK_NOT_IMPLEMENTED(!t->_fw_grad(0).defined(), call, " has no forward-mode derivative: an input carries a tangent");
+    if (!at::GradMode::is_enabled()) return;
+    for (const Tensor* t : inputs)
+        TORCH_CHECK(!t->requires_grad(), call, " has no backward and an input requires a gradient: call it under torch.no_grad()");
+}
+// A launch may have written to the caches: graphs that saved them, or views of them, are told (rc: not one of the refusals that come before any
+// launch).  A tensor of inference mode is in no graph and has no version.
+void raise_versions(int rc, std::initializer_list<const Tensor*> written) {
+    if (rc == FLAME_ATTN_ERR_INVALID || rc == FLAME_ATTN_ERR_UNSUPPORTED) return;
+    for (const Tensor* t : written)
+        if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
 struct PagedCall {
     Tensor table, kv_len, prefix_table, prefix_len;
 };
@@ -1071,6 +1086,7 @@ PyObject* py_kv_store(PyObject*, PyObject* const* a, Py_ssize_t n) {
         need_args(n, 7);
         const Tensor &k = tensor_arg(a[0], "k"), &v = tensor_arg(a[1], "v"), &kc = tensor_arg(a[2], "k_cache"), &vc = tensor_arg(a[3], "v_cache"),
                      &table = tensor_arg(a[4], "page_table"), &cu = tensor_arg(a[5], "cu"), &start = tensor_arg(a[6], "start");
+        check_no_derivative({&k, &v, &kc, &vc}, "a store into the cache");
         if (k.dim() != 3) fail(PyExc_ValueError, "k and v are 3-D [rows, key heads, D]");
         check_caches(kc, vc, 4, "the caches are 4-D [pages, key heads, page, D]");
         check_that(k.sizes() == v.sizes() && k.numel() > 0 && k.size(1) == kc.size(1) && k.size(2) == kc.size(3), "k and v have one shape, with the caches' heads and head dim");
@@ -1085,10 +1101,11 @@ PyObject* py_kv_store(PyObject*, PyObject* const* a, Py_ssize_t n) {
         {
             WithoutGil nogil;
             c10::OptionalDeviceGuard device(kc.device());
-            check_rc(g_api.flame_kv_store_bf16(ptr(k), ptr(v), ptr(kc), ptr(vc), ints(table), table.stride(0), (int)table.size(1), ints(cu), ints(start),
-                                               (int)table.size(0), (int)k.size(0), (int)k.size(1), (int)k.size(2), (int)kc.size(0), (int)kc.size(2), strides4(k),
-                                               strides4(v), strides4(kc), strides4(vc), stream_of(kc)),
-                     "flame_kv_store_bf16");
+            const int rc = g_api.flame_kv_store_bf16(ptr(k), ptr(v), ptr(kc), ptr(vc), ints(table), table.stride(0), (int)table.size(1), ints(cu), ints(start),
+                                                     (int)table.size(0), (int)k.size(0), (int)k.size(1), (int)k.size(2), (int)kc.size(0), (int)kc.size(2),
+                                                     strides4(k), strides4(v), strides4(kc), strides4(vc), stream_of(kc));
+            raise_versions(rc, {&kc, &vc});
+            check_rc(rc, "flame_kv_store_bf16");
         }
         return Py_NewRef(Py_None);
     });
@@ -1116,7 +1133,9 @@ std::vector<int32_t> int_list(PyObject* o) {
 PyObject* py_kv_copy_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
         need_args(n, 4);
-        Tensor kc = tensor_arg(a[0], "k_cache"), vc = tensor_arg(a[1], "v_cache");
+        const Tensor &k_cache = tensor_arg(a[0], "k_cache"), &v_cache = tensor_arg(a[1], "v_cache");
+        check_no_derivative({&k_cache, &v_cache}, "a copy of pages");
+        Tensor kc = k_cache, vc = v_cache;
         if (kc.dim() == 4 && vc.dim() == 4) kc = kc.unsqueeze(0), vc = vc.unsqueeze(0);
         check_caches(kc, vc, 5, "the caches are [pages, key heads, page, D], with the layers in front or without");
         const std::vector<int32_t> src = int_list(a[2]), dst = int_list(a[3]);
@@ -1126,9 +1145,10 @@ PyObject* py_kv_copy_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
         {
             WithoutGil nogil;
             c10::OptionalDeviceGuard device(kc.device());
-            check_rc(g_api.flame_kv_copy_pages_bf16(ptr(kc), ptr(vc), (int)kc.size(0), (int)kc.size(1), (int)kc.size(2), (int)kc.size(3), (int)kc.size(4),
-                                                    strides4(kc), strides4(vc), src.data(), dst.data(), (int)src.size(), stream_of(kc)),
-                     "flame_kv_copy_pages_bf16");
+            const int rc = g_api.flame_kv_copy_pages_bf16(ptr(kc), ptr(vc), (int)kc.size(0), (int)kc.size(1), (int)kc.size(2), (int)kc.size(3),
+                                                          (int)kc.size(4), strides4(kc), strides4(vc), src.data(), dst.data(), (int)src.size(), stream_of(kc));
+            if (!src.empty()) raise_versions(rc, {&k_cache, &v_cache});
+            check_rc(rc, "flame_kv_copy_pages_bf16");
         }
         return Py_NewRef(Py_None);
     });

@@ -187,7 +187,8 @@ class PagedCache:
         return PagedBatch(table.view(B, width), kv_len, start, cu, prefix if common else None, length if common else None, counts)
 
     def store(self, layer, k, v, batch) -> None:
-        """Rows k, v [new tokens of the batch, kv_heads, head_dim], sequence after sequence, to their places."""
+        """Rows k, v [new tokens of the batch, kv_heads, head_dim], sequence after sequence, to their places.  Inference only, as `attend`: rows
+        that require a gradient are refused unless torch.no_grad() is on."""
         if k.shape[0] != sum(batch.counts):
             raise ValueError("as many rows as the batch has new tokens")
         if not k.shape[0]:
