@@ -888,9 +888,9 @@ PyObject* py_sdpa_packed(PyObject*, PyObject* const* a, Py_ssize_t n) {
         need_args(n, 7);
         const Tensor &q = tensor_arg(a[0], "q"), &k = tensor_arg(a[1], "k"), &v = tensor_arg(a[2], "v"), &cu_q = tensor_arg(a[3], "cu_seqlens");
         const Tensor& cu_k = a[4] == Py_None ? cu_q : tensor_arg(a[4], "cu_seqlens_k");
-        const PackedSizes z = packed_sizes(q, k, v, cu_q, cu_k);
         for (const Tensor* t : {&q, &k, &v})
             TORCH_CHECK_NOT_IMPLEMENTED(!t->_fw_grad(0).defined(), "packed attention has no forward-mode derivative: an input carries a tangent");
+        const PackedSizes z = packed_sizes(q, k, v, cu_q, cu_k);
         const bool causal = bool_arg(a[5]);
         const double scale = a[6] == Py_None ? 1.0 / std::sqrt((double)z.D) : float_arg(a[6]);
         Tensor out;
@@ -1041,9 +1041,8 @@ PyObject* py_sdpa_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
         need_args(n, 8);
         const Tensor &q = tensor_arg(a[0], "q"), &kc = tensor_arg(a[1], "k_cache"), &vc = tensor_arg(a[2], "v_cache");
         const PagedCall c{tensor_arg(a[3], "page_table"), tensor_arg(a[4], "kv_len"), opt_tensor_arg(a[5], "prefix_table"), opt_tensor_arg(a[6], "prefix_len")};
+        check_no_derivative({&q, &kc, &vc}, "paged attention");
         check_paged(q, kc, vc, c);
-        TORCH_CHECK(!at::GradMode::is_enabled() || !(q.requires_grad() || kc.requires_grad() || vc.requires_grad()),
-                    "paged attention has no backward and an input requires a gradient: call it under torch.no_grad()");
         const float scale = (float)(a[7] == Py_None ? 1.0 / std::sqrt((double)q.size(3)) : float_arg(a[7]));
         Tensor o, lse;
         {

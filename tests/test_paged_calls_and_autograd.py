@@ -100,3 +100,31 @@ def test_caches_of_inference_mode():
     y["k"].requires_grad_(True)
     with torch.no_grad():
         store(y)
+
+
+@pytest.mark.parametrize("recorded", [False, True])
+def test_forward_mode_of_the_attention_calls(recorded):
+    """There is no forward-mode derivative, and a result without a tangent would mean a derivative of zero."""
+    x = inputs("cpu")
+    q = torch.randn(2, 4, 1, D).to(torch.bfloat16)
+    paged = [q, x["kc"], x["vc"], x["table"], torch.tensor([3, 4], dtype=torch.int32)]
+    packed = [torch.randn(5, 4, D).to(torch.bfloat16), x["k"], x["v"], x["cu"]]
+    for call, args in ((functional.sdpa_paged, paged), (functional.sdpa_packed, packed)):
+        for which in range(3):
+            with fwad.dual_level():
+                dual = list(args)
+                dual[which] = fwad.make_dual(dual[which].clone().requires_grad_(recorded), torch.ones_like(dual[which]))
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    call(*dual)
+                with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+                    call(*dual)
+
+
+def test_gradients_of_paged_attention():
+    x = inputs("cpu")
+    args = [torch.randn(2, 4, 1, D).to(torch.bfloat16), x["kc"], x["vc"], x["table"], torch.tensor([3, 4], dtype=torch.int32)]
+    for which in range(3):
+        leaves = list(args)
+        leaves[which] = leaves[which].clone().requires_grad_(True)
+        with pytest.raises(RuntimeError, match="no backward"):
+            functional.sdpa_paged(*leaves)
