@@ -941,6 +941,8 @@ PyObject* py_attn_packed_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
         need_args(n, 14);
         const Tensor &q = tensor_arg(a[0], "q"), &k = tensor_arg(a[1], "k"), &v = tensor_arg(a[2], "v"), &o = tensor_arg(a[3], "o"),
                      &d_o = tensor_arg(a[4], "do"), &lse = tensor_arg(a[5], "lse"), &cu_q = tensor_arg(a[6], "cu_q"), &cu_k = tensor_arg(a[7], "cu_k");
+        Grads g{opt_tensor_arg(a[11], "dq"), opt_tensor_arg(a[12], "dk"), opt_tensor_arg(a[13], "dv")};
+        check_that(g.dq.defined() == g.dk.defined() && g.dq.defined() == g.dv.defined(), "all three gradients or none");
         const PackedSizes z = packed_sizes(q, k, v, cu_q, cu_k);
         for (const Tensor* t : {&q, &k, &v}) check_that(t->scalar_type() == at::kBFloat16, "q, k and v are bf16");
         check_bf16_like(o, q, "o is a bf16 tensor of q's shape");
@@ -950,9 +952,7 @@ PyObject* py_attn_packed_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const bool causal = bool_arg(a[9]);
         const Tensor ws = opt_tensor_arg(a[10], "workspace");
         if (ws.defined()) check_workspace(ws, q);
-        Grads g{opt_tensor_arg(a[11], "dq"), opt_tensor_arg(a[12], "dk"), opt_tensor_arg(a[13], "dv")};
         if (g.dq.defined()) {
-            check_that(g.dk.defined() && g.dv.defined(), "all three gradients or none");
             check_bf16_like(g.dq, q, "dq is a bf16 tensor of q's shape");
             check_bf16_like(g.dk, k, "dk is a bf16 tensor of k's shape");
             check_bf16_like(g.dv, v, "dv is a bf16 tensor of v's shape");
