@@ -270,6 +270,10 @@ __device__ __forceinline__ float bf16_hi(uint32_t w) { return __builtin_bit_cast
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }   // v_exp_f32
 __device__ __forceinline__ float log2_fast(float x) { return __builtin_amdgcn_logf(x); }    // v_log_f32
 
+// By how much a score may exceed the running maximum that the exponentials take: 2^8 in the exponent domain, c = scale log2 e.  (Bounded:
+// 8 / c is infinite for scales below 1.6e-38, and a maximum of -inf plus that is NaN, which no score ever exceeds.)
+__device__ __forceinline__ float stale_scope(float c) { return fminf(8.0f / c, 3e38f); }
+
 // exchange with the lane 32 positions away (the other half of the wave)
 __device__ __forceinline__ float xhalf(float x) { return __shfl_xor(x, 32, 64); }
 

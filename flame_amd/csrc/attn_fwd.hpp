@@ -279,7 +279,7 @@ __device__ __forceinline__ void fwd_body(const FwdParams& p, const PackedUnit& u
 
     // ---- running state; each lane serves query column n
     const float c_log2 = p.scale * kLog2e;
-    const float stale_ok = 8.0f / c_log2;     // the reference maximum may lag the true one by 2^8
+    const float stale_ok = stale_scope(c_log2);     // the reference maximum may lag the true one by 2^8
     float m_run = -INFINITY, l_run = 0.f;
     f32x16 oacc[DB];
 #pragma unroll
@@ -909,7 +909,7 @@ __global__ __launch_bounds__(256) void fwd_wide_kernel(const FwdParams p) {
 
     // ---- running state; each lane serves query column n of both blocks
     const float c_log2 = p.scale * kLog2e;
-    const float stale_ok = 8.0f / c_log2;
+    const float stale_ok = stale_scope(c_log2);
     float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
     f32x16 oacc[2][DB];
 #pragma unroll

@@ -157,7 +157,7 @@ __global__ __launch_bounds__(64 * NW) void fwd_bigd_kernel(const FwdParams p) {
     }
 
     const float c_log2 = p.scale * kLog2e;
-    const float stale_ok = 8.0f / c_log2;     // the reference maximum may lag the true one by 2^8
+    const float stale_ok = stale_scope(c_log2);     // the reference maximum may lag the true one by 2^8
     float m_run = -INFINITY, l_run = 0.f;
     f32x16 oacc[NC][NDB];
 #pragma unroll

@@ -287,7 +287,7 @@ struct PagedRows {
             for (int db = 0; db < DB; ++db) voff[half][db] = row * RS + (((4 * db + 2 * tr_g16 + ((tr_r & 3) >> 1)) ^ swz<D>(row)) << 3) + 4 * (tr_r & 1);
         }
         c_log2 = p.scale * kLog2e;
-        stale_ok = fminf(8.0f / c_log2, 3e38f);        // the reference maximum may lag the true one by 2^8 (an infinite scope would never let the first one in)
+        stale_ok = stale_scope(c_log2);        // the reference maximum may lag the true one by 2^8
 #pragma unroll
         for (int db = 0; db < DB; ++db)
 #pragma unroll
