@@ -27,6 +27,7 @@
 #include "fast_div.hpp"
 #include "attn_fwd.hpp"
 #include "attn_fwd_bigd.hpp"
+#include "attn_fwd_merge.hpp"
 #include "attn_fwd_keyshare.hpp"
 #include "query_tile.hpp"
 #include "prep.hpp"
