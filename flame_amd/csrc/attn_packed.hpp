@@ -25,7 +25,7 @@ template <int D>
 __global__ __launch_bounds__(256, 2) void fwd_packed_kernel(const FwdParams p, const PackedArgs a) {
     constexpr int BM = 128;
     PackedUnit u;
-    const PackedWork work = packed_unit<BM, false, true>(a, (int)blockIdx.x, u);
+    const PackedWork work = packed_unit<BM, false>(a, (int)blockIdx.x, u);
     if (work == kPackedIdle) return;
     if (work == kPackedBehind) {
         packed_zero_rows<BM>(p.o + u.q_at(p.os), p.os.n, u.tile, u.Sq, p.dv);
@@ -42,7 +42,7 @@ template <int D, int NW>
 __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void fwd_packed_keyshare_kernel(const FwdParams p, const PackedArgs a) {
     constexpr int BM = 32;
     PackedUnit u;
-    const PackedWork work = packed_unit<BM, false, true>(a, (int)blockIdx.x, u);
+    const PackedWork work = packed_unit<BM, false>(a, (int)blockIdx.x, u);
     if (work == kPackedIdle) return;
     if (work == kPackedBehind) {
         packed_zero_rows<BM>(p.o + u.q_at(p.os), p.os.n, u.tile, u.Sq, p.dv);
@@ -68,7 +68,7 @@ template <int D>
 __global__ __launch_bounds__(256, 2) void bwd_dq_packed_kernel(const BwdParams p, const PackedArgs a) {
     constexpr int BM = 128;
     PackedUnit u;
-    const PackedWork work = packed_unit<BM, false, true>(a, (int)blockIdx.x, u);
+    const PackedWork work = packed_unit<BM, false>(a, (int)blockIdx.x, u);
     if (work == kPackedIdle) return;
     if (work == kPackedBehind) {
         packed_zero_rows<BM>(p.dq + u.q_at(p.dqs), p.dqs.n, u.tile, u.Sq, p.d);
@@ -81,7 +81,7 @@ template <int D>
 __global__ __launch_bounds__(256) void bwd_dkdv_packed_kernel(const BwdParams p, const PackedArgs a) {
     constexpr int BN = BwdTile<D>::BN;
     PackedUnit u;
-    const PackedWork work = packed_unit<BN, true, false>(a, (int)blockIdx.x, u);
+    const PackedWork work = packed_unit<BN, true>(a, (int)blockIdx.x, u);
     if (work == kPackedIdle) return;
     if (work == kPackedBehind) {
         packed_zero_rows<BN>(p.dk + u.k_at(p.dks), p.dks.n, u.tile, u.Sk, p.d);
@@ -117,7 +117,7 @@ template <int D, int G>
 __global__ __launch_bounds__(256) void fwd_packed_merge_kernel(const FwdParams p, const PackedArgs a) {
     constexpr int BM = 128, BN = 64;
     PackedUnit u;
-    if (packed_unit<BM, false, true, true>(a, (int)blockIdx.x, u) != kPackedTile || u.parts == 1) return;
+    if (packed_unit<BM, false, true>(a, (int)blockIdx.x, u) != kPackedTile || u.parts == 1) return;
     const int q0 = u.tile * BM, keys = max(a.causal ? min(u.Sk, q0 + BM + u.past) : u.Sk, 0);
     const int parts = packed_parts(u, (keys + BN - 1) / BN);
     if (parts == 1) return;
@@ -153,7 +153,7 @@ template <int D, int G>
 __global__ __launch_bounds__(256) void bwd_dq_packed_merge_kernel(const BwdParams p, const PackedArgs a) {
     constexpr int BM = 128, BN = 64;
     PackedUnit u;
-    if (packed_unit<BM, false, true, true>(a, (int)blockIdx.x, u) != kPackedTile || u.parts == 1) return;
+    if (packed_unit<BM, false, true>(a, (int)blockIdx.x, u) != kPackedTile || u.parts == 1) return;
     const int q0 = u.tile * BM, keys = max(a.causal ? min(u.Sk, q0 + BM + u.past) : u.Sk, 0);
     const int parts = packed_parts(u, (keys + BN - 1) / BN);
     if (parts == 1) return;
@@ -173,7 +173,7 @@ template <int D, int G>
 __global__ __launch_bounds__(256) void bwd_dkdv_packed_merge_kernel(const BwdParams p, const PackedArgs a) {
     constexpr int BM = BwdTile<D>::BM, BN = BwdTile<D>::BN;
     PackedUnit u;
-    if (packed_unit<BN, true, false, true>(a, (int)blockIdx.x, u) != kPackedTile || u.parts == 1) return;
+    if (packed_unit<BN, true, true>(a, (int)blockIdx.x, u) != kPackedTile || u.parts == 1) return;
     const int k0 = u.tile * BN, first = a.causal ? max(k0 - u.past, 0) / BM : 0, all = (u.Sq + BM - 1) / BM;
     if (first >= all) return;          // nothing attends to these keys: written by part 0
     const int parts = packed_parts(u, u.rep * (all - first));

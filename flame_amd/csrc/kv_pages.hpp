@@ -29,18 +29,10 @@ static __global__ __launch_bounds__(256) void kv_store_kernel(const KvStoreParam
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r0 = ((int)blockIdx.x * 4 + wave) * p.rows_per_wave;
     if (r0 >= p.rows) return;
-    // the last i with cu[i] <= r0
-    int lo = 0, count = p.n + 1;
-    while (count > 1) {
-        const int step = (count + 63) / 64, at = lo + lane * step;
-        const bool ok = lane == 0 || (lane * step < count && packed_bound(p.cu, at, p.rows) <= r0);
-        const int last = 63 - __clzll((long long)__ballot(ok));
-        lo += last * step;
-        count = min(step, count - last * step);
-    }
+    const int last = packed_find(p.n, r0, [&](int at) { return packed_bound(p.cu, at, p.rows); });      // sequence that begins at or before r0
     const int per_row = p.d / 8, n = p.Hkv * per_row, together = min(n, 64), sub = lane / together, r = r0 + sub;
     if (sub >= p.rows_per_wave || r >= p.rows) return;
-    int b = packed_uniform(lo);
+    int b = last;
     while (b < p.n && packed_bound(p.cu, b + 1, p.rows) <= r) ++b;
     if (b >= p.n) return;                              // behind the last sequence
     const int64_t pos = (int64_t)p.start[b] + (r - packed_bound(p.cu, b, p.rows));

@@ -77,14 +77,14 @@ __device__ __forceinline__ int packed_bound(const int32_t* cu, int i, int total)
 // the same value in every lane, which the compiler does not see (loads, divisions): into a scalar register
 __device__ __forceinline__ int packed_uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
-// The sequence that slot `r` belongs to (0 .. n): the last i with slot(i) <= r, 64 candidates at a time.  Every lane calls this.
-template <int TILE>
-__device__ __forceinline__ int packed_find(const int32_t* cu, int n, int total, int r) {
+// The last i of 0 .. n with slot(i) <= r, which is true of 0, 64 candidates at a time.  Every lane calls this.
+template <class F>
+__device__ __forceinline__ int packed_find(int n, int r, F&& slot) {
     const int lane = threadIdx.x & 63;
     int lo = 0, count = n + 1;
     while (count > 1) {
         const int step = (count + 63) / 64, at = lo + lane * step;
-        const bool ok = lane == 0 || (lane * step < count && packed_bound(cu, at, total) / TILE + at <= r);
+        const bool ok = lane == 0 || (lane * step < count && slot(at) <= r);
         const int last = 63 - __clzll((long long)__ballot(ok));
         lo += last * step;
         count = min(step, count - last * step);
@@ -117,9 +117,9 @@ __device__ __forceinline__ int wave_scan(int x) {
 }
 
 // The unit of workgroup `block`: a tile of TILE queries (KEYS: keys, of a key head) of one sequence, and a part of its walk.
-// LAST_FIRST: the tiles of a sequence come from the last to the first, which under the causal flag is from the longest walk to the
-// shortest.  MERGE: `block` counts tiles, not parts, and the unit is the first part of the tile; u.parts the most it can have.
-template <int TILE, bool KEYS, bool LAST_FIRST, bool MERGE = false>
+// The tiles of a sequence come from the longest walk under the causal flag to the shortest: of queries from the last to the first.
+// MERGE: `block` counts tiles, not parts, and the unit is the first part of the tile; u.parts the most it can have.
+template <int TILE, bool KEYS, bool MERGE = false>
 __device__ __forceinline__ PackedWork packed_unit(const PackedArgs& a, int block, PackedUnit& u) {
     constexpr int STEP = 64;       // rows of a step of the walk
     const int32_t* cu = KEYS ? a.cu_k : a.cu_q;
@@ -215,7 +215,7 @@ __device__ __forceinline__ PackedWork packed_unit(const PackedArgs& a, int block
         u.part = MERGE ? 0 : at - t * u.parts;
         u.unit = (u.unit + t * u.parts + u.part) * heads + head;
     } else {
-        const int i = packed_find<TILE>(cu, a.n, total, slot);
+        const int i = packed_find(a.n, slot, [&](int at) { return packed_bound(cu, at, total) / TILE + at; });
         const int first = packed_uniform(packed_bound(cu, i, total));
         t = slot - (first / TILE + i);
         if (i == a.n) {
@@ -232,7 +232,7 @@ __device__ __forceinline__ PackedWork packed_unit(const PackedArgs& a, int block
         if (t >= n_tiles) return kPackedIdle;
     }
     u.past = u.Sk - u.Sq;
-    u.tile = LAST_FIRST ? n_tiles - 1 - t : t;
+    u.tile = KEYS ? t : n_tiles - 1 - t;
     return kPackedTile;
 }
 
