@@ -5,6 +5,7 @@
 #include <cmath>
 
 #include "attn_packed.hpp"
+#include "launch_lds.hpp"
 #include "../../include/flame_attn.h"
 
 using namespace fattn;
@@ -30,20 +31,9 @@ bool overlaps(const int64_t* st, int rows, int heads, int D) {
     return n >= h ? n < h * (heads - 1) + D : h < n * (rows - 1) + D;
 }
 
-int set_lds(const void* kern, int bytes, std::atomic<uint64_t>& done) {      // a kernel's dynamic LDS size, once per kernel and device
-    int dev = 0;
-    if (hipGetDevice(&dev) != hipSuccess) return (int)hipErrorInvalidDevice;
-    const uint64_t bit = uint64_t(1) << (dev & 63);
-    if (done.load(std::memory_order_relaxed) & bit) return FLAME_ATTN_OK;
-    const hipError_t e = hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e != hipSuccess) return (int)e;
-    done.fetch_or(bit, std::memory_order_relaxed);
-    return FLAME_ATTN_OK;
-}
-
 template <class P>
 int launch(void (*kern)(P, PackedArgs), int lds, std::atomic<uint64_t>& done, int64_t units, int heads, const P& p, const PackedArgs& a, hipStream_t s, int threads = 256) {
-    if (const int rc = set_lds(reinterpret_cast<const void*>(kern), lds, done)) return rc;
+    if (const int rc = set_lds_of_device(reinterpret_cast<const void*>(kern), lds, done)) return rc;
     hipLaunchKernelGGL(kern, dim3((unsigned)(units * heads)), dim3(threads), (size_t)lds, s, p, a);
     return (int)hipGetLastError();
 }

@@ -8,6 +8,7 @@
 
 #include "attn_paged.hpp"
 #include "kv_pages.hpp"
+#include "launch_lds.hpp"
 #include "../../include/flame_attn.h"
 
 using namespace fattn;
@@ -46,17 +47,6 @@ int page_shift(int page) {
     return -1;
 }
 bool head_dim_ok(int D) { return D % 8 == 0 && D <= 128; }
-
-int set_lds(const void* kern, int bytes, std::atomic<uint64_t>& done) {      // a kernel's dynamic LDS size, once per kernel and device
-    int dev = 0;
-    if (hipGetDevice(&dev) != hipSuccess) return (int)hipErrorInvalidDevice;
-    const uint64_t bit = uint64_t(1) << (dev & 63);
-    if (done.load(std::memory_order_relaxed) & bit) return FLAME_ATTN_OK;
-    const hipError_t e = hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e != hipSuccess) return (int)e;
-    done.fetch_or(bit, std::memory_order_relaxed);
-    return FLAME_ATTN_OK;
-}
 
 // Most units that PagedCut makes of `tiles` tiles that `groups` walks (sequences, heads, row tiles) have together at most.
 int64_t most_units(int64_t tiles, int64_t groups) {
@@ -111,12 +101,12 @@ int launch_paged(const PagedParams& p, const PagedSizes& z, hipStream_t s) {
         const bool wide = grid <= 256;
         const auto kern = wide ? paged_direct_kernel<D, 8> : paged_direct_kernel<D, 4>;
         const int lds = PagedTile<D>::lds_bytes(wide ? 8 : 4);
-        if (const int rc = set_lds(reinterpret_cast<const void*>(kern), lds, wide ? done8 : done4)) return rc;
+        if (const int rc = set_lds_of_device(reinterpret_cast<const void*>(kern), lds, wide ? done8 : done4)) return rc;
         hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(wide ? 512 : 256), lds, s, p);
         return (int)hipGetLastError();
     }
     constexpr int lds = PagedTile<D>::lds_bytes(4);
-    if (const int rc = set_lds(reinterpret_cast<const void*>(paged_fwd_kernel<D>), lds, done)) return rc;
+    if (const int rc = set_lds_of_device(reinterpret_cast<const void*>(paged_fwd_kernel<D>), lds, done)) return rc;
     const int64_t room = D <= 64 ? 768 : 512;          // workgroups that the card holds (D = 64, 64 sequences of 4000: 512 of them 105.4 us, 768 102.8)
     hipLaunchKernelGGL(paged_fwd_kernel<D>, dim3((unsigned)std::min(room, z.prefix_units + z.own_units)), dim3(256), lds, s, p);
     if (const hipError_t e = hipGetLastError()) return (int)e;
