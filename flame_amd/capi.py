@@ -165,8 +165,8 @@ def packed_fwd_workspace_bytes(n_seqs, T_q, T_kv, H, D) -> int:
 def attn_packed_fwd(q, k, v, cu_q, cu_k, scale, causal=True, want_lse=True, out=None, lse_out=None, workspace=None):
     """O, LSE = flame_attn_packed_fwd_bf16(...): sequences of different lengths one behind the other.
 
-    q [T_q, H, D], k/v [T_kv, H_kv, D] bf16, D stride 1; cu_q, cu_k: int32 [sequences + 1] on the device, the bounds of
-    the sequences' rows.  causal: query i attends to key j <= i + (keys - queries) of its sequence.  Returns o [T_q, H, D]
+    q [T_q, H, D], k/v [T_kv, H_kv, D] bf16, D stride 1; cu_q, cu_k: int32 [sequences + 1] on the device, rising from 0, the
+    bounds of the sequences' rows.  causal: query i attends to key j <= i + (keys - queries) of its sequence.  Returns o [T_q, H, D]
     and lse fp32 [H, T_q] (None without want_lse); rows behind the last sequence are 0 and -inf.  `workspace`: uint8 device
     tensor, used where it holds packed_fwd_workspace_bytes(...) (allocated here when omitted)."""
     return host().attn_packed_fwd(q, k, v, cu_q, cu_k, scale, causal, want_lse, out, lse_out, workspace)
@@ -179,7 +179,7 @@ def packed_bwd_workspace_bytes(n_seqs, T_q, T_kv, H, H_kv, D) -> int:
 
 
 def attn_packed_bwd(q, k, v, o, do, lse, cu_q, cu_k, scale, causal=True, workspace=None, grads=None):
-    """dQ, dK, dV = flame_attn_packed_bwd_bf16(...).  `workspace`: uint8 device tensor, best of
+    """dQ, dK, dV = flame_attn_packed_bwd_bf16(...).  `grads`: buffers for all three.  `workspace`: uint8 device tensor, best of
     packed_bwd_workspace_bytes(...) bytes (allocated here when omitted), at least two fp32 values per query row and head."""
     dq, dk, dv = grads if grads is not None else (None, None, None)
     return host().attn_packed_bwd(q, k, v, o, do, lse, cu_q, cu_k, scale, causal, workspace, dq, dk, dv)
@@ -204,7 +204,7 @@ def attn_paged_fwd(q, k_cache, v_cache, page_table, kv_len, scale, prefix_table=
 
 
 def kv_store(k, v, k_cache, v_cache, page_table, cu, start):
-    """flame_kv_store_bf16(...): rows k, v [rows, H_kv, D] of the sequences that cu (int32 [sequences + 1]) bounds to the
+    """flame_kv_store_bf16(...): rows k, v [rows, H_kv, D] of the sequences that cu (int32 [sequences + 1], rising from 0) bounds to the
     places start[b], start[b] + 1, ... (int32 [sequences]) of their pages.  Autograd records nothing: inputs that require a gradient
     are refused while it is enabled, and a graph that saved a view of the caches raises in its backward."""
     host().kv_store(k, v, k_cache, v_cache, page_table, cu, start)

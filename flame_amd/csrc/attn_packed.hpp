@@ -8,8 +8,8 @@
 // partial gradients per head.
 //
 // What bounds them is what bounds the dense kernels, at their rates: the matrix instructions and the exponentials between them.  Forward,
-// eight prompts of 1 to 4096, 32 heads on 8, D = 128: 292 us, 1.0 PFLOP/s (as much as the dense causal one on 4096); training on six documents of
-// 333 to 4608, the same heads: forward 370, dQ 520, dK/dV 680 us.  Small batches: the longest walk, one step of 64 keys after the other at 0.6 to 1 us;
+// eight prompts of 1 to 4096, 32 heads on 8, D = 128: 292 to 319 us by the card, 0.91 to 1.0 PFLOP/s (as much as the dense causal one on 4096); training on six
+// documents of 333 to 4608, the same heads: forward 360 to 370, dQ 500 to 520, dK/dV 660 to 680 us.  Small batches: the longest walk, one step of 64 keys after the other at 0.6 to 1 us;
 // a few heads of 1000 to 2000 rows: forward 13 to 18 us, backward 48 to 58.
 // Roundings to 16 bits, which the matrix instructions' operands take: P before it meets V and dO, dS before it meets K and Q, O as it is saved,
 // from which delta is formed; all sums are fp32.  dQ and dK are therefore off by 0.0025 of their root mean square against 0.0017 of one

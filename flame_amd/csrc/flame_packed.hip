@@ -59,7 +59,9 @@ constexpr PackedCut kCutFwd{9, 16, 16, 1.6f}, kCutDq{9, 8, 12, 1.6f};
 PackedCut cut_dkdv(int D) { return PackedCut{8, 8, 12, D <= 64 ? 0.65f : 1.6f}; }
 // Whether a problem gets room for walks in parts, which the device then cuts or not by the lengths (PackedCut): not where whole walks fill the
 // 256 compute units one and a half times, nor where the mean walk is short, nor where no lengths of these sums would be cut (the fewest
-// steps: a causal self-attention's).
+// steps: a causal self-attention's), nor of more than 64 sequences.  The mean stands for the longest walk, which the host does not know: one
+// long sequence among many short ones stays whole (us, D = 128, causal; 4 heads of 8192: forward 88, with 8 of 50 rows 117; on 2 key heads, backward 265,
+// with 8 of 50 267, with 31 of 50 439; one head of 8000, backward 112, with 15 of 10 285).
 // (Whole -> in parts, us, D = 128.  Forward: 4 heads of 8192 117 -> 88, 32 of 128 rows on 8192 keys 115 -> 32, 8 of 100 rows on 30000 400 -> 37.  Backward: 4 of
 // 1024 53 -> 48, 8 on 2 of 612 67 -> 52, of 2000 207 -> 82, 4 on 2 of 8192 439 -> 263.  Left whole: 24 of 1200 23 and 64, in parts 35 and 94.)
 bool parts_pay(const PackedCut& cut, int64_t slots, int heads, int n_seqs, int walked_rows) {
@@ -83,7 +85,9 @@ Parts parts_of(const PackedCut& cut, int tile_rows, int walked_rows, int n_seqs,
     return z;
 }
 // Workgroups of 32 queries whose wavefronts share the keys, in place of 128 queries per workgroup: where two fit a compute unit, or four at D = 64, all
-// at once, the second half of them for walks that are not the shortest; and where no walk is so long that parts of it (above) are better.
+// at once, the second half of them for walks that are not the shortest; and where walks are not so long that parts of them (above) are better, for
+// which all keys stand up to three sequences and four times the mean beyond: one long walk among many short ones passes, too (one head of 8000 43 us, with
+// 15 of 10 rows 61).
 // (128 queries -> 32, us.  D = 128: 24 heads of 77 7.7 -> 6.5, 4 of 1024 19.7 -> 12.8, 4 of 2000 25.6 -> 18.5, 8 of 1200 24.5 -> 17.6, 16 of four pieces of 100 on
 // 900 keys 19.5 -> 14.9; beyond: 24 of 1024 21.5 -> 26.1, 32 of 700 15.7 -> 21.0, 8 of 4000 53.5 -> 60; short: 24 of eight times 32 6.9 -> 7.4.  D = 64: 8 of 612 11.3 -> 7.8, 12 of
 // 2000 24.3 -> 18.4, 16 of 2000 26.9 -> 20.2; beyond: 24 of 2000 25.6 -> 29.7.  8 heads of 100 on 4000 keys: 23.6 -> 25.5, D = 64 18.6 -> 17.9.)

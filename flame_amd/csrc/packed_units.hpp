@@ -7,7 +7,8 @@
 //   is left at the end is short: under the causal flag tile by tile over all sequences (training on six documents of 333 to 4608, us:
 //   sequence by sequence 1543, tile by tile 1515), else sequence by sequence.  On grids that leave compute units idle the walks are cut
 //   into parts (PackedCut) whose partial sums a second launch joins.
-//   More: in their own order.  Every sequence gets the slots [slot(i), slot(i + 1)) with slot(i) = cu[i] / tile + i, at least as many as
+//   More: in their own order, whole (100 of 16 to 512 rows, 32 heads on 8, D = 128, forward and backward 231 and 736 us; with one of 4096 behind them 357
+//   and 1208, before them 372 and 1164).  Every sequence gets the slots [slot(i), slot(i + 1)) with slot(i) = cu[i] / tile + i, at least as many as
 //   it has tiles and at most one more, so that a search finds it without a sum over the lengths.
 // The rows behind the last sequence are the last tiles of that numbering: their workgroups write zeros.
 // Bounds that fall or lead out of the tensor are cut to it: the result is then of no use, but nothing outside is touched.

@@ -42,7 +42,7 @@ def sdpa_packed(q, k, v, cu_seqlens, cu_seqlens_k=None, is_causal=None, scale=No
     H a multiple of H_kv (head h reads key head h // (H // H_kv)).  Differentiable, once: a backward with create_graph=True is
     refused.
 
-    cu_seqlens (and cu_seqlens_k where the keys have other lengths): int32 [sequences + 1] on the device, the rows of
+    cu_seqlens (and cu_seqlens_k where the keys have other lengths): int32 [sequences + 1] on the device, rising from 0, the rows of
     sequence i being cu_seqlens[i] .. cu_seqlens[i + 1] - 1; a recorded graph holds them, so they may not be refilled before
     its backward.  is_causal=True: query i of a sequence attends to keys j <= i + (keys - queries), the last query to
     all of them.  Queries without a key and rows behind the last sequence come out as zeros, with zero gradients.
@@ -58,6 +58,7 @@ def sdpa_paged(q, k_cache, v_cache, page_table, kv_len, prefix_table=None, prefi
 
     page_table: int32 [B, pages], the pages of a sequence's own keys in their order; kv_len: int32 [B], how many own keys,
     the N new ones among them.  prefix_table (int32 [pages]) and prefix_len (int32 [1]): keys that all sequences have in
-    front of their own, read once for the batch.  Token i attends to the prefix and to own keys j <= kv_len - N + i.
+    front of their own, read once for the batch.  Token i attends to the prefix and to own keys j <= kv_len - N + i (an infinity or
+    NaN in a later token's V reaches it all the same: its weight of 0 multiplies it).
     q of another dtype is promoted to bf16 and the result is cast back."""
     return capi.host().sdpa_paged(q, k_cache, v_cache, page_table, kv_len, prefix_table, prefix_len, scale)

@@ -16,7 +16,8 @@
 The book is plain integers on the host: a page that several sequences share is counted and never written; what goes to the
 device is one small upload per `extend`.  Keys and values move in capi.kv_store and capi.kv_copy_pages, attention is
 functional.sdpa_paged; nothing here computes on the GPU by itself.  Not thread-safe; calls are ordered by the stream that is
-current when they are made.
+current when they are made.  A batch is of use until one of its sequences is extended, cut or freed or the cache is compacted: after
+that its places may belong to others.  Inference only: `store` and `attend` are for torch.no_grad() or tensors that require no gradient.
 """
 from __future__ import annotations
 

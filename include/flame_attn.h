@@ -286,7 +286,8 @@ int flame_attn_packed_bwd_bf16(const void* Q, const void* K, const void* V, cons
  * sequences share, then their own: softmax over both.  The shared prefix has prefix_len[0] tokens (one int32 on the device) on the pages
  * prefix_table[0 .. prefix_pages - 1] and is read once for the batch; null, null and 0 pages: none.  kv_len [B]: the keys of a sequence's own pages,
  * its N new tokens among them (stored before the call).  Token i of the N attends to the whole prefix and to own keys
- * j <= kv_len[b] - N + i.  A row without a key has O = 0 and LSE = -inf.  H a multiple of H_kv: head h reads key head
+ * j <= kv_len[b] - N + i; the others' V enters its tile's products with the weight 0, so that infinities and NaN in the V of later tokens reach it, as in
+ * the other causal calls.  A row without a key has O = 0 and LSE = -inf.  H a multiple of H_kv: head h reads key head
  * h / (H / H_kv).  D any multiple of 8 up to 128.  LSE: fp32, contiguous [B*H, N], or null.
  * `workspace`: device memory, 16-byte aligned, of at least flame_attn_paged_workspace_bytes(...) bytes (0: none is needed, or the
  * call would be refused), used only during the call; nothing in it has to start at any value.  Calls that overlap (other streams,

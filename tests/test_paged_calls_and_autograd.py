@@ -128,3 +128,21 @@ def test_gradients_of_paged_attention():
         leaves[which] = leaves[which].clone().requires_grad_(True)
         with pytest.raises(RuntimeError, match="no backward"):
             functional.sdpa_paged(*leaves)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("mode", [torch.enable_grad, torch.no_grad, torch.inference_mode])
+def test_layers_of_a_cache_share_its_version(mode):
+    from flame_amd.paged_cache import PagedCache
+    c = PagedCache(2, 8, PAGE, HKV, D)
+    a = c.new()
+    batch = c.extend([a], [5])
+    k, v = torch.randn(2, 5, HKV, D, device="cuda").to(torch.bfloat16)
+    before = c.k._version, c.v._version
+    with mode():
+        c.store(1, k, v, batch)
+    assert c.k._version > before[0] and c.v._version > before[1]
+    fork, before = c.fork(a), c.k._version
+    with mode():
+        c.extend([a, fork], [1, 1])                 # copies the shared page
+    assert c.k._version > before and torch.equal(c.k[1, c.pages(fork)[0], :, :5], c.k[1, c.pages(a)[0], :, :5])
