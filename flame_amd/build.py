@@ -31,7 +31,7 @@ def hipcc_version() -> str:
     return f"{hip} clang-{clang}"
 
 
-SOURCES = ("flame_attn.hip", "flame_packed.hip", "flame_paged.hip")      # of the attention library
+SOURCES = ("flame_attn.hip", "flame_packed.hip", "flame_paged.hip", "flame_paged8.hip", "flame_rotary.hip")      # of the attention library
 
 STATIC_LIB_PATH = os.path.join(LIB_DIR, "libflame_attn_hip.a")
 

@@ -193,28 +193,51 @@ def paged_workspace_bytes(B, H, H_kv, N, D, page, table_pages, prefix_pages=0) -
 
 
 def attn_paged_fwd(q, k_cache, v_cache, page_table, kv_len, scale, prefix_table=None, prefix_len=None, want_lse=False, out=None,
-                   workspace=None):
-    """O, LSE = flame_attn_paged_fwd_bf16(...): the last N tokens of every sequence against a paged cache.
+                   workspace=None, k_scale=None, v_scale=None):
+    """O, LSE = flame_attn_paged_fwd_bf16(...), flame_attn_paged_fwd_q8(...) where the caches have scales: the last N tokens of every
+    sequence against a paged cache.
 
-    q [B, H, N, D]; caches bf16 [pages, H_kv, page, D]; page_table int32 [B, pages of a sequence], kv_len int32 [B]: a
+    q [B, H, N, D]; caches bf16 [pages, H_kv, page, D], or int8 or float8_e4m3fn with k_scale, v_scale fp32 [pages, H_kv, page / block];
+    page_table int32 [B, pages of a sequence], kv_len int32 [B]: a
     sequence's own keys, the N new ones among them; prefix_table int32 [pages] and prefix_len int32 [1]: keys that all
     sequences share in front of their own.  `workspace`: uint8 device tensor of at least paged_workspace_bytes(...) bytes
     (allocated here when omitted; 0: none is needed).  lse fp32 [B * H, N] or None.  Inference only."""
-    return host().attn_paged_fwd(q, k_cache, v_cache, page_table, kv_len, scale, prefix_table, prefix_len, want_lse, out, workspace)
+    return host().attn_paged_fwd(q, k_cache, v_cache, page_table, kv_len, scale, prefix_table, prefix_len, want_lse, out, workspace, k_scale, v_scale)
 
 
-def kv_store(k, v, k_cache, v_cache, page_table, cu, start):
-    """flame_kv_store_bf16(...): rows k, v [rows, H_kv, D] of the sequences that cu (int32 [sequences + 1], rising from 0) bounds to the
-    places start[b], start[b] + 1, ... (int32 [sequences]) of their pages.  Autograd records nothing: inputs that require a gradient
+def kv_store(k, v, k_cache, v_cache, page_table, cu, start, k_scale=None, v_scale=None):
+    """flame_kv_store_bf16(...), flame_kv_store_q8(...) where the caches have scales: rows k, v [rows, H_kv, D] of the sequences that cu
+    (int32 [sequences + 1], rising from 0) bounds to the places start[b], start[b] + 1, ... (int32 [sequences]) of their pages.
+
+    Caches in 8 bits: int8 or float8_e4m3fn, D a multiple of 16 up to 128, k_scale and v_scale fp32 [pages, H_kv, page / block], `block` tokens
+    (a power of two up to 128) sharing one.  A block begun by this call gets the scale its largest magnitude needs; one that
+    holds older tokens keeps its scale or doubles it until the new rows fit, and the older codes follow.  Infinities and NaN make
+    a block's scale NaN.  Autograd records nothing: inputs that require a gradient
     are refused while it is enabled, and a graph that saved a view of the caches raises in its backward."""
-    host().kv_store(k, v, k_cache, v_cache, page_table, cu, start)
+    host().kv_store(k, v, k_cache, v_cache, page_table, cu, start, k_scale, v_scale)
 
 
-def kv_copy_pages(k_cache, v_cache, src, dst):
-    """flame_kv_copy_pages_bf16(...): page src[i] to page dst[i] (sequences of ints) in both caches, [pages, H_kv, page, D]
+def kv_load(k_cache, v_cache, page_table, cu, start, rows, k_scale=None, v_scale=None, out=None):
+    """k, v = flame_kv_load(...), the way back of kv_store: bf16 [rows, H_kv, D], row cu[b] + i what place start[b] + i of sequence b
+    holds.  Rows behind the last sequence are zeros, rows without a place in the cache NaN.  `out`: buffers for both."""
+    k, v = out if out is not None else (None, None)
+    return host().kv_load(k_cache, v_cache, page_table, cu, start, rows, k_scale, v_scale, k, v)
+
+
+def kv_copy_pages(k_cache, v_cache, src, dst, k_scale=None, v_scale=None):
+    """flame_kv_copy_pages_bf16(...), flame_kv_copy_pages_q8(...) where the caches have scales: page src[i] to page dst[i] (sequences of
+    ints) in both caches, [pages, H_kv, page, D]
     or [layers, pages, H_kv, page, D], in all layers.  A page that is written twice, or read and written, is refused.
     Autograd is told what kv_store tells it."""
-    host().kv_copy_pages(k_cache, v_cache, src, dst)
+    host().kv_copy_pages(k_cache, v_cache, src, dst, k_scale, v_scale)
+
+
+# ---------------------------------------------------------------- rotary positions
+def rotary(q, k, turns, interleaved=False, size=1.0, positions=None, cu_seqlens=None, start=None, inverse=False):
+    """flame_rotary(...): q (and k, or None) [rows, heads, D] or [B, heads, S, D], bf16, fp16 or fp32, with pairs of the first
+    2 * len(turns) elements of every head turned.  turns: int64 [pairs] on the device, 2^64 / (2 pi) times the radians per
+    position (flame_amd.rotary makes them).  Differentiable; functional.rotary has the rest."""
+    return host().rotary(q, k, turns, interleaved, size, positions, cu_seqlens, start, inverse)
 
 
 KERNEL_KINDS = ("fwd", "unused1", "bwd_dkdv", "bwd_dq", "sage_kmean", "sage_quant", "sage_fwd", "input_prep",

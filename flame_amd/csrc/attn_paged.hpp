@@ -99,6 +99,10 @@ struct PagedTile {
     static constexpr int RPD = 1024 / (RS * 2);                    // rows per copy
 };
 
+// dynamic LDS of a workgroup of nw wavefronts
+template <int D>
+constexpr int paged_lds_bytes(const PagedParams*, int nw) { return PagedTile<D>::lds_bytes(nw); }
+
 // This wavefront's reads of LDS have returned and none moves to behind this: a copy may overwrite what they read.
 __device__ __forceinline__ void lds_reads_done() {
     asm volatile("" ::: "memory");
@@ -370,12 +374,66 @@ struct PagedRows {
     }
 };
 
+// The end of a unit whose wavefronts have walked keys of their own: their states become one, which is the result (direct) or goes to the
+// merge.  `lds`: WAVE_FLOATS floats per wavefront, at least 32 D, into which no copy is under way; `bad`: the rows are NaN.
+template <int D, int NW, int WAVE_FLOATS>
+__device__ __forceinline__ void paged_unit_join(const PagedParams& p, const PagedUnit& u, PagedRows<D>& w, float* lds, int tid, bool bad, bool direct,
+                                                float* out_o, f32x2* out_ml) {
+    constexpr int DB = D / 32;
+    const int lane = tid & 63, wave = packed_uniform(tid >> 6), n = lane & 31, h = lane >> 5;
+    w.l_run += xhalf(w.l_run);
+    if (__any(bad)) w.l_run = __builtin_nanf("");    // a page outside the cache, or more keys than pages: NaN
+    __shared__ f32x2 state[NW][32];
+    if (h == 0) state[wave][n] = f32x2{w.m_run, w.l_run};
+    __syncthreads();                                   // (no copy is under way: every wavefront has waited for its last one)
+    float M = -INFINITY, L = 0.f;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) M = fmaxf(M, state[i][n][0]);
+    const float M_to = M == -INFINITY ? 0.f : M;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) L += state[i][n][1] * exp2_fast((state[i][n][0] - M_to) * w.c_log2);
+    const float f = exp2_fast((w.m_run - M_to) * w.c_log2);
+    float* const sums = lds + wave * WAVE_FLOATS;       // [32][D], granules of four swizzled by the row
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const f32x16& a = w.oacc[db];
+            *reinterpret_cast<f32x4*>(sums + n * D + (((8 * db + 2 * g + h) ^ (n & 7)) << 2)) = f32x4{a[4 * g] * f, a[4 * g + 1] * f, a[4 * g + 2] * f, a[4 * g + 3] * f};
+        }
+    __shared__ f32x2 joined[32];
+    if (wave == 0 && h == 0) joined[n] = f32x2{M * w.c_log2, L};
+    __syncthreads();
+    for (int e = tid; e < u.rows * (D / 4); e += 64 * NW) {
+        const int r = e / (D / 4), g = e % (D / 4);
+        if (4 * g >= p.d) continue;
+        f32x4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < NW; ++i) a += *reinterpret_cast<const f32x4*>(lds + i * WAVE_FLOATS + r * D + ((g ^ (r & 7)) << 2));
+        if (direct) {
+            const float l = joined[r][1], inv = l == 0.f ? 0.f : 1.0f / l;
+            const PagedRow at = paged_row(p, u, r);
+            *reinterpret_cast<u32x2*>(p.o + at.b * p.os.b + at.h * p.os.h + at.i * p.os.n + 4 * g) = u32x2{pack_bf16(a[0] * inv, a[1] * inv), pack_bf16(a[2] * inv, a[3] * inv)};
+        } else {
+            *reinterpret_cast<f32x4*>(out_o + (int64_t)r * p.d + 4 * g) = a;
+        }
+    }
+    if (tid < u.rows) {
+        const f32x2 ml = joined[tid];
+        if (!direct) out_ml[tid] = ml;
+        else if (p.lse) {
+            const PagedRow at = paged_row(p, u, tid);
+            p.lse[((int64_t)at.b * p.H + at.h) * p.N + at.i] = ml[1] == 0.f ? -INFINITY : (ml[0] + log2_fast(ml[1])) * kLn2;
+        }
+    }
+}
+
 // A unit whose wavefronts walk keys of their own: wavefront w the tiles from tile0 + w * `run` on, STRIDED: tile0 + w, tile0 + w + NW, ...
 template <int D, int NW, bool STRIDED>
 __device__ __forceinline__ void paged_unit_body(const PagedParams& p, const PagedUnit& u, uint16_t* lds, bool bad, bool direct, float* out_o, f32x2* out_ml) {
     using T = PagedTile<D>;
     constexpr int DC = D / 16, DB = D / 32, NDMA = T::NDMA;
-    const int tid = paged_thread(), lane = tid & 63, wave = packed_uniform(tid >> 6), n = lane & 31, h = lane >> 5;
+    const int tid = paged_thread(), lane = tid & 63, wave = packed_uniform(tid >> 6), n = lane & 31;
     uint16_t* const mine = lds + wave * T::WAVE_ELEMS;
     const uint32_t lds_k = lds_addr(mine), lds_v = lds_k + 2u * T::TILE_ELEMS;
     const uint16_t* const kbase = p.k + u.kv_head * p.ks.h;
@@ -425,52 +483,7 @@ __device__ __forceinline__ void paged_unit_body(const PagedParams& p, const Page
         w.add(vf, pf);
     }
 
-    // ---- the wavefronts' states become one
-    w.l_run += xhalf(w.l_run);
-    if (__any(bad | (pages.bad && t_lo < t_hi))) w.l_run = __builtin_nanf("");    // a page outside the cache, or more keys than pages: NaN
-    __shared__ f32x2 state[NW][32];
-    if (h == 0) state[wave][n] = f32x2{w.m_run, w.l_run};
-    __syncthreads();                                   // (no copy is under way: every wavefront has waited for its last one)
-    float M = -INFINITY, L = 0.f;
-#pragma unroll
-    for (int i = 0; i < NW; ++i) M = fmaxf(M, state[i][n][0]);
-    const float M_to = M == -INFINITY ? 0.f : M;
-#pragma unroll
-    for (int i = 0; i < NW; ++i) L += state[i][n][1] * exp2_fast((state[i][n][0] - M_to) * w.c_log2);
-    const float f = exp2_fast((w.m_run - M_to) * w.c_log2);
-    float* const sums = reinterpret_cast<float*>(mine);       // [32][D], granules of four swizzled by the row
-#pragma unroll
-    for (int db = 0; db < DB; ++db)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const f32x16& a = w.oacc[db];
-            *reinterpret_cast<f32x4*>(sums + n * D + (((8 * db + 2 * g + h) ^ (n & 7)) << 2)) = f32x4{a[4 * g] * f, a[4 * g + 1] * f, a[4 * g + 2] * f, a[4 * g + 3] * f};
-        }
-    __shared__ f32x2 joined[32];
-    if (wave == 0 && h == 0) joined[n] = f32x2{M * w.c_log2, L};
-    __syncthreads();
-    for (int e = tid; e < u.rows * (D / 4); e += 64 * NW) {
-        const int r = e / (D / 4), g = e % (D / 4);
-        if (4 * g >= p.d) continue;
-        f32x4 a = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < NW; ++i) a += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + i * T::WAVE_ELEMS) + r * D + ((g ^ (r & 7)) << 2));
-        if (direct) {
-            const float l = joined[r][1], inv = l == 0.f ? 0.f : 1.0f / l;
-            const PagedRow at = paged_row(p, u, r);
-            *reinterpret_cast<u32x2*>(p.o + at.b * p.os.b + at.h * p.os.h + at.i * p.os.n + 4 * g) = u32x2{pack_bf16(a[0] * inv, a[1] * inv), pack_bf16(a[2] * inv, a[3] * inv)};
-        } else {
-            *reinterpret_cast<f32x4*>(out_o + (int64_t)r * p.d + 4 * g) = a;
-        }
-    }
-    if (tid < u.rows) {
-        const f32x2 ml = joined[tid];
-        if (!direct) out_ml[tid] = ml;
-        else if (p.lse) {
-            const PagedRow at = paged_row(p, u, tid);
-            p.lse[((int64_t)at.b * p.H + at.h) * p.N + at.i] = ml[1] == 0.f ? -INFINITY : (ml[0] + log2_fast(ml[1])) * kLn2;
-        }
-    }
+    paged_unit_join<D, NW, T::WAVE_ELEMS / 2>(p, u, w, reinterpret_cast<float*>(lds), tid, bad | (pages.bad && t_lo < t_hi), direct, out_o, out_ml);
 }
 
 // A unit of the prefix with 128 rows: the wavefronts have 32 each and share the tiles, a quarter of each copied by every wavefront.
@@ -554,8 +567,8 @@ __device__ __forceinline__ void paged_shared_body(const PagedParams& p, const Pa
 // The units are dealt to the workgroups in turn, as the host does not know how many there are and a workgroup without one would cost as
 // much as the summing of the batch: those of the prefix first, then the own ones, of which the first go to the workgroups that have
 // none of the prefix, a few each while the others are at theirs (24 sequences on a prefix of 8192 34.5 -> 29.8 us, D = 64 35.5 -> 27.0).
-template <int D>
-__global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void paged_fwd_kernel(const PagedParams p) {
+template <int D, class P>
+__global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void paged_fwd_kernel(const P p) {
     extern __shared__ __attribute__((aligned(1024))) uint16_t lds[];
     __shared__ int sums[4], found[4];
     const int G = p.H / p.Hkv, rows = p.N * G, rt = PagedCut::row_tiles(rows), slot_rows = min(32, rows);
@@ -624,8 +637,8 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void paged_fwd_kernel(const P
 }
 
 // Short tables, no prefix: blockIdx.x = (sequence, key head, 32 rows).  The first pages are requested before the number of keys is known.
-template <int D, int NW>
-__global__ __launch_bounds__(64 * NW, NW == 4 ? (D <= 64 ? 3 : 2) : 2) void paged_direct_kernel(const PagedParams p) {
+template <int D, int NW, class P>
+__global__ __launch_bounds__(64 * NW, NW == 4 ? (D <= 64 ? 3 : 2) : 2) void paged_direct_kernel(const P p) {
     extern __shared__ __attribute__((aligned(1024))) uint16_t lds[];
     const int rows = p.N * (p.H / p.Hkv), rt = PagedCut::row_tiles(rows);
     const int pair = packed_uniform((int)blockIdx.x / rt), b = packed_uniform(pair / p.Hkv);
@@ -644,6 +657,8 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? (D <= 64 ? 3 : 2) : 2) void page
     u.tiles = paged_tiles(u.keys);
     paged_unit_body<D, NW, true>(p, u, lds, bad, true, nullptr, nullptr);
 }
+
+int launch_paged_merge(const PagedParams& p, hipStream_t s);        // compiled in flame_paged.hip
 
 // Joins the units of a row: SHARE wavefronts take a share of the units each (4: a workgroup per row, 1: a workgroup for four rows).  Bound by the
 // latency of plan, maxima and sums one behind the other, about 6 us with its launch.

@@ -65,12 +65,17 @@ struct KvCopyParams {
     int granules;                  // of 16 bytes in a page
     int chunks;                    // workgroups per page and tensor
     int contiguous;                // a page is one piece of memory in both tensors
+    // SCALES: fp32 [layers][pages][Hkv][blocks] of each
+    float* s[2];
+    int64_t s_layer[2], s_page[2], s_head[2], s_block[2];
+    int blocks;
 };
 
 constexpr int kKvCopyPerThread = 4;
 
 // blockIdx.x: chunk of a page, of K or V; y: layer; z: pair.  Bound by memory: 600 pages of 16 tokens, 8 heads, D = 128 in 24 layers 386 us,
 // 4.9 TB/s of what is read and written, as fast as a large copy.  Four granules per thread are requested before the first is stored.
+template <bool SCALES>
 static __global__ __launch_bounds__(256) void kv_copy_kernel(const KvCopyParams p, const KvCopyPairs pairs) {
     const int which = (int)blockIdx.x / p.chunks, chunk = (int)blockIdx.x - which * p.chunks;
     uint16_t* const layer = p.c[which] + (int)blockIdx.y * p.layer[which];
@@ -93,6 +98,14 @@ static __global__ __launch_bounds__(256) void kv_copy_kernel(const KvCopyParams 
 #pragma unroll
     for (int i = 0; i < kKvCopyPerThread; ++i)
         if (g0 + 256 * i < p.granules) *reinterpret_cast<u32x4*>(to + at[i]) = w[i];
+    if constexpr (SCALES) {
+        float* const of = p.s[which] + (int)blockIdx.y * p.s_layer[which];
+        for (int i = chunk * 256 + (int)threadIdx.x; i < p.Hkv * p.blocks; i += p.chunks * 256) {
+            const int h = i / p.blocks;
+            const int64_t at = h * p.s_head[which] + (i - h * p.blocks) * p.s_block[which];
+            of[pairs.dst[blockIdx.z] * p.s_page[which] + at] = of[pairs.src[blockIdx.z] * p.s_page[which] + at];
+        }
+    }
 }
 
 }  // namespace fattn

@@ -1,0 +1,213 @@
+// Rows to the pages of a cache in 8 bits and back (kv_codes.hpp).
+//
+// A block of T tokens of one head has a scale.  The largest magnitude a of the rows that a call brings to a block decides it:
+//   rows from the block's first token on:  s = a / Q rounded up to four significant bits, at least 2^-100 (Q: the largest code)
+//   rows behind older tokens:              s' = s 2^k with the least k >= 0 such that a <= Q s', and the older codes c become c 2^-k, rounded
+//   a not finite, or s none that a store has left:  NaN, which every answer that attends to the block then is
+// and a number x becomes x / s, rounded to the nearest code, the even one of two.
+// Growing by powers of two, a block's codes are off by less than one of its last steps however often it grew: 1/2 + 1/4 + ...; by the ratio that
+// a needs they would drift by half a step each time.  Four bits of s cost int8 a sixteenth of its resolution at most, on average a thirty-second, and give this: x has
+// eight significant bits, so x / s either is a border between two codes or is 2^-15 away from it, and fp32 arithmetic finds the same codes as exact arithmetic.
+#pragma once
+#include "kv_codes.hpp"
+#include "packed_units.hpp"
+
+namespace fattn {
+
+struct KvStore8Params {
+    const uint16_t* x[2];          // K and V: [rows][Hkv][d] through xs (n: row, h: head)
+    uint8_t* c[2];                 // [pages][Hkv][page][d] through cs (b: page, h: head, n: token; bytes)
+    float* s[2];                   // [pages][Hkv][page / T] through ss (b: page, h: head, n: block)
+    Strides xs[2], cs[2], ss[2];
+    const int32_t* table;
+    int64_t table_stride;
+    int table_pages;
+    const int32_t* cu;             // [n + 1]: rows of the sequences
+    const int32_t* start;          // [n]: place of a sequence's first row in its pages
+    int n, rows, Hkv, d, n_pages, page_shift, block_shift;
+    uint32_t units;                // slots * 2 * Hkv
+};
+
+// Slots for the blocks that sequences write to, at least as many as there can be: [slot(i), slot(i + 1)).  n rows touch at most n / T + 2 blocks of
+// T > 1 tokens.
+__host__ __device__ inline int64_t kv_store8_slot(int64_t first_row, int i, int block_shift) {
+    return (first_row >> block_shift) + (block_shift ? 2 * (int64_t)i : 0);
+}
+
+// LANES threads per unit, which is a block of one head of K or of V, with E granules of 8 numbers each.  Neighbouring units are neighbouring heads.
+// Bound by memory and, for few rows, by the chain of search, table, old scale and rows.
+template <int CODE, int LANES, int E>
+static __global__ __launch_bounds__(256) void kv_store8_kernel(const KvStore8Params p) {
+    constexpr float Q = kLargestCode<CODE>;
+    const uint32_t unit = (blockIdx.x * 256u + threadIdx.x) / LANES, unit0 = __builtin_amdgcn_readfirstlane(unit);
+    const int lane = threadIdx.x & (LANES - 1);
+    __shared__ uint32_t tops[4];
+    if (LANES <= 64 && unit0 >= p.units) return;       // (a workgroup of one unit: always below)
+    const uint32_t per_slot = 2u * (uint32_t)p.Hkv;
+    auto slot_of = [&](int i) { return (int)kv_store8_slot(packed_bound(p.cu, i, p.rows), i, p.block_shift); };
+    int b = packed_find(p.n, (int)(unit0 / per_slot), slot_of);
+    const uint32_t at = min(unit, p.units - 1u);
+    const int slot = (int)(at / per_slot), rest = (int)(at - (uint32_t)slot * per_slot), which = rest >= p.Hkv, head = rest - (which ? p.Hkv : 0);
+    while (b < p.n && slot_of(b + 1) <= slot) ++b;
+    // the block of this unit: tokens [lo, hi) of the sequence are new in it
+    int64_t lo = 0, hi = 0, begin = 0;
+    int page = -1, first_row = 0;
+    if (unit < p.units && b < p.n) {
+        const int row0 = packed_bound(p.cu, b, p.rows);
+        const int64_t start = p.start[b], end = start + max(packed_bound(p.cu, b + 1, p.rows) - row0, 0);
+        begin = ((start >> p.block_shift) + (slot - slot_of(b))) << p.block_shift;
+        lo = max(start, begin);
+        hi = min(end, begin + (1 << p.block_shift));
+        first_row = row0 + (int)(lo - start);
+        if (lo < hi && begin >= 0 && (begin >> p.page_shift) < p.table_pages) page = p.table[b * p.table_stride + (begin >> p.page_shift)];
+    }
+    const bool there = page >= 0 && page < p.n_pages;
+    if (LANES <= 64 && !there) return;                 // (a unit's lanes leave together)
+    const int per_row = p.d / 8, n = there ? (int)(hi - lo) * per_row : 0;
+    const uint16_t* const x = (which ? p.x[1] : p.x[0]) + head * (which ? p.xs[1].h : p.xs[0].h) + first_row * (which ? p.xs[1].n : p.xs[0].n);
+    const int64_t x_row = which ? p.xs[1].n : p.xs[0].n, c_row = which ? p.cs[1].n : p.cs[0].n;
+    const int token0 = (int)(begin & ((1 << p.page_shift) - 1)), old = (int)(lo - begin);
+    uint8_t* const c = (which ? p.c[1] : p.c[0]) + page * (which ? p.cs[1].b : p.cs[0].b) + head * (which ? p.cs[1].h : p.cs[0].h) + token0 * c_row;
+    float* const scale = (which ? p.s[1] : p.s[0]) + page * (which ? p.ss[1].b : p.ss[0].b) + head * (which ? p.ss[1].h : p.ss[0].h) +
+                         (token0 >> p.block_shift) * (which ? p.ss[1].n : p.ss[0].n);
+    const float s_old = there && old ? *scale : 0.f;
+    u32x4 w[E];
+    uint32_t top = 0;                                  // two magnitudes, as whole numbers: what is not finite is larger than all others
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        const int g = lane + i * LANES, row = g / per_row;
+        w[i] = u32x4{0u, 0u, 0u, 0u};
+        if (g < n) w[i] = *reinterpret_cast<const u32x4*>(x + row * x_row + 8 * (g - row * per_row));
+    }
+    auto higher = [](uint32_t a, uint32_t b) {
+        typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+    };
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) top = higher(top, w[i][j] & 0x7fff7fffu);
+#pragma unroll
+    for (int m = 1; m < (LANES < 64 ? LANES : 64); m *= 2) top = higher(top, (uint32_t)__shfl_xor((int)top, m, 64));
+    if constexpr (LANES > 64) {
+        if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+        __syncthreads();
+        top = higher(higher(tops[0], tops[1]), higher(tops[2], tops[3]));
+        if (!there) return;
+    }
+    top = max(top & 0xffffu, top >> 16);
+    const float a = __builtin_bit_cast(float, top << 16);
+    float s;
+    int grow = 0;
+    bool lost = top >= 0x7f80u;
+    if (old == 0) {
+        s = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, a / Q) + 0xfffffu) & ~0xfffffu);
+        s = fmaxf(s, kLeastScale);
+    } else {
+        lost |= !(s_old >= kLeastScale && s_old <= 3.4e38f);
+        if (!lost && a > Q * s_old) {
+            int e;
+            const float m = __builtin_frexpf(a / (Q * s_old), &e);
+            grow = m > 0.5f ? e : e - 1;
+        }
+        s = __builtin_ldexpf(s_old, grow);
+    }
+    if (lost) s = 1.f;
+    const float r = 1.0f / s;
+    auto quotient = [&](float v) {                     // v / s, correctly rounded where that is a border of the codes
+        const float q = v * r;
+        return fmaf(fmaf(-q, s, v), r, q);
+    };
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        const int g = lane + i * LANES, row = g / per_row;
+        if (g >= n) continue;
+        u32x2 out;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+            out[j] = lost ? 0u : f32_to_codes<CODE>(quotient(bf16_lo(w[i][2 * j])), quotient(bf16_hi(w[i][2 * j])), quotient(bf16_lo(w[i][2 * j + 1])),
+                                                    quotient(bf16_hi(w[i][2 * j + 1])));
+        *reinterpret_cast<u32x2*>(c + (old + row) * c_row + 8 * (g - row * per_row)) = out;
+    }
+    if (grow > 0 && !lost) {                           // the older tokens' codes
+        const float f = __builtin_ldexpf(1.0f, -grow);
+        for (int g = lane; g < old * per_row; g += LANES) {
+            const int row = g / per_row;
+            u32x2* const place = reinterpret_cast<u32x2*>(c + row * c_row + 8 * (g - row * per_row));
+            u32x2 v = *place;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const f32x4 y = codes_to_f32<CODE>(v[j]);
+                v[j] = f32_to_codes<CODE>(y[0] * f, y[1] * f, y[2] * f, y[3] * f);
+            }
+            *place = v;
+        }
+    }
+    if (lane == 0) *scale = lost ? __builtin_nanf("") : s;
+}
+
+struct KvLoadParams {
+    const void* c[2];              // K and V: [pages][Hkv][page][d] through cs (b: page, h: head, n: token)
+    const float* s[2];             // scales of codes, or null: bf16
+    uint16_t* y[2];                // [rows][Hkv][d] through ys (n: row, h: head)
+    Strides cs[2], ss[2], ys[2];
+    const int32_t* table;
+    int64_t table_stride;
+    int table_pages;
+    const int32_t* cu;             // [n + 1]: rows of the sequences
+    const int32_t* start;          // [n]: place of a sequence's first row in its pages
+    int n, rows, Hkv, d, n_pages, page_shift, block_shift;
+    int rows_per_wave;
+};
+
+// CODE < 0: bf16.  A wavefront takes one row, all heads of K and V, 16 bytes of the cache per lane and access, or as many rows as make 64 accesses.
+// Rows behind the last sequence are zeros, a row without a place in the cache is NaN.
+template <int CODE>
+static __global__ __launch_bounds__(256) void kv_load_kernel(const KvLoadParams p) {
+    constexpr int PER = CODE < 0 ? 8 : 16;             // numbers in 16 bytes
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r0 = ((int)blockIdx.x * 4 + wave) * p.rows_per_wave;
+    if (r0 >= p.rows) return;
+    const int last = packed_find(p.n, r0, [&](int at) { return packed_bound(p.cu, at, p.rows); });
+    const int per_row = p.d / PER, n = p.Hkv * per_row, together = min(n, 64), sub = lane / together, r = r0 + sub;
+    if (sub >= p.rows_per_wave || r >= p.rows) return;
+    int b = last;
+    while (b < p.n && packed_bound(p.cu, b + 1, p.rows) <= r) ++b;
+    const bool behind = b >= p.n;
+    int page = -1;
+    int64_t pos = 0;
+    if (!behind) {
+        pos = (int64_t)p.start[b] + (r - packed_bound(p.cu, b, p.rows));
+        if (pos >= 0 && (pos >> p.page_shift) < p.table_pages) page = p.table[b * p.table_stride + (pos >> p.page_shift)];
+    }
+    const bool there = page >= 0 && page < p.n_pages;
+    const int token = (int)(pos & ((1 << p.page_shift) - 1));
+    const uint32_t other = behind ? 0u : 0x7fc07fc0u;
+    for (int e = lane - sub * together; e < n; e += together) {
+        const int h = e / per_row, col = PER * (e - h * per_row);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            uint16_t* const to = p.y[t] + r * p.ys[t].n + h * p.ys[t].h + col;
+            u32x4 w = u32x4{other, other, other, other}, more = w;
+            if (there) {
+                const int64_t from = page * p.cs[t].b + h * p.cs[t].h + token * p.cs[t].n + col;
+                if constexpr (CODE < 0) {
+                    w = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p.c[t]) + from);
+                } else {
+                    const u32x4 c = *reinterpret_cast<const u32x4*>(static_cast<const uint8_t*>(p.c[t]) + from);
+                    const float s = p.s[t][page * p.ss[t].b + h * p.ss[t].h + (token >> p.block_shift) * p.ss[t].n];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const f32x4 v = codes_to_f32<CODE>(c[i]);
+                        (i < 2 ? w : more)[2 * (i & 1)] = pack_bf16(v[0] * s, v[1] * s);
+                        (i < 2 ? w : more)[2 * (i & 1) + 1] = pack_bf16(v[2] * s, v[3] * s);
+                    }
+                }
+            }
+            *reinterpret_cast<u32x4*>(to) = w;
+            if constexpr (CODE >= 0) *reinterpret_cast<u32x4*>(to + 8) = more;
+        }
+    }
+}
+
+}  // namespace fattn

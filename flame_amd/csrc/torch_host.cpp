@@ -14,6 +14,7 @@
 #include <dlfcn.h>
 
 #include <algorithm>
+#include <array>
 #include <cmath>
 #include <unordered_set>
 #include <vector>
@@ -44,6 +45,7 @@ using at::Tensor;
     X(flame_attn_bwd_materialised_bf16) X(flame_sage_quant_qk_int8_ks) X(flame_sage_attn_fwd_bias_int8)                 \
     X(flame_attn_packed_fwd_bf16) X(flame_attn_packed_fwd_workspace_bytes) X(flame_attn_packed_bwd_bf16) X(flame_attn_packed_bwd_workspace_bytes)                \
     X(flame_attn_paged_workspace_bytes) X(flame_attn_paged_fwd_bf16) X(flame_kv_store_bf16) X(flame_kv_copy_pages_bf16)  \
+    X(flame_attn_paged_fwd_q8) X(flame_kv_store_q8) X(flame_kv_load) X(flame_kv_copy_pages_q8) X(flame_rotary)           \
     X(flame_attn_prep_rmsnorm_rope_bf16) X(flame_bf16_to_fp8) X(flame_fp8_to_bf16) X(flame_attn_cast_qkv_f32_to_bf16) X(flame_attn_cast_bf16_to_f32)
 
 struct Api {
@@ -865,7 +867,7 @@ struct SdpaPacked : public torch::autograd::Function<SdpaPacked> {
 
 // A leaf whose gradients an earlier graph, still alive, accumulates on another stream: its backward would wait for that stream, which
 // in a capture is an error that the autograd engine does not survive.  Refused where the capture can still be told.
-void check_capture(const Tensor& t) {
+void check_capture(const Tensor& t, const char* call) {
     if (!t.requires_grad()) return;
     const c10::Stream now = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).unwrap();
     const auto first = t.is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(t) : t.grad_fn();
@@ -878,7 +880,7 @@ void check_capture(const Tensor& t) {
         for (const auto& edge : node->next_edges()) todo.push_back(edge.function.get());
         if (!dynamic_cast<torch::autograd::AccumulateGrad*>(node)) continue;
         const auto stream = node->stream();
-        TORCH_CHECK(!stream || *stream == now, "packed attention: a graph recorded on another stream holds one of the leaves; delete it before its backward is captured");
+        TORCH_CHECK(!stream || *stream == now, call, ": a graph recorded on another stream holds one of the leaves; delete it before its backward is captured");
     }
 }
 
@@ -900,7 +902,7 @@ PyObject* py_sdpa_packed(PyObject*, PyObject* const* a, Py_ssize_t n) {
             const at::ScalarType orig = q.scalar_type();
             const bool graph = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad());
             if (graph && c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None)
-                for (const Tensor* t : {&q, &k, &v}) check_capture(*t);
+                for (const Tensor* t : {&q, &k, &v}) check_capture(*t, "packed attention");
             const Tensor qb = packed_rows(q), kb = packed_rows(k), vb = packed_rows(v);
             Tensor lse;
             if (graph) out = SdpaPacked::apply(qb, kb, vb, cu_q, cu_k, causal, scale);
@@ -967,11 +969,33 @@ PyObject* py_attn_packed_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // ---------------------------------------------------------------- paged cache
+// Scales of a cache in 8 bits; undefined: the cache is bf16.
+struct CacheScales {
+    Tensor k, v;
+    bool codes() const { return k.defined(); }
+    int block(const Tensor& kc) const { return codes() ? (int)(kc.size(-2) / k.size(-1)) : 0; }        // tokens that share one
+    const int64_t* ks() const { return codes() ? k.strides().data() : nullptr; }
+    const int64_t* vs() const { return codes() ? v.strides().data() : nullptr; }
+};
+int cache_dtype(const Tensor& kc) {
+    return kc.scalar_type() == at::kChar ? FLAME_ATTN_DTYPE_I8 : kc.scalar_type() == at::kFloat8_e4m3fn ? FLAME_ATTN_DTYPE_E4M3 : FLAME_ATTN_DTYPE_BF16;
+}
 // [pages, Hkv, page, D], or with the layers in front for the copies
-void check_caches(const Tensor& kc, const Tensor& vc, int64_t dims, const char* what) {
+void check_caches(const Tensor& kc, const Tensor& vc, const CacheScales& c, int64_t dims, const char* what) {
     if (kc.dim() != dims || vc.dim() != dims) fail(PyExc_ValueError, what);
     check_that(kc.sizes() == vc.sizes() && kc.numel() > 0, "the two caches have one shape");
-    check_that(kc.scalar_type() == at::kBFloat16 && vc.scalar_type() == at::kBFloat16, "the caches are bf16");
+    check_that(c.k.defined() == c.v.defined(), "both caches have scales, or neither has");
+    if (!c.codes()) {
+        check_that(kc.scalar_type() == at::kBFloat16 && vc.scalar_type() == at::kBFloat16, "the caches are bf16 (8 bits: with their scales)");
+    } else {
+        check_that(cache_dtype(kc) != FLAME_ATTN_DTYPE_BF16 && kc.scalar_type() == vc.scalar_type(), "caches with scales are both int8 or both float8_e4m3fn");
+        for (const Tensor* t : {&c.k, &c.v}) {
+            check_that(t->dim() == dims - 1 && t->scalar_type() == at::kFloat, "the scales are fp32 tensors, of one dimension less than the caches");
+            for (int64_t ax = 0; ax + 2 < dims; ++ax) check_that(t->size(ax) == kc.size(ax), "the scales have the caches' pages and heads");
+            check_that(t->size(dims - 2) > 0 && t->size(dims - 2) == c.k.size(dims - 2) && kc.size(dims - 2) % t->size(dims - 2) == 0, "the scales divide a page into blocks");
+            check_device(*t, kc, "all tensors are on one GPU");
+        }
+    }
     check_device(kc, kc, "the tensors are on a GPU");
     check_device(vc, kc, "all tensors are on one GPU");
 }
@@ -988,26 +1012,27 @@ const int32_t* ints(const Tensor& t) { return static_cast<const int32_t*>(ptr(t)
 
 // Inputs of a call that autograd knows nothing of: what they carry would be lost without a word.
 void check_no_derivative(std::initializer_list<const Tensor*> inputs, const char* call) {
-    for (const Tensor* t : inputs) TORCH_CHECK_NOT_IMPLEMENTED(!t->_fw_grad(0).defined(), call, " has no forward-mode derivative: an input carries a tangent");
+    for (const Tensor* t : inputs) TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), call, " has no forward-mode derivative: an input carries a tangent");
     if (!at::GradMode::is_enabled()) return;
     for (const Tensor* t : inputs)
-        TORCH_CHECK(!t->requires_grad(), call, " has no backward and an input requires a gradient: call it under torch.no_grad()");
+        TORCH_CHECK(!t->defined() || !t->requires_grad(), call, " has no backward and an input requires a gradient: call it under torch.no_grad()");
 }
 // A launch may have written to the caches: graphs that saved them, or views of them, are told (rc: not one of the refusals that come before any
 // launch).  A tensor of inference mode is in no graph and has no version.
 void raise_versions(int rc, std::initializer_list<const Tensor*> written) {
     if (rc == FLAME_ATTN_ERR_INVALID || rc == FLAME_ATTN_ERR_UNSUPPORTED) return;
     for (const Tensor* t : written)
-        if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+        if (t->defined() && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
 }
 
 struct PagedCall {
     Tensor table, kv_len, prefix_table, prefix_len;
+    CacheScales scales;
 };
 // checks of everything but q's dtype and layout
 void check_paged(const Tensor& q, const Tensor& kc, const Tensor& vc, const PagedCall& c) {
     check_4d(q);
-    check_caches(kc, vc, 4, "the caches are 4-D [pages, key heads, page, D]");
+    check_caches(kc, vc, c.scales, 4, "the caches are 4-D [pages, key heads, page, D]");
     check_device(kc, q, "all tensors are on one GPU");
     check_that(q.numel() > 0 && q.size(3) == kc.size(3) && q.size(1) % kc.size(1) == 0, "q is [B, H, N, D] with the caches' head dim and a multiple of their heads");
     check_table(c.table, q.size(0), q);
@@ -1029,19 +1054,29 @@ void call_paged(const Tensor& q, const Tensor& kc, const Tensor& vc, const Paged
     if (want_lse) lse = empty({(int64_t)B * H, N}, at::kFloat, q);
     if (!workspace.defined())
         if (const size_t need = g_api.flame_attn_paged_workspace_bytes(B, H, Hkv, N, D, page, pages, prefix)) workspace = bytes_like(need, q);
+    if (c.scales.codes()) {
+        check_rc(g_api.flame_attn_paged_fwd_q8(ptr(q), ptr(kc), ptr(vc), cache_dtype(kc), static_cast<const float*>(ptr(c.scales.k)),
+                                               static_cast<const float*>(ptr(c.scales.v)), c.scales.block(kc), ptr(o), ptr(lse), ints(c.table), c.table.stride(0),
+                                               pages, ints(c.kv_len), ints(c.prefix_table), prefix, ints(c.prefix_len), B, H, Hkv, N, D, (int)kc.size(0), page,
+                                               scale, strides4(q), strides4(kc), strides4(vc), c.scales.ks(), c.scales.vs(), strides4(o), ptr(workspace),
+                                               workspace.defined() ? (size_t)workspace.numel() : 0, stream_of(q)),
+                 "flame_attn_paged_fwd_q8");
+        return;
+    }
     check_rc(g_api.flame_attn_paged_fwd_bf16(ptr(q), ptr(kc), ptr(vc), ptr(o), ptr(lse), ints(c.table), c.table.stride(0), pages, ints(c.kv_len),
                                              ints(c.prefix_table), prefix, ints(c.prefix_len), B, H, Hkv, N, D, (int)kc.size(0), page, scale, strides4(q),
                                              strides4(kc), strides4(vc), strides4(o), ptr(workspace), workspace.defined() ? (size_t)workspace.numel() : 0, stream_of(q)),
              "flame_attn_paged_fwd_bf16");
 }
 
-// sdpa_paged(q, k_cache, v_cache, page_table, kv_len, prefix_table | None, prefix_len | None, scale | None) -> o
+// sdpa_paged(q, k_cache, v_cache, page_table, kv_len, prefix_table | None, prefix_len | None, scale | None, k_scale | None, v_scale | None) -> o
 PyObject* py_sdpa_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
-        need_args(n, 8);
+        need_args(n, 10);
         const Tensor &q = tensor_arg(a[0], "q"), &kc = tensor_arg(a[1], "k_cache"), &vc = tensor_arg(a[2], "v_cache");
-        const PagedCall c{tensor_arg(a[3], "page_table"), tensor_arg(a[4], "kv_len"), opt_tensor_arg(a[5], "prefix_table"), opt_tensor_arg(a[6], "prefix_len")};
-        check_no_derivative({&q, &kc, &vc}, "paged attention");
+        const PagedCall c{tensor_arg(a[3], "page_table"), tensor_arg(a[4], "kv_len"), opt_tensor_arg(a[5], "prefix_table"), opt_tensor_arg(a[6], "prefix_len"),
+                          {opt_tensor_arg(a[8], "k_scale"), opt_tensor_arg(a[9], "v_scale")}};
+        check_no_derivative({&q, &kc, &vc, &c.scales.k, &c.scales.v}, "paged attention");
         check_paged(q, kc, vc, c);
         const float scale = (float)(a[7] == Py_None ? 1.0 / std::sqrt((double)q.size(3)) : float_arg(a[7]));
         Tensor o, lse;
@@ -1056,12 +1091,13 @@ PyObject* py_sdpa_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
-// attn_paged_fwd(q, k_cache, v_cache, page_table, kv_len, scale, prefix_table, prefix_len, want_lse, out, workspace) -> (o, lse | None)
+// attn_paged_fwd(q, k_cache, v_cache, page_table, kv_len, scale, prefix_table, prefix_len, want_lse, out, workspace, k_scale, v_scale) -> (o, lse | None)
 PyObject* py_attn_paged_fwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
-        need_args(n, 11);
+        need_args(n, 13);
         const Tensor &q = tensor_arg(a[0], "q"), &kc = tensor_arg(a[1], "k_cache"), &vc = tensor_arg(a[2], "v_cache");
-        const PagedCall c{tensor_arg(a[3], "page_table"), tensor_arg(a[4], "kv_len"), opt_tensor_arg(a[6], "prefix_table"), opt_tensor_arg(a[7], "prefix_len")};
+        const PagedCall c{tensor_arg(a[3], "page_table"), tensor_arg(a[4], "kv_len"), opt_tensor_arg(a[6], "prefix_table"), opt_tensor_arg(a[7], "prefix_len"),
+                          {opt_tensor_arg(a[11], "k_scale"), opt_tensor_arg(a[12], "v_scale")}};
         check_paged(q, kc, vc, c);
         check_that(q.scalar_type() == at::kBFloat16, "q is bf16");
         const float scale = (float)float_arg(a[5]);
@@ -1079,15 +1115,16 @@ PyObject* py_attn_paged_fwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
-// kv_store(k, v, k_cache, v_cache, page_table, cu, start)
+// kv_store(k, v, k_cache, v_cache, page_table, cu, start, k_scale | None, v_scale | None)
 PyObject* py_kv_store(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
-        need_args(n, 7);
+        need_args(n, 9);
         const Tensor &k = tensor_arg(a[0], "k"), &v = tensor_arg(a[1], "v"), &kc = tensor_arg(a[2], "k_cache"), &vc = tensor_arg(a[3], "v_cache"),
                      &table = tensor_arg(a[4], "page_table"), &cu = tensor_arg(a[5], "cu"), &start = tensor_arg(a[6], "start");
-        check_no_derivative({&k, &v, &kc, &vc}, "a store into the cache");
+        const CacheScales scales{opt_tensor_arg(a[7], "k_scale"), opt_tensor_arg(a[8], "v_scale")};
+        check_no_derivative({&k, &v, &kc, &vc, &scales.k, &scales.v}, "a store into the cache");
         if (k.dim() != 3) fail(PyExc_ValueError, "k and v are 3-D [rows, key heads, D]");
-        check_caches(kc, vc, 4, "the caches are 4-D [pages, key heads, page, D]");
+        check_caches(kc, vc, scales, 4, "the caches are 4-D [pages, key heads, page, D]");
         check_that(k.sizes() == v.sizes() && k.numel() > 0 && k.size(1) == kc.size(1) && k.size(2) == kc.size(3), "k and v have one shape, with the caches' heads and head dim");
         check_that(k.scalar_type() == at::kBFloat16 && v.scalar_type() == at::kBFloat16, "k and v are bf16");
         check_device(k, kc, "all tensors are on one GPU");
@@ -1100,13 +1137,62 @@ PyObject* py_kv_store(PyObject*, PyObject* const* a, Py_ssize_t n) {
         {
             WithoutGil nogil;
             c10::OptionalDeviceGuard device(kc.device());
-            const int rc = g_api.flame_kv_store_bf16(ptr(k), ptr(v), ptr(kc), ptr(vc), ints(table), table.stride(0), (int)table.size(1), ints(cu), ints(start),
-                                                     (int)table.size(0), (int)k.size(0), (int)k.size(1), (int)k.size(2), (int)kc.size(0), (int)kc.size(2),
-                                                     strides4(k), strides4(v), strides4(kc), strides4(vc), stream_of(kc));
-            raise_versions(rc, {&kc, &vc});
-            check_rc(rc, "flame_kv_store_bf16");
+            const int seqs = (int)table.size(0), rows = (int)k.size(0), heads = (int)k.size(1), D = (int)k.size(2), pages = (int)kc.size(0), page = (int)kc.size(2);
+            const int rc = scales.codes()
+                               ? g_api.flame_kv_store_q8(ptr(k), ptr(v), ptr(kc), ptr(vc), cache_dtype(kc), static_cast<float*>(ptr(scales.k)),
+                                                         static_cast<float*>(ptr(scales.v)), scales.block(kc), ints(table), table.stride(0), (int)table.size(1), ints(cu),
+                                                         ints(start), seqs, rows, heads, D, pages, page, strides4(k), strides4(v), strides4(kc), strides4(vc),
+                                                         scales.ks(), scales.vs(), stream_of(kc))
+                               : g_api.flame_kv_store_bf16(ptr(k), ptr(v), ptr(kc), ptr(vc), ints(table), table.stride(0), (int)table.size(1), ints(cu), ints(start),
+                                                           seqs, rows, heads, D, pages, page, strides4(k), strides4(v), strides4(kc), strides4(vc), stream_of(kc));
+            raise_versions(rc, {&kc, &vc, &scales.k, &scales.v});
+            check_rc(rc, scales.codes() ? "flame_kv_store_q8" : "flame_kv_store_bf16");
         }
         return Py_NewRef(Py_None);
+    });
+}
+
+// kv_load(k_cache, v_cache, page_table, cu, start, rows, k_scale | None, v_scale | None, k_out | None, v_out | None) -> (k, v)
+PyObject* py_kv_load(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        need_args(n, 10);
+        const Tensor &kc = tensor_arg(a[0], "k_cache"), &vc = tensor_arg(a[1], "v_cache"), &table = tensor_arg(a[2], "page_table"), &cu = tensor_arg(a[3], "cu"),
+                     &start = tensor_arg(a[4], "start");
+        const long rows = long_arg(a[5]);
+        const CacheScales scales{opt_tensor_arg(a[6], "k_scale"), opt_tensor_arg(a[7], "v_scale")};
+        Tensor k = opt_tensor_arg(a[8], "k_out"), v = opt_tensor_arg(a[9], "v_out");
+        check_no_derivative({&kc, &vc, &scales.k, &scales.v, &k, &v}, "a load from the cache");
+        check_caches(kc, vc, scales, 4, "the caches are 4-D [pages, key heads, page, D]");
+        check_that(rows > 0, "a load has at least one row");
+        size32(rows);
+        check_that(k.defined() == v.defined(), "both outputs or neither");
+        for (const Tensor* t : {&k, &v}) {
+            if (!t->defined()) continue;
+            check_that(t->scalar_type() == at::kBFloat16 && t->dim() == 3 && t->size(0) == rows && t->size(1) == kc.size(1) && t->size(2) == kc.size(3),
+                       "the outputs are bf16 [rows, key heads, D]");
+            check_device(*t, kc, "all tensors are on one GPU");
+        }
+        check_bounds(cu, kc);
+        check_table(table, cu.size(0) - 1, kc);
+        check_ints(start, cu.size(0) - 1, kc, "start is an int32 [sequences] tensor");
+        for (const Tensor* t : {&kc, &table})
+            for (int64_t s : t->sizes()) size32(s);
+        {
+            WithoutGil nogil;
+            c10::OptionalDeviceGuard device(kc.device());
+            const bool given = k.defined();
+            if (!given) {
+                k = empty({rows, kc.size(1), kc.size(3)}, at::kBFloat16, kc);
+                v = empty({rows, kc.size(1), kc.size(3)}, at::kBFloat16, kc);
+            }
+            const int rc = g_api.flame_kv_load(ptr(kc), ptr(vc), cache_dtype(kc), static_cast<const float*>(ptr(scales.k)), static_cast<const float*>(ptr(scales.v)),
+                                               scales.block(kc), ptr(k), ptr(v), ints(table), table.stride(0), (int)table.size(1), ints(cu), ints(start),
+                                               (int)table.size(0), (int)rows, (int)kc.size(1), (int)kc.size(3), (int)kc.size(0), (int)kc.size(2), strides4(kc),
+                                               strides4(vc), scales.ks(), scales.vs(), strides4(k), strides4(v), stream_of(kc));
+            if (given) raise_versions(rc, {&k, &v});
+            check_rc(rc, "flame_kv_load");
+        }
+        return pair(k, v);
     });
 }
 
@@ -1128,15 +1214,21 @@ std::vector<int32_t> int_list(PyObject* o) {
     Py_DECREF(seq);
     return out;
 }
-// kv_copy_pages(k_cache, v_cache, src, dst): caches [pages, Hkv, page, D] or [layers, pages, Hkv, page, D]
+// kv_copy_pages(k_cache, v_cache, src, dst, k_scale | None, v_scale | None): caches [pages, Hkv, page, D] or [layers, pages, Hkv, page, D]
 PyObject* py_kv_copy_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
-        need_args(n, 4);
+        need_args(n, 6);
         const Tensor &k_cache = tensor_arg(a[0], "k_cache"), &v_cache = tensor_arg(a[1], "v_cache");
-        check_no_derivative({&k_cache, &v_cache}, "a copy of pages");
+        const CacheScales given{opt_tensor_arg(a[4], "k_scale"), opt_tensor_arg(a[5], "v_scale")};
+        check_no_derivative({&k_cache, &v_cache, &given.k, &given.v}, "a copy of pages");
         Tensor kc = k_cache, vc = v_cache;
-        if (kc.dim() == 4 && vc.dim() == 4) kc = kc.unsqueeze(0), vc = vc.unsqueeze(0);
-        check_caches(kc, vc, 5, "the caches are [pages, key heads, page, D], with the layers in front or without");
+        CacheScales scales = given;
+        if (kc.dim() == 4 && vc.dim() == 4) {
+            kc = kc.unsqueeze(0), vc = vc.unsqueeze(0);
+            if (given.k.defined()) scales.k = given.k.unsqueeze(0);
+            if (given.v.defined()) scales.v = given.v.unsqueeze(0);
+        }
+        check_caches(kc, vc, scales, 5, "the caches are [pages, key heads, page, D], with the layers in front or without");
         const std::vector<int32_t> src = int_list(a[2]), dst = int_list(a[3]);
         check_that(src.size() == dst.size(), "as many sources as destinations");
         size32((int64_t)src.size());
@@ -1144,12 +1236,150 @@ PyObject* py_kv_copy_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
         {
             WithoutGil nogil;
             c10::OptionalDeviceGuard device(kc.device());
-            const int rc = g_api.flame_kv_copy_pages_bf16(ptr(kc), ptr(vc), (int)kc.size(0), (int)kc.size(1), (int)kc.size(2), (int)kc.size(3),
-                                                          (int)kc.size(4), strides4(kc), strides4(vc), src.data(), dst.data(), (int)src.size(), stream_of(kc));
-            if (!src.empty()) raise_versions(rc, {&k_cache, &v_cache});
-            check_rc(rc, "flame_kv_copy_pages_bf16");
+            const int layers = (int)kc.size(0), pages = (int)kc.size(1), heads = (int)kc.size(2), page = (int)kc.size(3), D = (int)kc.size(4);
+            const int rc = scales.codes()
+                               ? g_api.flame_kv_copy_pages_q8(ptr(kc), ptr(vc), static_cast<float*>(ptr(scales.k)), static_cast<float*>(ptr(scales.v)), layers, pages,
+                                                              heads, page, D, scales.block(kc), strides4(kc), strides4(vc), scales.ks(), scales.vs(), src.data(),
+                                                              dst.data(), (int)src.size(), stream_of(kc))
+                               : g_api.flame_kv_copy_pages_bf16(ptr(kc), ptr(vc), layers, pages, heads, page, D, strides4(kc), strides4(vc), src.data(), dst.data(),
+                                                                (int)src.size(), stream_of(kc));
+            if (!src.empty()) raise_versions(rc, {&k_cache, &v_cache, &given.k, &given.v});
+            check_rc(rc, scales.codes() ? "flame_kv_copy_pages_q8" : "flame_kv_copy_pages_bf16");
         }
         return Py_NewRef(Py_None);
+    });
+}
+
+// ---------------------------------------------------------------- rotary positions
+// How the heads are turned, and by which positions: those of every token, or those of the rows of packed sequences.
+struct RotaryCall {
+    Tensor turns, positions, cu, start;
+    bool interleaved = false;
+    double size = 1.0;
+};
+Tensor rotary_input(const Tensor& x) { return x.stride(-1) == 1 || x.size(-1) == 1 ? x : x.clone(at::MemoryFormat::Contiguous); }
+// [rows, heads, D] or [B, heads, S, D] as (B, heads, S, D) strides
+std::array<int64_t, 4> rotary_strides(const Tensor& x) {
+    if (x.dim() == 4) return {x.stride(0), x.stride(1), x.stride(2), 1};
+    return {0, x.stride(1), x.stride(0), 1};
+}
+int call_rotary(const Tensor& q, const Tensor& k, const RotaryCall& c, bool inverse, Tensor& yq, Tensor& yk) {
+    const bool rows = q.dim() == 3;
+    const auto qs = rotary_strides(q), qo = rotary_strides(yq);
+    std::array<int64_t, 4> ks{}, ko{};
+    if (k.defined()) ks = rotary_strides(k), ko = rotary_strides(yk);
+    const int dtype = q.scalar_type() == at::kFloat ? FLAME_ATTN_DTYPE_F32 : q.scalar_type() == at::kHalf ? FLAME_ATTN_DTYPE_F16 : FLAME_ATTN_DTYPE_BF16;
+    return g_api.flame_rotary(ptr(q), ptr(yq), (int)q.size(1), qs.data(), qo.data(), ptr(k), ptr(yk), k.defined() ? (int)k.size(1) : 0, ks.data(), ko.data(), dtype,
+                              static_cast<const int64_t*>(ptr(c.turns)), (int)(2 * c.turns.numel()), c.interleaved, (float)c.size, inverse, ints(c.positions),
+                              c.positions.defined() && c.positions.dim() == 2 && c.positions.size(0) > 1 ? c.positions.stride(0) : 0, ints(c.cu), ints(c.start),
+                              c.cu.defined() ? (int)c.cu.size(0) - 1 : 0, rows ? 1 : (int)q.size(0), (int)q.size(rows ? 0 : 2), (int)q.size(-1), stream_of(q));
+}
+// a result of x's shape, dense in x's order of axes where x is dense
+Tensor rotary_like(const Tensor& x) {
+    Tensor y = at::empty_like(x);
+    return y.stride(-1) == 1 || y.size(-1) == 1 ? y : at::empty(x.sizes(), x.options());
+}
+
+struct Rotary : public torch::autograd::Function<Rotary> {
+    // the positions and frequencies are all that the backward needs; it is a turn itself and so can be derived again
+    using Maybe = std::optional<Tensor>;        // (a plain argument of this kind is asked for its device)
+    static Tensor tensor(const Maybe& t) { return t ? *t : Tensor(); }
+    static Maybe maybe(const Tensor& t) { return t.defined() ? Maybe(t) : std::nullopt; }
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Maybe& maybe_k, const Tensor& turns,
+                                                  const Maybe& positions, const Maybe& cu, const Maybe& start, bool interleaved, double size, bool inverse) {
+        const RotaryCall c{turns, tensor(positions), tensor(cu), tensor(start), interleaved, size};
+        const Tensor k = tensor(maybe_k);
+        Tensor yq = rotary_like(q), yk = k.defined() ? rotary_like(k) : Tensor();
+        const int rc = call_rotary(q, k, c, inverse, yq, yk);
+        if (rc != FLAME_ATTN_OK) throw_python({"flame_rotary", rc});
+        ctx->save_for_backward({turns, c.positions, c.cu, c.start});
+        ctx->saved_data["interleaved"] = interleaved;
+        ctx->saved_data["size"] = size;
+        ctx->saved_data["inverse"] = inverse;
+        if (!k.defined()) return {yq};
+        return {yq, yk};
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        const bool interleaved = ctx->saved_data["interleaved"].toBool(), inverse = ctx->saved_data["inverse"].toBool();
+        const double size = ctx->saved_data["size"].toDouble();
+        c10::OptionalDeviceGuard device(grads[0].device());
+        const Tensor dq = rotary_input(grads[0]), dk = grads.size() > 1 ? rotary_input(grads[1]) : Tensor();
+        torch::autograd::variable_list out;
+        if (at::GradMode::is_enabled()) {
+            out = Rotary::apply(dq, maybe(dk), saved[0], maybe(saved[1]), maybe(saved[2]), maybe(saved[3]), interleaved, size, !inverse);
+        } else {
+            const RotaryCall c{saved[0], saved[1], saved[2], saved[3], interleaved, size};
+            Tensor yq = rotary_like(dq), yk = dk.defined() ? rotary_like(dk) : Tensor();
+            const int rc = call_rotary(dq, dk, c, !inverse, yq, yk);
+            if (rc != FLAME_ATTN_OK) throw_python({"flame_rotary", rc});
+            out = {yq, yk};
+        }
+        return {out[0], grads.size() > 1 ? out[1] : Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+
+// rotary(q, k | None, turns, interleaved, size, positions | None, cu | None, start | None, inverse) -> q' or (q', k')
+PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        need_args(n, 9);
+        const Tensor& q = tensor_arg(a[0], "q");
+        const Tensor k = opt_tensor_arg(a[1], "k");
+        const RotaryCall c{tensor_arg(a[2], "turns"), opt_tensor_arg(a[5], "positions"), opt_tensor_arg(a[6], "cu_seqlens"), opt_tensor_arg(a[7], "start"),
+                           bool_arg(a[3]), float_arg(a[4])};
+        const bool inverse = bool_arg(a[8]);
+        for (const Tensor* t : {&q, &k})
+            TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), "rotary positions have no forward-mode derivative: an input carries a tangent");
+        if (q.dim() != 3 && q.dim() != 4) fail(PyExc_ValueError, "rotary positions expect [rows, heads, D] or [B, heads, S, D]");
+        const bool rows = q.dim() == 3;
+        check_that(q.numel() > 0, "rotary positions need at least one element");
+        check_that(q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf || q.scalar_type() == at::kFloat, "q and k are bf16, fp16 or fp32");
+        check_device(q, q, "the tensors are on a GPU");
+        if (k.defined()) {
+            check_that(k.dim() == q.dim() && k.numel() > 0 && k.scalar_type() == q.scalar_type(), "k has q's type and number of axes");
+            for (int64_t ax = 0; ax < q.dim(); ++ax) check_that(ax == 1 || k.size(ax) == q.size(ax), "k has q's shape, but for the heads");
+            check_device(k, q, "all tensors are on one GPU");
+        }
+        check_that(c.turns.scalar_type() == at::kLong && c.turns.dim() == 1 && c.turns.is_contiguous() && c.turns.numel() > 0 && 2 * c.turns.numel() <= q.size(-1),
+                   "turns is a contiguous int64 tensor of at most half the head dim");
+        check_device(c.turns, q, "all tensors are on one GPU");
+        check_that(c.positions.defined() != c.cu.defined(), "either positions or bounds of sequences");
+        if (c.positions.defined()) {
+            check_that(!c.start.defined(), "first positions are those of bounded sequences");
+            const Tensor& p = c.positions;
+            check_that(p.scalar_type() == at::kInt && (p.dim() == 1 || (p.dim() == 2 && !rows && p.size(0) == q.size(0))) && p.size(-1) == q.size(rows ? 0 : 2) &&
+                           (p.stride(-1) == 1 || p.size(-1) == 1),
+                       "positions are int32, contiguous, one for every row, or [S] or [B, S]");
+            check_device(p, q, "all tensors are on one GPU");
+        } else {
+            check_that(rows, "bounds of sequences are for [rows, heads, D]");
+            check_bounds(c.cu, q);
+            if (c.start.defined()) check_ints(c.start, c.cu.size(0) - 1, q, "start is an int32 [sequences] tensor");
+        }
+        for (const Tensor* t : {&q, &k, &c.cu})
+            if (t->defined())
+                for (int64_t s : t->sizes()) size32(s);
+        Tensor yq, yk;
+        {
+            WithoutGil nogil;
+            c10::OptionalDeviceGuard device(q.device());
+            const bool graph = at::GradMode::is_enabled() && (q.requires_grad() || (k.defined() && k.requires_grad()));
+            if (graph && c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None)
+                for (const Tensor* t : {&q, &k})
+                    if (t->defined()) check_capture(*t, "rotary positions");
+            const Tensor qx = rotary_input(q), kx = k.defined() ? rotary_input(k) : Tensor();
+            if (graph) {
+                const auto out = Rotary::apply(qx, Rotary::maybe(kx), c.turns, Rotary::maybe(c.positions), Rotary::maybe(c.cu), Rotary::maybe(c.start), c.interleaved,
+                                               c.size, inverse);
+                yq = out[0];
+                if (k.defined()) yk = out[1];
+            } else {
+                yq = rotary_like(qx);
+                if (k.defined()) yk = rotary_like(kx);
+                check_rc(call_rotary(qx, kx, c, inverse, yq, yk), "flame_rotary");
+            }
+        }
+        return k.defined() ? pair(yq, yk) : THPVariable_Wrap(yq);
     });
 }
 
@@ -1193,7 +1423,9 @@ PyMethodDef g_methods[] = {FLAME_HOST_METHOD("bind", py_bind),
                            FLAME_HOST_METHOD("sdpa_paged", py_sdpa_paged),
                            FLAME_HOST_METHOD("attn_paged_fwd", py_attn_paged_fwd),
                            FLAME_HOST_METHOD("kv_store", py_kv_store),
+                           FLAME_HOST_METHOD("kv_load", py_kv_load),
                            FLAME_HOST_METHOD("kv_copy_pages", py_kv_copy_pages),
+                           FLAME_HOST_METHOD("rotary", py_rotary),
                            FLAME_HOST_METHOD("attn_packed_fwd", py_attn_packed_fwd),
                            FLAME_HOST_METHOD("attn_packed_bwd", py_attn_packed_bwd),
                            {nullptr, nullptr, 0, nullptr}};

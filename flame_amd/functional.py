@@ -52,13 +52,28 @@ def sdpa_packed(q, k, v, cu_seqlens, cu_seqlens_k=None, is_causal=None, scale=No
     return capi.host().sdpa_packed(q, k, v, cu_seqlens, cu_seqlens_k, is_causal is not None and bool(is_causal), scale)
 
 
-def sdpa_paged(q, k_cache, v_cache, page_table, kv_len, prefix_table=None, prefix_len=None, scale=None):
-    """Attention of the last N tokens of every sequence, q [B, H, N, D], against a paged cache, bf16 [pages, H_kv, page, D]
+def sdpa_paged(q, k_cache, v_cache, page_table, kv_len, prefix_table=None, prefix_len=None, scale=None, k_scale=None, v_scale=None):
+    """Attention of the last N tokens of every sequence, q [B, H, N, D], against a paged cache [pages, H_kv, page, D], bf16 or in 8 bits
     (inference only; flame_amd.paged_cache keeps such a cache).
 
     page_table: int32 [B, pages], the pages of a sequence's own keys in their order; kv_len: int32 [B], how many own keys,
     the N new ones among them.  prefix_table (int32 [pages]) and prefix_len (int32 [1]): keys that all sequences have in
     front of their own, read once for the batch.  Token i attends to the prefix and to own keys j <= kv_len - N + i (an infinity or
     NaN in a later token's V reaches it all the same: its weight of 0 multiplies it).
+    Caches of int8 or float8_e4m3fn come with k_scale, v_scale (fp32 [pages, H_kv, page / block]), as capi.kv_store leaves them:
+    a number is its code times the scale of its block of tokens.
     q of another dtype is promoted to bf16 and the result is cast back."""
-    return capi.host().sdpa_paged(q, k_cache, v_cache, page_table, kv_len, prefix_table, prefix_len, scale)
+    return capi.host().sdpa_paged(q, k_cache, v_cache, page_table, kv_len, prefix_table, prefix_len, scale, k_scale, v_scale)
+
+
+def rotary(rope, q, k=None, positions=None, cu_seqlens=None, start=None):
+    """Rotary positions: q, and k with it, [rows, heads, D] or [B, heads, S, D] in bf16, fp16 or fp32, turned as `rope` (a
+    flame_amd.rotary.Rotary) says.  Returns q', or (q', k') with k.  Differentiable, as often as wanted.
+
+    Where the tokens are: positions, int32 on the device, one for every row, or [S] or [B, S]; or, for rows of packed sequences,
+    their bounds cu_seqlens (int32 [sequences + 1], as sdpa_packed takes them) and the position of each one's first row (start, int32
+    [sequences]; omitted: 0).  Rows behind the last sequence come out as zeros.  A recorded graph holds these tensors, so
+    they may not be refilled before its backward.  Its backward may be captured into a graph, with what sdpa_packed says of leaves."""
+    if q.shape[-1] != rope.head_dim:
+        raise ValueError(f"the head dim is {rope.head_dim}")
+    return capi.rotary(q, k, rope.turns_on(q.device), rope.interleaved, rope.size, positions, cu_seqlens, start)

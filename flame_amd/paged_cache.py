@@ -1,6 +1,6 @@
 """A paged cache of keys and values for incremental inference: the tensors, and the host's book of pages.
 
-    cache = PagedCache(layers=24, pages=4096, page=64, kv_heads=8, head_dim=128)
+    cache = PagedCache(layers=24, pages=4096, page=64, kv_heads=8, head_dim=128)       # dtype=torch.int8: half the bytes
     seq = cache.new()
     batch = cache.extend([seq], [len(prompt)])        # pages for the prompt; tables and lengths on the device
     for layer in ...:                                 # the prompt itself: functional.sdpa_packed
@@ -13,9 +13,17 @@
             o = cache.attend(layer, q, batch)         # q [8, H, 1, D]
     cache.free(answers)
 
+Pieces of prompts, different numbers of new tokens against what the sequences hold already:
+
+    batch, held = cache.extend(seqs, counts), cache.held(seqs)
+    q, k = functional.rotary(rope, q, k, cu_seqlens=batch.cu, start=batch.past)
+    for layer in ...:
+        cache.store(layer, k, v, batch)
+        o = cache.attend_rows(layer, q, batch, held)        # q [new tokens, H, D]
+
 The book is plain integers on the host: a page that several sequences share is counted and never written; what goes to the
-device is one small upload per `extend`.  Keys and values move in capi.kv_store and capi.kv_copy_pages, attention is
-functional.sdpa_paged; nothing here computes on the GPU by itself.  Not thread-safe; calls are ordered by the stream that is
+device is one small upload per `extend`.  Keys and values move in capi.kv_store, capi.kv_load and capi.kv_copy_pages, attention is
+functional.sdpa_paged or, for pieces, functional.sdpa_packed; nothing here computes on the GPU by itself.  Not thread-safe; calls are ordered by the stream that is
 current when they are made.  A batch is of use until one of its sequences is extended, cut or freed or the cache is compacted: after
 that its places may belong to others.  Inference only: `store` and `attend` are for torch.no_grad() or tensors that require no gradient.
 """
@@ -35,6 +43,7 @@ class PagedBatch:
     page_table: torch.Tensor            # [B, pages] of the sequences' own keys
     kv_len: torch.Tensor                # [B] own keys, the new ones among them
     start: torch.Tensor                 # [B] place of the first new token among the own ones
+    past: torch.Tensor                  # [B] its position: all tokens before it, the prefix's too
     cu: torch.Tensor                    # [B + 1] bounds of the new tokens' rows
     prefix_table: torch.Tensor | None   # [pages] that all sequences share in front of their own
     prefix_len: torch.Tensor | None     # [1]
@@ -42,18 +51,29 @@ class PagedBatch:
 
 
 class PagedCache:
-    """k, v: bf16 [layers, pages, kv_heads, page, head_dim]."""
+    """k, v: [layers, pages, kv_heads, page, head_dim], bf16, or with dtype int8 or float8_e4m3fn in 8 bits, rounded as they are stored, and
+    k_scale, v_scale: fp32 [layers, pages, kv_heads, page / block], a scale for every `block` tokens of a head (else None)."""
 
-    def __init__(self, layers, pages, page, kv_heads, head_dim, device="cuda"):
+    def __init__(self, layers, pages, page, kv_heads, head_dim, device="cuda", dtype=torch.bfloat16, block=16):
         if min(layers, pages, kv_heads, head_dim) < 1:
             raise ValueError("layers, pages, kv_heads and head_dim are positive")
         if page < 16 or page > 65536 or page & (page - 1):
             raise ValueError("a page holds a power of two tokens from 16 to 65536")
         if head_dim % 8 or head_dim > 128:
             raise ValueError("head_dim is a multiple of 8 up to 128")
+        if dtype not in (torch.bfloat16, torch.int8, torch.float8_e4m3fn):
+            raise ValueError("dtype is bfloat16, int8 or float8_e4m3fn")
         self.page = page
-        self.k = torch.empty((layers, pages, kv_heads, page, head_dim), dtype=torch.bfloat16, device=device)
+        self.k = torch.empty((layers, pages, kv_heads, page, head_dim), dtype=dtype, device=device)
         self.v = torch.empty_like(self.k)
+        self.k_scale = self.v_scale = None
+        if dtype != torch.bfloat16:
+            if head_dim % 16:
+                raise ValueError("in 8 bits head_dim is a multiple of 16")
+            if block < 1 or block > min(page, 128) or block & (block - 1):
+                raise ValueError("a power of two tokens up to 128 and to the page share a scale")
+            self.k_scale = torch.zeros((layers, pages, kv_heads, page // block), dtype=torch.float32, device=device)
+            self.v_scale = torch.zeros_like(self.k_scale)
         self._users = [0] * pages               # sequences that hold the page
         self._free = list(range(pages))         # a heap: the lowest page first
         self._pages: dict[int, list[int]] = {}
@@ -151,7 +171,7 @@ class PagedCache:
                     pages = pages[:-1]
                 lists.append(pages + new if new else pages)
             if src:
-                capi.kv_copy_pages(self.k, self.v, src, dst)
+                capi.kv_copy_pages(self.k, self.v, src, dst, *self._scales())
             batch = self._batch(lists, [self._len[s] + n for s, n in zip(seqs, counts)], counts, share_prefix)
         except BaseException:
             for p in taken:
@@ -179,13 +199,13 @@ class PagedCache:
         for x in lists:
             row = x[common:]
             data += row + [0] * (width - len(row))
-        data += [m - held for m in lens] + [m - n - held for m, n in zip(lens, counts)]
+        data += [m - held for m in lens] + [m - n - held for m, n in zip(lens, counts)] + [m - n for m, n in zip(lens, counts)]
         at = [0]
         for n in counts:
             at.append(at[-1] + n)
         up = torch.tensor(data + at, dtype=torch.int32).to(self.k.device)
-        prefix, length, table, kv_len, start, cu = up.split([common, 1, B * width, B, B, B + 1])
-        return PagedBatch(table.view(B, width), kv_len, start, cu, prefix if common else None, length if common else None, counts)
+        prefix, length, table, kv_len, start, past, cu = up.split([common, 1, B * width, B, B, B, B + 1])
+        return PagedBatch(table.view(B, width), kv_len, start, past, cu, prefix if common else None, length if common else None, counts)
 
     def store(self, layer, k, v, batch) -> None:
         """Rows k, v [new tokens of the batch, kv_heads, head_dim], sequence after sequence, to their places.  Inference only, as `attend`: rows
@@ -194,13 +214,48 @@ class PagedCache:
             raise ValueError("as many rows as the batch has new tokens")
         if not k.shape[0]:
             return
-        capi.kv_store(k, v, self.k[layer], self.v[layer], batch.page_table, batch.cu, batch.start)
+        capi.kv_store(k, v, self.k[layer], self.v[layer], batch.page_table, batch.cu, batch.start, *self._scales(layer))
+
+    def _scales(self, layer=slice(None)):
+        """What the calls take behind their other arguments: the scales of one layer or all, nothing with bf16."""
+        return () if self.k_scale is None else (self.k_scale[layer], self.v_scale[layer])
+
+    def held(self, seqs) -> PagedBatch:
+        """All that the sequences hold, as `load` and `attend_rows` take it: every token counts as new, from place 0 on."""
+        seqs = list(seqs)
+        if not seqs or len(set(seqs)) < len(seqs):
+            raise ValueError("different sequences")
+        lens = [self._len[s] for s in seqs]
+        return self._batch([self._pages[s] for s in seqs], lens, lens, False)
+
+    def load(self, layer, held):
+        """k, v: bf16 [tokens of `held`, kv_heads, head_dim], sequence after sequence."""
+        rows = sum(held.counts)
+        if not rows:
+            return (torch.empty((0, self.k.shape[2], self.k.shape[4]), dtype=torch.bfloat16, device=self.k.device) for _ in range(2))
+        return capi.kv_load(self.k[layer], self.v[layer], held.page_table, held.cu, held.start, rows, *self._scales(layer))
+
+    def attend_rows(self, layer, q, batch, held, scale=None):
+        """Attention of the batch's new tokens, q [rows, H, head_dim], any number of them of a sequence (stored before), to all that their
+        sequences hold: the cache is read back into packed rows and functional.sdpa_packed attends to those.  `held`: self.held of the
+        batch's sequences, in its order, made after the batch.  Inference only, as `attend`."""
+        if q.shape[0] != sum(batch.counts):
+            raise ValueError("as many rows as the batch has new tokens")
+        if len(held.counts) != len(batch.counts) or any(n > m for n, m in zip(batch.counts, held.counts)):
+            raise ValueError("`held` is of other sequences than the batch")
+        if torch.is_grad_enabled() and q.requires_grad:
+            raise RuntimeError("attention to the cache has no backward and q requires a gradient: call it under torch.no_grad()")
+        if not q.shape[0]:
+            return torch.empty_like(q)
+        k, v = self.load(layer, held)
+        return functional.sdpa_packed(q, k, v, batch.cu, held.cu, is_causal=True, scale=scale)
 
     def attend(self, layer, q, batch, scale=None):
         """functional.sdpa_paged of q [B, H, N, head_dim], the batch's N new tokens of each sequence (stored before)."""
         if any(n != q.shape[2] for n in batch.counts):
             raise ValueError("q holds the batch's new tokens, the same number of every sequence")
-        return functional.sdpa_paged(q, self.k[layer], self.v[layer], batch.page_table, batch.kv_len, batch.prefix_table, batch.prefix_len, scale)
+        return functional.sdpa_paged(q, self.k[layer], self.v[layer], batch.page_table, batch.kv_len, batch.prefix_table, batch.prefix_len, scale,
+                                     *self._scales(layer))
 
     # ------------------------------------------------------------------------------------------------ compaction
     def compact(self) -> int:
@@ -210,7 +265,7 @@ class PagedCache:
         src = [p for p in range(held, len(self._users)) if self._users[p]]
         dst = [p for p in range(held) if not self._users[p]]
         if src:
-            capi.kv_copy_pages(self.k, self.v, src, dst)
+            capi.kv_copy_pages(self.k, self.v, src, dst, *self._scales())
             to = dict(zip(src, dst))
             for p, q in to.items():
                 self._users[q], self._users[p] = self._users[p], 0

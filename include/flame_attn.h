@@ -321,6 +321,69 @@ int flame_kv_copy_pages_bf16(void* K_cache, void* V_cache, int layers, int n_pag
                              void* stream);
 
 /* ------------------------------------------------------------------------------------------------
+ * The paged cache in 8 bits.  No counterpart in the reference.
+ *   - K_cache, V_cache: bytes [n_pages, H_kv, page, D] through four strides, multiples of 16 (the last 1), bases on 16 bytes; cache_dtype
+ *     FLAME_ATTN_DTYPE_I8 (whole numbers from -127 to 127) or FLAME_ATTN_DTYPE_E4M3 (largest value 448).  D a multiple of 16 up to 128.
+ *   - K_scale, V_scale: fp32 [n_pages, H_kv, page / block] through three strides of any kind: a code stands for code * scale, the scale
+ *     that of its block of `block` tokens and its head.  block: a power of two up to 128 and to the page.
+ *   - The store decides a block's scale from the largest magnitude a of the rows it brings to it (Q: the largest code).  From the block's first
+ *     token on: a / Q, rounded up to four significant bits, at least 2^-100.  Behind older tokens: the scale that is there times the least power
+ *     of two, 1 or more, with which a fits, and the older codes are divided by that power and rounded.  A number x becomes x / scale rounded
+ *     to the nearest code, the even one of two.  Infinities and NaN, and a block whose beginning was not stored by such a call, make the scale
+ *     NaN, and with it every answer that attends to the block, until its first token is stored again.
+ *   - Everything else, page tables, lengths, workspaces (flame_attn_paged_workspace_bytes), is as above.
+ * ---------------------------------------------------------------------------------------------- */
+int flame_attn_paged_fwd_q8(const void* Q, const void* K_cache, const void* V_cache, int cache_dtype, const float* K_scale,
+                            const float* V_scale, int block, void* O, void* LSE, const int32_t* page_table, int64_t table_stride,
+                            int table_pages, const int32_t* kv_len, const int32_t* prefix_table, int prefix_pages,
+                            const int32_t* prefix_len, int B, int H, int H_kv, int N, int D, int n_pages, int page, float scale,
+                            const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides, const int64_t* ks_strides,
+                            const int64_t* vs_strides, const int64_t* o_strides, void* workspace, size_t workspace_bytes,
+                            void* stream);
+
+/* As flame_kv_store_bf16, into codes and scales: rows K, V are bf16.  Two rows for one place, or two sequences that write to one block, leave
+ * the block with numbers of no use.  K_scale and V_scale are different tensors.  At most 2^30 - 1 times block and head of K or V,
+ * counted as T / block + 2 n_seqs blocks (block = 1: T). */
+int flame_kv_store_q8(const void* K, const void* V, void* K_cache, void* V_cache, int cache_dtype, float* K_scale, float* V_scale,
+                      int block, const int32_t* page_table, int64_t table_stride, int table_pages, const int32_t* cu,
+                      const int32_t* start, int n_seqs, int T, int H_kv, int D, int n_pages, int page, const int64_t* k_strides,
+                      const int64_t* v_strides, const int64_t* kc_strides, const int64_t* vc_strides, const int64_t* ks_strides,
+                      const int64_t* vs_strides, void* stream);
+
+/* The way back: row cu[b] + i of K and V [T, H_kv, D], bf16, is what place start[b] + i of sequence b holds (code * scale, rounded once).
+ * cache_dtype FLAME_ATTN_DTYPE_BF16 reads a bf16 cache (no scales, their strides and `block` unused, D any multiple of 8).  Rows behind the last
+ * sequence become zeros, rows whose place lies outside the sequence's pages or on a page outside the cache NaN.  K and V are different
+ * tensors.  Rows as many as flame_kv_store_bf16 takes. */
+int flame_kv_load(const void* K_cache, const void* V_cache, int cache_dtype, const float* K_scale, const float* V_scale, int block,
+                  void* K, void* V, const int32_t* page_table, int64_t table_stride, int table_pages, const int32_t* cu,
+                  const int32_t* start, int n_seqs, int T, int H_kv, int D, int n_pages, int page, const int64_t* kc_strides,
+                  const int64_t* vc_strides, const int64_t* ks_strides, const int64_t* vs_strides, const int64_t* k_strides,
+                  const int64_t* v_strides, void* stream);
+
+/* As flame_kv_copy_pages_bf16, with the scales (four element strides: layer, page, head, block). */
+int flame_kv_copy_pages_q8(void* K_cache, void* V_cache, float* K_scale, float* V_scale, int layers, int n_pages, int H_kv, int page,
+                           int D, int block, const int64_t* k_strides, const int64_t* v_strides, const int64_t* ks_strides,
+                           const int64_t* vs_strides, const int32_t* src, const int32_t* dst, int n, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Rotary positions.  Pairs of the first rotary_dim elements of a head, (2 i, 2 i + 1) with `interleaved`, else (i, i + rotary_dim / 2), are
+ * turned by the angle position * f_i, (a, b) -> size (a cos - b sin, b cos + a sin); the others are copied.  The reference turns whole heads,
+ * neighbours in pairs, by tables of positions in a row (src/bf16_ops.rs:361-394).
+ *   - Q [B,H,S,D] and, with it or not (null, 0 heads), K [B,H_kv,S,D] through four ELEMENT strides in (B, H, S, D) order, the last 1;
+ *     dtype FLAME_ATTN_DTYPE_BF16, _F16 or _F32.  Any D, any even rotary_dim up to it, any alignment: 16-byte rows and halves of whole 16 bytes are
+ *     faster.  Q_out and K_out may be Q and K with the same strides.
+ *   - turns [rotary_dim / 2] on the device: f_i / (2 pi) * 2^64, rounded, f_i in radians per position.  The angle is exact for any int32 position.
+ *   - positions: int32, row b position_stride elements behind the one before (0: one row for all), S entries.  Or null, and B = 1: row r of sequence i,
+ *     cu[i] <= r < cu[i + 1] (int32 [n_seqs + 1], rising from 0), is at position start[i] + r - cu[i] (start null: 0); rows behind the
+ *     last sequence become zeros.
+ *   - inverse: the turns go backwards, which with the same size is the gradient.
+ * ---------------------------------------------------------------------------------------------- */
+int flame_rotary(const void* Q, void* Q_out, int H, const int64_t* q_strides, const int64_t* qo_strides, const void* K, void* K_out,
+                 int H_kv, const int64_t* k_strides, const int64_t* ko_strides, int dtype, const int64_t* turns, int rotary_dim,
+                 int interleaved, float size, int inverse, const int32_t* positions, int64_t position_stride, const int32_t* cu,
+                 const int32_t* start, int n_seqs, int B, int S, int D, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
  * The materialised path: every shape the fused kernels refuse.  Any head dim D >= 1 (no multiple-of-8 rule, no
  * upper limit, D stride 1 and non-negative strides as the only layout rules), a value head dim Dv of its own,
  * causal flag, key lengths, keep-mask and (forward) additive bias as in the primary entry points, and the
@@ -572,7 +635,7 @@ int flame_attn_profiling_read(FlameAttnKernelTimes* out);
 /* ------------------------------------------------------------------------------------------------
  * Small conversions the host layer needs at the boundary.
  * ---------------------------------------------------------------------------------------------- */
-enum { FLAME_ATTN_DTYPE_BF16 = 0, FLAME_ATTN_DTYPE_F32 = 1 };
+enum { FLAME_ATTN_DTYPE_BF16 = 0, FLAME_ATTN_DTYPE_F32 = 1, FLAME_ATTN_DTYPE_F16 = 2, FLAME_ATTN_DTYPE_I8 = 3, FLAME_ATTN_DTYPE_E4M3 = 4 };
 /* Binary keep-mask in bf16 / fp32 (>= 0.5 attends; the public mask convention of the reference,
  * src/sdpa.rs:458-470) -> contiguous uint8 keep-mask of n elements. */
 int flame_attn_convert_keep_mask(const void* src, int src_dtype, void* dst_u8, int64_t n, void* stream);

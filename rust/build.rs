@@ -46,7 +46,7 @@ fn main() {
         .unwrap_or_else(|| "?".to_string());
 
     let mut objects = Vec::new();
-    for name in ["flame_attn", "flame_packed", "flame_paged"] {
+    for name in ["flame_attn", "flame_packed", "flame_paged", "flame_paged8", "flame_rotary"] {
         let obj = out.join(format!("{name}.o"));
         let mut cc = Command::new(&hipcc);
         cc.args(["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC"])

@@ -209,6 +209,43 @@ extern "C" {
         d: c_int, k_strides: *const i64, v_strides: *const i64, src: *const i32, dst: *const i32, n: c_int,
         stream: *mut c_void
     ) -> c_int;
+    pub fn flame_attn_paged_fwd_q8(
+        q: *const c_void, k_cache: *const c_void, v_cache: *const c_void, cache_dtype: c_int, k_scale: *const f32,
+        v_scale: *const f32, block: c_int, o: *mut c_void, lse: *mut c_void, page_table: *const i32,
+        table_stride: i64, table_pages: c_int, kv_len: *const i32, prefix_table: *const i32, prefix_pages: c_int,
+        prefix_len: *const i32, b: c_int, h: c_int, h_kv: c_int, n: c_int, d: c_int, n_pages: c_int, page: c_int,
+        scale: f32, q_strides: *const i64, k_strides: *const i64, v_strides: *const i64, ks_strides: *const i64,
+        vs_strides: *const i64, o_strides: *const i64, workspace: *mut c_void, workspace_bytes: usize,
+        stream: *mut c_void
+    ) -> c_int;
+    pub fn flame_kv_store_q8(
+        k: *const c_void, v: *const c_void, k_cache: *mut c_void, v_cache: *mut c_void, cache_dtype: c_int,
+        k_scale: *mut f32, v_scale: *mut f32, block: c_int, page_table: *const i32, table_stride: i64,
+        table_pages: c_int, cu: *const i32, start: *const i32, n_seqs: c_int, t: c_int, h_kv: c_int, d: c_int,
+        n_pages: c_int, page: c_int, k_strides: *const i64, v_strides: *const i64, kc_strides: *const i64,
+        vc_strides: *const i64, ks_strides: *const i64, vs_strides: *const i64, stream: *mut c_void
+    ) -> c_int;
+    pub fn flame_kv_load(
+        k_cache: *const c_void, v_cache: *const c_void, cache_dtype: c_int, k_scale: *const f32,
+        v_scale: *const f32, block: c_int, k: *mut c_void, v: *mut c_void, page_table: *const i32,
+        table_stride: i64, table_pages: c_int, cu: *const i32, start: *const i32, n_seqs: c_int, t: c_int,
+        h_kv: c_int, d: c_int, n_pages: c_int, page: c_int, kc_strides: *const i64, vc_strides: *const i64,
+        ks_strides: *const i64, vs_strides: *const i64, k_strides: *const i64, v_strides: *const i64,
+        stream: *mut c_void
+    ) -> c_int;
+    pub fn flame_kv_copy_pages_q8(
+        k_cache: *mut c_void, v_cache: *mut c_void, k_scale: *mut f32, v_scale: *mut f32, layers: c_int,
+        n_pages: c_int, h_kv: c_int, page: c_int, d: c_int, block: c_int, k_strides: *const i64,
+        v_strides: *const i64, ks_strides: *const i64, vs_strides: *const i64, src: *const i32, dst: *const i32,
+        n: c_int, stream: *mut c_void
+    ) -> c_int;
+    pub fn flame_rotary(
+        q: *const c_void, q_out: *mut c_void, h: c_int, q_strides: *const i64, qo_strides: *const i64,
+        k: *const c_void, k_out: *mut c_void, h_kv: c_int, k_strides: *const i64, ko_strides: *const i64,
+        dtype: c_int, turns: *const i64, rotary_dim: c_int, interleaved: c_int, size: f32, inverse: c_int,
+        positions: *const i32, position_stride: i64, cu: *const i32, start: *const i32, n_seqs: c_int, b: c_int,
+        s: c_int, d: c_int, stream: *mut c_void
+    ) -> c_int;
     pub fn flame_attn_materialised_workspace_bytes(
         b: c_int, h: c_int, n_q: c_int, n_kv: c_int, d: c_int, dv: c_int, backward: c_int
     ) -> usize;
