@@ -5,19 +5,21 @@
 // numbers out of codes and scales would take one for every element and a rounding.  The codes become bf16 (exactly) on their way from LDS to the
 // matrix instructions: a value's column comes through the transposing read of 8 bits, eight tokens at a time, in the order of the weights.
 //
-// The way of units, plan and merge is that of the bf16 cache.  A wavefront has two tiles of K, V and scales in LDS, as many bytes as one of bf16,
-// and requests a tile two steps ahead.
+// The way of units, plan and merge is that of the bf16 cache.  With half the bytes a tile's arithmetic weighs twice as much, so rows come in blocks of 16
+// (v_mfma_f32_16x16x32_bf16), one block where a sequence has no more rows than that: half of the exponentials and of what goes with them.  A
+// wavefront has two tiles of K, V and scales in LDS and requests a tile two steps ahead.
 #pragma once
 #include "attn_paged.hpp"
 #include "kv_codes.hpp"
 
 namespace fattn {
 
-template <int CODE>
+// R: blocks of 16 rows that a unit of own keys has, 1 or 2.
+template <int CODE, int R>
 struct Paged8Params : PagedParams {        // k, v unused; ks, vs in bytes
     const uint8_t* k8;
     const uint8_t* v8;
-    const float* k_scale;          // [pages][Hkv][page / block] through kss, vss (b: page, h: head, n: block)
+    const float* k_scale;          // [pages][Hkv][page / block] through kss, vss (b: page, h: head, n: block; bytes, b and n below 2^31)
     const float* v_scale;
     Strides kss, vss;
     int block_shift;               // log2 of the tokens that share a scale
@@ -28,21 +30,19 @@ struct Paged8Tile {
     static_assert(D == 64 || D == 128, "rows of 64 or 128 bytes");
     static constexpr int BN = 32, RB = D;                          // keys, bytes of a row
     static constexpr int TILE = BN * RB, SCALES = 2 * BN * 4;      // bytes: of K or V, of both scales
-    static constexpr int STAGE = 2 * TILE + SCALES;
+    static constexpr int V = TILE, S = 2 * TILE, STAGE = 2 * TILE + SCALES;
     static constexpr int WAVE = 2 * STAGE;
     static_assert(WAVE >= 32 * D * 4, "the 32 x D fp32 sums at the end");
     static constexpr int NDMA = TILE / 1024, RPD = 1024 / RB, GPR = RB / 16;       // copies per tile, rows per copy, granules per row
     static constexpr int lds_bytes(int nw) { return nw * WAVE; }
-    // Swizzle of the 16-byte granules of a row.  Free of bank conflicts: 16-byte reads of one granule of 16 rows one behind the other, and the transposing
-    // reads, whose half wavefront takes two neighbouring granules of rows 4 h .. 4 h + 3 and 8 + 4 h .. 8 + 4 h + 3.  Rows 16 apart have the same.
+    // Swizzle of the 16-byte granules of a row.  Free of bank conflicts: 16-byte reads of one granule of the 16 rows of either half, and the transposing
+    // reads, whose half wavefront takes one granule of rows 8 x .. 8 x + 7 and 16 + 8 x .. 16 + 8 x + 7.
     static __device__ __forceinline__ constexpr int swz(int row) {
-        if (RB == 64) return (row >> 2) & 3;
-        const int pair = row >> 1;
-        return (pair & 4) | ((pair & 1) << 1) | ((pair >> 1) & 1);
+        return RB == 64 ? ((row >> 2) & 3) ^ ((row >> 4) << 1) : ((row >> 1) & 3) | ((((row >> 3) ^ (row >> 4)) & 1) << 2);
     }
 };
-template <int D, int CODE>
-constexpr int paged_lds_bytes(const Paged8Params<CODE>*, int nw) { return Paged8Tile<D>::lds_bytes(nw); }
+template <int D, int CODE, int R>
+constexpr int paged_lds_bytes(const Paged8Params<CODE, R>*, int nw) { return Paged8Tile<D>::lds_bytes(nw); }
 
 // ds_read_b64_tr_b8: a group of 16 lanes reads 8 rows of 16 bytes, lane r the half r % 2 of row r / 2; lane i receives byte i of each row.
 __device__ __forceinline__ u32x2 lds_read_tr8(const uint8_t* p) {
@@ -50,39 +50,52 @@ __device__ __forceinline__ u32x2 lds_read_tr8(const uint8_t* p) {
     typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
     return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2*)(p)));
 }
+// v_mfma_f32_16x16x32_bf16: lane l, g = l / 16, n = l % 16: A[n][8 g .. 8 g + 7], B[8 g .. 8 g + 7][n], D[4 g + r][n]
+__device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 
 // Copies of a tile (NDMA of 1 KiB) and of its scales to LDS.  Rows past the last key (`most` of the tile) re-read it.
-template <int D, int CODE>
+template <int D, class P>
 struct Paged8Copy {
     using T = Paged8Tile<D>;
     static constexpr int EACH = T::NDMA / 2;           // per 16 rows, which lie in one page
-    const Paged8Params<CODE>& p;
+    const P& p;
     const PagedUnit& u;
     PagedPages& pages;
-    int lane;
-    uint32_t k_off[EACH], v_off[EACH];                 // bytes of this lane within 16 rows
+    const int lane;
+    const uint8_t* const k_base;
+    const uint8_t* const v_base;
+    uint32_t k_off[T::NDMA], v_off[T::NDMA];           // bytes of this lane within 16 rows
+    const char* s_base;                                // lanes 0 .. 31: K's scales, 32 .. 63: V's
+    int s_page, s_block;                               // bytes from page to page, from block to block
+    int key0, most, e0, e1;                            // of the tile that is aimed at: first key, last key of it, the pages of its halves
 
-    __device__ __forceinline__ Paged8Copy(const Paged8Params<CODE>& p, const PagedUnit& u, PagedPages& pages, int lane) : p(p), u(u), pages(pages), lane(lane) {
+    __device__ __forceinline__ Paged8Copy(const P& p, const PagedUnit& u, PagedPages& pages, int lane)
+        : p(p), u(u), pages(pages), lane(lane), k_base(p.k8 + u.kv_head * p.ks.h), v_base(p.v8 + u.kv_head * p.vs.h) {
 #pragma unroll
-        for (int j = 0; j < EACH; ++j) {
-            const int row = j * T::RPD + lane / T::GPR, g = lane % T::GPR ^ T::swz(row), from = 16 * g < p.d ? 16 * g : 0;
-            k_off[j] = (uint32_t)(row * (int)p.ks.n + from);
-            v_off[j] = (uint32_t)(row * (int)p.vs.n + from);
+        for (int i = 0; i < T::NDMA; ++i) {
+            const int row = i % EACH * T::RPD + lane / T::GPR, g = lane % T::GPR ^ T::swz(row + 16 * (i / EACH)), from = 16 * g < p.d ? 16 * g : 0;
+            k_off[i] = (uint32_t)(row * (int)p.ks.n + from);
+            v_off[i] = (uint32_t)(row * (int)p.vs.n + from);
         }
+        s_base = lane < 32 ? reinterpret_cast<const char*>(p.k_scale) + u.kv_head * p.kss.h : reinterpret_cast<const char*>(p.v_scale) + u.kv_head * p.vss.h;
+        s_page = (int)(lane < 32 ? p.kss.b : p.vss.b);
+        s_block = (int)(lane < 32 ? p.kss.n : p.vss.n);
     }
-    // the pages that tile t needs are there
-    __device__ __forceinline__ void find(int t) {
-        if (!pages.holds(p, (t + 1) * T::BN - 1)) pages.load(p, u, lane, (t * T::BN) >> p.page_shift);
+    __device__ __forceinline__ void aim(int t) {
+        key0 = t * T::BN;
+        most = u.keys - 1 - key0;
+        if (!pages.holds(p, key0 + T::BN - 1)) pages.load(p, u, lane, key0 >> p.page_shift);
+        e0 = __builtin_amdgcn_readlane(pages.mine, (key0 >> p.page_shift) - pages.first);
+        e1 = most >= 16 ? __builtin_amdgcn_readlane(pages.mine, ((key0 + 16) >> p.page_shift) - pages.first) : e0;
     }
-    __device__ __forceinline__ void tile(const uint8_t* base, const Strides& st, const uint32_t (&off)[EACH], int t, uint32_t dst) const {
-        const int key0 = t * T::BN, most = u.keys - 1 - key0;
+    __device__ __forceinline__ void tile(const uint8_t* base, const Strides& st, const uint32_t (&off)[T::NDMA], uint32_t dst) const {
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             const int from = 16 * half <= most ? half : 0;         // a half without a key: the last key is in the other one
-            const uint8_t* const rows = base + pages.rows16(p, key0 + 16 * from, st);
+            const uint8_t* const rows = base + (half ? e1 : e0) * st.b + ((key0 + 16 * from) & ((1 << p.page_shift) - 1)) * st.n;
 #pragma unroll
             for (int j = 0; j < EACH; ++j) {
-                uint32_t o = off[j];
+                uint32_t o = off[half * EACH + j];
                 if (16 * half + 15 > most) {
                     const int row = j * T::RPD + lane / T::GPR;
                     o += (uint32_t)((min(16 * half + row, most) - 16 * from - row) * (int)st.n);
@@ -91,205 +104,327 @@ struct Paged8Copy {
             }
         }
     }
-    __device__ __forceinline__ void k(int t, uint32_t dst) const { tile(p.k8 + u.kv_head * p.ks.h, p.ks, k_off, t, dst); }
-    __device__ __forceinline__ void v(int t, uint32_t dst) const { tile(p.v8 + u.kv_head * p.vs.h, p.vs, v_off, t, dst); }
-    // lanes 0 .. 31: K, 32 .. 63: V
-    __device__ __forceinline__ void scales(int t, uint32_t dst) const {
-        const int key0 = t * T::BN, most = u.keys - 1 - key0, at = min(lane & 31, most), token = (key0 + at) & ((1 << p.page_shift) - 1);
-        const int e0 = __builtin_amdgcn_readlane(pages.mine, (key0 >> p.page_shift) - pages.first);
-        const int e1 = most >= 16 ? __builtin_amdgcn_readlane(pages.mine, ((key0 + 16) >> p.page_shift) - pages.first) : e0;
-        const int64_t k0 = e0 * p.kss.b + u.kv_head * p.kss.h, k1 = e1 * p.kss.b + u.kv_head * p.kss.h;
-        const int64_t v0 = e0 * p.vss.b + u.kv_head * p.vss.h, v1 = e1 * p.vss.b + u.kv_head * p.vss.h;
-        const float* const from = lane < 32 ? p.k_scale + (at < 16 ? k0 : k1) : p.v_scale + (at < 16 ? v0 : v1);
-        dma4(from + (token >> p.block_shift) * (int)(lane < 32 ? p.kss.n : p.vss.n), dst);
+    __device__ __forceinline__ void k(uint32_t dst) const { tile(k_base, p.ks, k_off, dst); }
+    __device__ __forceinline__ void v(uint32_t dst) const { tile(v_base, p.vs, v_off, dst); }
+    __device__ __forceinline__ void scales(uint32_t dst) const {
+        const int at = min(lane & 31, most), token = (key0 + at) & ((1 << p.page_shift) - 1), e = at < 16 ? e0 : e1;
+        dma4(s_base + (int64_t)e * s_page + (int64_t)(token >> p.block_shift) * s_block, dst);
     }
 };
 
-template <int D, int CODE>
-struct Paged8Rows : PagedRows<D> {
+// What a wavefront holds of 16 R rows: their queries as MFMA fragments and the running softmax over the keys it has seen.  Lane (n, g): row n of
+// every block; of a tile the keys 16 k + 4 g .. + 3, k = 0, 1, which are the contraction's steps of the second product in this order.
+template <int D, int CODE, int R>
+struct Paged8Rows {
     using T = Paged8Tile<D>;
-    using PagedRows<D>::qf;
-    static constexpr int DC = D / 16, DB = D / 32;
-    int k_at[DB];              // K: row n, granule 2 c + h, which are the contraction's steps 2 c and 2 c + 1
-    int v_at;                  // V: rows 4 h + 0 .. 3, 8 + 4 h + 0 .. 3
-    int v_granule[DB];         // (swizzled)
+    static constexpr int DC = D / 64, DB = D / 16;
+    bf16x8 qf[R][2 * DC];
+    f32x4 oacc[R][DB];
+    float m_run[R], l_run[R], c_log2, stale_ok;
+    int k_at[2][DC];           // K: row 16 k + n, granule 4 c + g, which are the contraction's steps 2 c and 2 c + 1
+    int v_at[DB];              // V: rows 4 g + 0 .. 3, 16 + 4 g + 0 .. 3, granule db
+    int s_at;
 
-    __device__ __forceinline__ void begin(const PagedParams& p, int lane, const PagedRow& at, bool there) {
-        const int n = lane & 31, h = lane >> 5, r = (lane & 15) >> 1, row = 4 * h + (r & 3) + 8 * (r >> 2);
-        const uint16_t* const qrow = p.q + at.b * p.qs.b + at.h * p.qs.h + at.i * p.qs.n;
+    __device__ __forceinline__ void begin(const PagedParams& p, const PagedUnit& u, int lane, int row0) {
+        const int n = lane & 15, g = lane >> 4, j = n >> 1, row = 4 * g + (j & 3) + 16 * (j >> 2);
 #pragma unroll
-        for (int dc = 0; dc < DC; ++dc) {
-            const int d0 = 32 * (dc >> 1) + 16 * h + 8 * (dc & 1);
-            qf[dc] = __builtin_bit_cast(bf16x8, ldg16(qrow + d0, there && d0 < p.d));
-        }
-        v_at = row * T::RB + 8 * (lane & 1);
+        for (int b = 0; b < R; ++b) {
+            const int r = row0 + 16 * b + n;
+            const PagedRow at = paged_row(p, u, min(r, u.rows - 1));
+            const uint16_t* const qrow = p.q + at.b * p.qs.b + at.h * p.qs.h + at.i * p.qs.n;
 #pragma unroll
-        for (int c = 0; c < DB; ++c) {
-            k_at[c] = n * T::RB + (((2 * c + h) ^ T::swz(n)) << 4);
-            v_granule[c] = ((2 * c + ((lane >> 4) & 1)) ^ T::swz(row)) << 4;
-        }
-        this->c_log2 = p.scale * kLog2e;
-        this->stale_ok = stale_scope(this->c_log2);
+            for (int dc = 0; dc < 2 * DC; ++dc) {
+                const int d0 = 64 * (dc >> 1) + 16 * g + 8 * (dc & 1);
+                qf[b][dc] = __builtin_bit_cast(bf16x8, ldg16(qrow + d0, r < u.rows && d0 < p.d));
+            }
 #pragma unroll
-        for (int db = 0; db < DB; ++db)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) this->oacc[db][i] = 0.f;
-    }
-    __device__ __forceinline__ void read_k(u32x4 (&k)[DB], const uint8_t* tile) const {
-#pragma unroll
-        for (int c = 0; c < DB; ++c) k[c] = *reinterpret_cast<const u32x4*>(tile + k_at[c]);
-    }
-    __device__ __forceinline__ void read_v(u32x2 (&v)[2 * DB], const uint8_t* tile) const {
-#pragma unroll
-        for (int i = 0; i < 2 * DB; ++i) v[i] = lds_read_tr8(tile + v_at + v_granule[i % DB] + 16 * (i / DB) * T::RB);
-    }
-    // of the keys 8 g + 4 h .. + 3, the rows that this lane's scores and weights are of
-    static __device__ __forceinline__ void read_scales(f32x4 (&s)[4], const float* scales, int lane) {
-#pragma unroll
-        for (int g = 0; g < 4; ++g) s[g] = *reinterpret_cast<const f32x4*>(scales + 8 * g + 4 * (lane >> 5));
-    }
-    __device__ __forceinline__ f32x16 scores(const u32x4 (&k)[DB], const f32x4 (&scale)[4]) const {
-        f32x16 s;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = 0.f;
-#pragma unroll
-        for (int c = 0; c < DB; ++c) {
-            s = mfma32(codes_to_bf16<CODE>(k[c][0], k[c][1]), qf[2 * c], s);
-            s = mfma32(codes_to_bf16<CODE>(k[c][2], k[c][3]), qf[2 * c + 1], s);
+            for (int db = 0; db < DB; ++db) oacc[b][db] = f32x4{0.f, 0.f, 0.f, 0.f};
+            m_run[b] = -INFINITY;
+            l_run[b] = 0.f;
         }
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] *= scale[r >> 2][r & 3];
-        return s;
-    }
-    // as PagedRows::weights; what meets V is the weight times V's scale, rounded to bf16
-    __device__ __forceinline__ void weights(f32x16& s, const f32x4 (&scale)[4], bf16x8 (&pf)[2]) {
-        const float shift = (this->m_run == -INFINITY ? 0.f : this->m_run) * this->c_log2;
-        float sum[2] = {0.f, 0.f};
+        for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            s[r] = exp2_fast(fmaf(s[r], this->c_log2, -shift));
-            sum[r & 1] += s[r];
-            s[r] *= scale[r >> 2][r & 3];
+            for (int c = 0; c < DC; ++c) k_at[k][c] = (16 * k + n) * T::RB + (((4 * c + g) ^ T::swz(16 * k + n)) << 4);
+#pragma unroll
+        for (int db = 0; db < DB; ++db) v_at[db] = T::V + row * T::RB + ((db ^ T::swz(row)) << 4) + 8 * (lane & 1);
+        s_at = T::S + 16 * g;
+        c_log2 = p.scale * kLog2e;
+        stale_ok = stale_scope(c_log2);        // the reference maximum may lag the true one by 2^8
+    }
+    // (stage: bytes of the tile's stage)
+    __device__ __forceinline__ void read_k(u32x4 (&k)[2][DC], const uint8_t* mine, int stage) const {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int c = 0; c < DC; ++c) k[i][c] = *reinterpret_cast<const u32x4*>(mine + stage + k_at[i][c]);
+    }
+    __device__ __forceinline__ void read_v(u32x2 (&v)[DB], const uint8_t* mine, int stage) const {
+#pragma unroll
+        for (int db = 0; db < DB; ++db) v[db] = lds_read_tr8(mine + stage + v_at[db]);
+    }
+    __device__ __forceinline__ void read_scales(f32x4 (&s)[2], const uint8_t* mine, int stage) const {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) s[k] = *reinterpret_cast<const f32x4*>(mine + stage + s_at + 64 * k);
+    }
+    __device__ __forceinline__ void scores(f32x4 (&s)[R][2], const u32x4 (&k)[2][DC], const f32x4 (&scale)[2]) const {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+            for (int b = 0; b < R; ++b) s[b][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < DC; ++c) {
+                const bf16x8 lo = codes_to_bf16<CODE>(k[i][c][0], k[i][c][1]), hi = codes_to_bf16<CODE>(k[i][c][2], k[i][c][3]);
+#pragma unroll
+                for (int b = 0; b < R; ++b) {
+                    s[b][i] = mfma16(lo, qf[b][2 * c], s[b][i]);
+                    s[b][i] = mfma16(hi, qf[b][2 * c + 1], s[b][i]);
+                }
+            }
+#pragma unroll
+            for (int b = 0; b < R; ++b) s[b][i] *= scale[i];
         }
-        this->l_run += sum[0] + sum[1];
-        pf[0] = pack8(s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7]);
-        pf[1] = pack8(s[8], s[9], s[10], s[11], s[12], s[13], s[14], s[15]);
     }
-    __device__ __forceinline__ void add(const u32x2 (&v)[2 * DB], const bf16x8 (&pf)[2]) {
+    // keys of the tile from `limit` (of block b) on are excluded
+    __device__ __forceinline__ static void exclude(f32x4 (&s)[2], int lane, int limit) {
+        const int lim = limit - 4 * (lane >> 4);
 #pragma unroll
-        for (int i = 0; i < 2 * DB; ++i) this->oacc[i % DB] = mfma32(codes_to_bf16<CODE>(v[i][0], v[i][1]), pf[i / DB], this->oacc[i % DB]);
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[k][r] = 16 * k + r >= lim ? -INFINITY : s[k][r];
+    }
+    static __device__ __forceinline__ float over_groups_max(float x) {
+        x = fmaxf(x, __shfl_xor(x, 16, 64));
+        return max_of_halves(x);
+    }
+    static __device__ __forceinline__ float over_groups_sum(float x) {
+        x += __shfl_xor(x, 16, 64);
+        return x + xhalf(x);
+    }
+    // the maximum of a tile's scores joins the running one, which moves (and the sums are rescaled) only when it lags by more than 2^8
+    __device__ __forceinline__ void fold(const f32x4 (&s)[R][2]) {
+        float top[R];
+        bool behind = false;
+#pragma unroll
+        for (int b = 0; b < R; ++b) {
+            top[b] = s[b][0][0];
+#pragma unroll
+            for (int r = 1; r < 8; ++r) top[b] = fmaxf(top[b], s[b][r >> 2][r & 3]);
+            behind |= top[b] > m_run[b] + stale_ok;
+        }
+        if (__any(behind)) {
+#pragma unroll
+            for (int b = 0; b < R; ++b) {
+                const float m_new = fmaxf(m_run[b], over_groups_max(top[b])), m_to = m_new == -INFINITY ? 0.f : m_new;
+                const float alpha = exp2_fast((m_run[b] - m_to) * c_log2);
+                m_run[b] = m_new;
+                l_run[b] *= alpha;
+#pragma unroll
+                for (int db = 0; db < DB; ++db) oacc[b][db] *= alpha;
+            }
+        }
+    }
+    // exp2 of the scores against the running maximum.  What meets V is the weight times V's scale, rounded to bf16 (the sum l is of the unrounded
+    // weights): the matrix instructions take no wider operand
+    __device__ __forceinline__ void weights(f32x4 (&s)[R][2], const f32x4 (&scale)[2], bf16x8 (&pf)[R]) {
+#pragma unroll
+        for (int b = 0; b < R; ++b) {
+            const float shift = (m_run[b] == -INFINITY ? 0.f : m_run[b]) * c_log2;
+            float sum[2] = {0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float e = exp2_fast(fmaf(s[b][k][r], c_log2, -shift));
+                    sum[r & 1] += e;
+                    s[b][k][r] = e * scale[k][r];
+                }
+            l_run[b] += sum[0] + sum[1];
+            pf[b] = pack8(s[b][0][0], s[b][0][1], s[b][0][2], s[b][0][3], s[b][1][0], s[b][1][1], s[b][1][2], s[b][1][3]);
+        }
+    }
+    __device__ __forceinline__ void add(const u32x2 (&v)[DB], const bf16x8 (&pf)[R]) {
+#pragma unroll
+        for (int db = 0; db < DB; ++db) {
+            const bf16x8 vf = codes_to_bf16<CODE>(v[db][0], v[db][1]);
+#pragma unroll
+            for (int b = 0; b < R; ++b) oacc[b][db] = mfma16(vf, pf[b], oacc[b][db]);
+        }
     }
 };
 
-// The walk of one wavefront over the tiles t_lo, t_lo + STEP, ... below t_hi.  `mine`: its Paged8Tile::WAVE bytes of LDS; limit: this lane's row
-// attends to the keys below it, clean: every row to those below this.  Of the stage of tile t: K, V and the scales of tile t + 2 STEP follow as soon as
+// The walk of one wavefront over the tiles t_lo, t_lo + STEP, ... below t_hi.  `mine`: its Paged8Tile::WAVE bytes of LDS; limit: this lane's row of a
+// block attends to the keys below it, clean: every row to those below this.  Of the stage of tile t: K, V and the scales of tile t + 2 STEP follow as soon as
 // those of t are in registers, in the order K, scales, V, which is what the numbers of copies under way below count.
-template <int STEP, int D, int CODE>
-__device__ __forceinline__ void paged8_walk(const PagedUnit& u, Paged8Copy<D, CODE>& copy, Paged8Rows<D, CODE>& w, const uint8_t* mine, int t_lo, int t_hi,
-                                            int limit, int clean) {
+template <int STEP, int D, int CODE, int R, class P>
+__device__ __forceinline__ void paged8_walk(Paged8Copy<D, P>& copy, Paged8Rows<D, CODE, R>& w, const uint8_t* mine, int t_lo, int t_hi, const int (&limit)[R],
+                                            int clean) {
     using T = Paged8Tile<D>;
-    constexpr int DB = D / 32, N = T::NDMA;
-    int at = 0;                                        // bytes: this tile's stage
+    constexpr int N = T::NDMA;
     const uint32_t lds = lds_addr(mine);
-    for (int t = t_lo; t < t_hi; t += STEP) {
+    auto step = [&](int t, auto stage_tag) {
+        constexpr int stage = decltype(stage_tag)::value * T::STAGE;
         const bool one = t + STEP < t_hi, two = t + 2 * STEP < t_hi;
-        if (two) copy.find(t + 2 * STEP);
+        if (two) copy.aim(t + 2 * STEP);
         if (one) wait_vm<3 * N + 1>();                 // K and scales of t have landed (V of t, all of the next may be on their way)
         else wait_vm<N>();
-        u32x4 k[DB];
-        f32x4 ks[4], vs[4];
-        w.read_k(k, mine + at);
-        w.read_scales(ks, reinterpret_cast<const float*>(mine + at + 2 * T::TILE), copy.lane);
-        w.read_scales(vs, reinterpret_cast<const float*>(mine + at + 2 * T::TILE) + 32, copy.lane);
+        u32x4 k[2][D / 64];
+        f32x4 scale[2], s[R][2];
+        w.read_k(k, mine, stage);
+        w.read_scales(scale, mine, stage);
+        f32x4 v_scale[2];
+        w.read_scales(v_scale, mine, stage + 128);
         lds_reads_done();
-        if (two) copy.k(t + 2 * STEP, lds + at);
-        f32x16 s = w.scores(k, ks);
-        if ((t + 1) * T::BN > clean) w.exclude(s, copy.lane, limit - t * T::BN);
+        if (two) copy.k(lds + stage);
+        w.scores(s, k, scale);
+        if ((t + 1) * T::BN > clean) {
+#pragma unroll
+            for (int b = 0; b < R; ++b) w.exclude(s[b], copy.lane, limit[b] - t * T::BN);
+        }
         w.fold(s);
-        bf16x8 pf[2];
-        w.weights(s, vs, pf);
+        bf16x8 pf[R];
+        w.weights(s, v_scale, pf);
         if (two) wait_vm<3 * N + 1>();                 // V of t
         else if (one) wait_vm<2 * N + 1>();
         else wait_vm<0>();
-        u32x2 v[2 * DB];
-        w.read_v(v, mine + at + T::TILE);
+        u32x2 v[D / 16];
+        w.read_v(v, mine, stage);
         lds_reads_done();
         if (two) {
-            copy.scales(t + 2 * STEP, lds + at + 2 * T::TILE);
-            copy.v(t + 2 * STEP, lds + at + T::TILE);
+            copy.scales(lds + stage + T::S);
+            copy.v(lds + stage + T::V);
         }
         w.add(v, pf);
-        at = T::STAGE - at;
+    };
+    for (int t = t_lo; t < t_hi; t += 2 * STEP) {
+        step(t, std::integral_constant<int, 0>{});
+        if (t + STEP < t_hi) step(t + STEP, std::integral_constant<int, 1>{});
     }
 }
 // ... its first two tiles
-template <int STEP, int D, int CODE>
-__device__ __forceinline__ void paged8_start(Paged8Copy<D, CODE>& copy, const uint8_t* mine, int t_lo, int t_hi) {
+template <int STEP, int D, class P>
+__device__ __forceinline__ void paged8_start(Paged8Copy<D, P>& copy, const uint8_t* mine, int t_lo, int t_hi) {
     using T = Paged8Tile<D>;
     const uint32_t lds = lds_addr(mine);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        const int t = t_lo + i * STEP;
-        if (t >= t_hi) break;
-        if (i) copy.find(t);
-        copy.k(t, lds + i * T::STAGE);
-        copy.scales(t, lds + i * T::STAGE + 2 * T::TILE);
-        copy.v(t, lds + i * T::STAGE + T::TILE);
+        if (t_lo + i * STEP >= t_hi) break;
+        copy.aim(t_lo + i * STEP);
+        copy.k(lds + i * T::STAGE);
+        copy.scales(lds + i * T::STAGE + T::S);
+        copy.v(lds + i * T::STAGE + T::V);
     }
 }
+// This lane's rows of the blocks from row0 on attend to the keys below `limit`; returns below which key all rows do.
+template <int R>
+__device__ __forceinline__ int paged8_limits(const PagedParams& p, const PagedUnit& u, int lane, int row0, int (&limit)[R]) {
+#pragma unroll
+    for (int b = 0; b < R; ++b) limit[b] = u.own ? max(u.keys - u.lag + paged_row(p, u, min(row0 + 16 * b + (lane & 15), u.rows - 1)).i, 0) : u.keys;
+    return u.own ? max(u.keys - u.lag, 0) : u.keys;
+}
 
-template <int D, int NW, bool STRIDED, int CODE>
-__device__ __forceinline__ void paged_unit_body(const Paged8Params<CODE>& p, const PagedUnit& u, uint16_t* lds, bool bad, bool direct, float* out_o,
-                                                f32x2* out_ml) {
+// A unit whose wavefronts walk keys of their own: as in attn_paged.hpp.
+template <int D, int NW, bool STRIDED, int R, int CODE, class P>
+__device__ __forceinline__ void paged8_unit(const P& p, const PagedUnit& u, uint8_t* lds, bool bad, bool direct, float* out_o, f32x2* out_ml) {
     using T = Paged8Tile<D>;
-    const int tid = paged_thread(), lane = tid & 63, wave = packed_uniform(tid >> 6), n = lane & 31;
-    const uint8_t* const mine = reinterpret_cast<const uint8_t*>(lds) + wave * T::WAVE;
+    constexpr int DB = D / 16, ROWS = 16 * R;
+    const int tid = paged_thread(), lane = tid & 63, wave = packed_uniform(tid >> 6), n = lane & 15, g = lane >> 4;
+    const uint8_t* const mine = lds + wave * T::WAVE;
     constexpr int STEP = STRIDED ? NW : 1;
     const int run = (u.tiles + NW - 1) / NW;
     const int t_lo = u.tile0 + (STRIDED ? wave : wave * run), t_hi = STRIDED ? u.tile0 + u.tiles : min(t_lo + run, u.tile0 + u.tiles);
     PagedPages pages;
-    Paged8Copy<D, CODE> copy(p, u, pages, lane);
-    if (t_lo < t_hi) {
-        pages.load(p, u, lane, (t_lo * T::BN) >> p.page_shift);
-        paged8_start<STEP>(copy, mine, t_lo, t_hi);
+    if (STRIDED || t_lo < t_hi) pages.load(p, u, lane, (t_lo * T::BN) >> p.page_shift);
+    Paged8Copy<D, P> copy(p, u, pages, lane);
+    paged8_start<STEP>(copy, mine, t_lo, t_hi);
+    Paged8Rows<D, CODE, R> w;
+    w.begin(p, u, lane, 0);
+    int limit[R];
+    const int clean = paged8_limits<R>(p, u, lane, 0, limit);
+    paged8_walk<STEP>(copy, w, mine, t_lo, t_hi, limit, clean);
+
+    // ---- the wavefronts' states become one
+    __shared__ f32x2 state[NW][ROWS], joined[ROWS];
+    const bool lost = __any(bad | (pages.bad && t_lo < t_hi));                    // a page outside the cache, or more keys than pages: NaN
+#pragma unroll
+    for (int b = 0; b < R; ++b) {
+        w.l_run[b] = lost ? __builtin_nanf("") : w.over_groups_sum(w.l_run[b]);
+        if (g == 0) state[wave][16 * b + n] = f32x2{w.m_run[b], w.l_run[b]};
     }
-    const PagedRow me = paged_row(p, u, min(n, u.rows - 1));
-    Paged8Rows<D, CODE> w;
-    w.begin(p, lane, me, n < u.rows);
-    const int limit = u.own ? max(u.keys - u.lag + me.i, 0) : u.keys, clean = u.own ? max(u.keys - u.lag, 0) : u.keys;
-    paged8_walk<STEP>(u, copy, w, mine, t_lo, t_hi, limit, clean);
-    paged_unit_join<D, NW, T::WAVE / 4>(p, u, w, reinterpret_cast<float*>(lds), tid, bad | pages.bad, direct, out_o, out_ml);
+    __syncthreads();                                   // (no copy is under way: every wavefront has waited for its last one)
+    float* const sums = reinterpret_cast<float*>(lds + wave * T::WAVE);           // [rows][D], granules of four swizzled by the row
+#pragma unroll
+    for (int b = 0; b < R; ++b) {
+        float M = -INFINITY, L = 0.f;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) M = fmaxf(M, state[i][16 * b + n][0]);
+        const float M_to = M == -INFINITY ? 0.f : M;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) L += state[i][16 * b + n][1] * exp2_fast((state[i][16 * b + n][0] - M_to) * w.c_log2);
+        const float f = exp2_fast((w.m_run[b] - M_to) * w.c_log2);
+#pragma unroll
+        for (int db = 0; db < DB; ++db) *reinterpret_cast<f32x4*>(sums + (16 * b + n) * D + (((4 * db + g) ^ (n & 7)) << 2)) = w.oacc[b][db] * f;
+        if (wave == 0 && g == 0) joined[16 * b + n] = f32x2{M * w.c_log2, L};
+    }
+    __syncthreads();
+    for (int e = tid; e < u.rows * (D / 4); e += 64 * NW) {
+        const int r = e / (D / 4), q = e % (D / 4);
+        if (4 * q >= p.d) continue;
+        f32x4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < NW; ++i) a += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + i * T::WAVE) + r * D + ((q ^ (r & 7)) << 2));
+        if (direct) {
+            const float l = joined[r][1], inv = l == 0.f ? 0.f : 1.0f / l;
+            const PagedRow at = paged_row(p, u, r);
+            *reinterpret_cast<u32x2*>(p.o + at.b * p.os.b + at.h * p.os.h + at.i * p.os.n + 4 * q) = u32x2{pack_bf16(a[0] * inv, a[1] * inv), pack_bf16(a[2] * inv, a[3] * inv)};
+        } else {
+            *reinterpret_cast<f32x4*>(out_o + (int64_t)r * p.d + 4 * q) = a;
+        }
+    }
+    if (tid < u.rows) {
+        const f32x2 ml = joined[tid];
+        if (!direct) out_ml[tid] = ml;
+        else if (p.lse) {
+            const PagedRow at = paged_row(p, u, tid);
+            p.lse[((int64_t)at.b * p.H + at.h) * p.N + at.i] = ml[1] == 0.f ? -INFINITY : (ml[0] + log2_fast(ml[1])) * kLn2;
+        }
+    }
+}
+// Own keys: R blocks; a prefix, whose rows are those of several sequences: two.
+template <int D, int NW, bool STRIDED, int CODE, int R>
+__device__ __forceinline__ void paged_unit_body(const Paged8Params<CODE, R>& p, const PagedUnit& u, uint16_t* lds, bool bad, bool direct, float* out_o, f32x2* out_ml) {
+    if (STRIDED || u.own || R == 2) paged8_unit<D, NW, STRIDED, R, CODE>(p, u, reinterpret_cast<uint8_t*>(lds), bad, direct, out_o, out_ml);
+    else paged8_unit<D, NW, STRIDED, 2, CODE>(p, u, reinterpret_cast<uint8_t*>(lds), bad, direct, out_o, out_ml);
 }
 
 // A unit of the prefix with 128 rows: the wavefronts have 32 each.
-template <int D, int CODE>
-__device__ __forceinline__ void paged_shared_body(const Paged8Params<CODE>& p, const PagedUnit& u, uint16_t* lds, bool bad, float* out_o, f32x2* out_ml) {
+template <int D, int CODE, int R>
+__device__ __forceinline__ void paged_shared_body(const Paged8Params<CODE, R>& p, const PagedUnit& u, uint16_t* lds, bool bad, float* out_o, f32x2* out_ml) {
     using T = Paged8Tile<D>;
-    constexpr int DB = D / 32;
-    const int tid = paged_thread(), lane = tid & 63, wave = packed_uniform(tid >> 6), n = lane & 31, h = lane >> 5;
+    using P = Paged8Params<CODE, R>;
+    const int tid = paged_thread(), lane = tid & 63, wave = packed_uniform(tid >> 6), n = lane & 15, g = lane >> 4;
     const uint8_t* const mine = reinterpret_cast<const uint8_t*>(lds) + wave * T::WAVE;
-    const int rows = min(32, u.rows - 32 * wave), t_lo = u.tile0, t_hi = u.tile0 + u.tiles;
-    if (rows <= 0) return;
+    const int row0 = 32 * wave, t_lo = u.tile0, t_hi = u.tile0 + u.tiles;
+    if (row0 >= u.rows) return;
     PagedPages pages;
-    Paged8Copy<D, CODE> copy(p, u, pages, lane);
     pages.load(p, u, lane, (t_lo * T::BN) >> p.page_shift);
+    Paged8Copy<D, P> copy(p, u, pages, lane);
     paged8_start<1>(copy, mine, t_lo, t_hi);
-    const PagedRow me = paged_row(p, u, min(32 * wave + n, u.rows - 1));
-    Paged8Rows<D, CODE> w;
-    w.begin(p, lane, me, n < rows);
-    paged8_walk<1>(u, copy, w, mine, t_lo, t_hi, u.keys, u.keys);
-    w.l_run += xhalf(w.l_run);
-    if (__any(bad | pages.bad)) w.l_run = __builtin_nanf("");
-    if (n >= rows) return;
-    float* const out = out_o + (int64_t)(32 * wave + n) * p.d + 4 * h;
+    Paged8Rows<D, CODE, 2> w;
+    w.begin(p, u, lane, row0);
+    const int limit[2] = {u.keys, u.keys};
+    paged8_walk<1>(copy, w, mine, t_lo, t_hi, limit, u.keys);
+    const bool lost = __any(bad | pages.bad);
 #pragma unroll
-    for (int db = 0; db < DB; ++db)
+    for (int b = 0; b < 2; ++b) {
+        const int r = row0 + 16 * b + n;
+        const float l = lost ? __builtin_nanf("") : w.over_groups_sum(w.l_run[b]);
+        if (r >= u.rows) continue;
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const f32x16& a = w.oacc[db];
-            if (32 * db + 8 * g + 4 * h < p.d) *reinterpret_cast<f32x4*>(out + 32 * db + 8 * g) = f32x4{a[4 * g], a[4 * g + 1], a[4 * g + 2], a[4 * g + 3]};
-        }
-    if (h == 0) out_ml[32 * wave + n] = f32x2{w.m_run * w.c_log2, w.l_run};
+        for (int db = 0; db < D / 16; ++db)
+            if (16 * db + 4 * g < p.d) *reinterpret_cast<f32x4*>(out_o + (int64_t)r * p.d + 16 * db + 4 * g) = w.oacc[b][db];
+        if (g == 0) out_ml[r] = f32x2{w.m_run[b] * w.c_log2, l};
+    }
 }
 
 }  // namespace fattn

@@ -27,8 +27,8 @@ int launch_store(const KvStore8Params& p, hipStream_t s) {
     return launch_store<CODE, 256, 8>(p, s);           // up to 128 tokens of 128 numbers
 }
 
-template <int CODE>
-int attend(const Paged8Params<CODE>& p, const PagedSizes& z, hipStream_t s) {
+template <int CODE, int R>
+int attend(const Paged8Params<CODE, R>& p, const PagedSizes& z, hipStream_t s) {
     return p.d <= 64 ? launch_paged<64>(p, z, s) : launch_paged<128>(p, z, s);
 }
 
@@ -49,6 +49,8 @@ int flame_attn_paged_fwd_q8(const void* Q, const void* K_cache, const void* V_ca
     if ((rc = check_view(Q, q_strides, 4)) || (rc = check_byte_view(K_cache, k_strides, 4)) || (rc = check_byte_view(V_cache, v_strides, 4)) ||
         (rc = check_scales(K_scale, ks_strides, 3, page / block)) || (rc = check_scales(V_scale, vs_strides, 3, page / block)) || (rc = check_view(O, o_strides, 4)))
         return rc;
+    for (const int64_t* st : {ks_strides, vs_strides})             // kept in bytes and 32 bits
+        if (st[0] > INT32_MAX / 4 || st[2] > INT32_MAX / 4) return FLAME_ATTN_ERR_UNSUPPORTED;
     const int64_t o_size[4] = {B, H, N, D};
     if (overlaps(o_strides, o_size, 4)) return FLAME_ATTN_ERR_UNSUPPORTED;
     PagedSizes z;
@@ -73,8 +75,8 @@ int flame_attn_paged_fwd_q8(const void* Q, const void* K_cache, const void* V_ca
         p.qs = Strides{q_strides[0], q_strides[1], q_strides[2]};
         p.ks = Strides{k_strides[0], k_strides[1], k_strides[2]};
         p.vs = Strides{v_strides[0], v_strides[1], v_strides[2]};
-        p.kss = Strides{ks_strides[0], ks_strides[1], ks_strides[2]};
-        p.vss = Strides{vs_strides[0], vs_strides[1], vs_strides[2]};
+        p.kss = Strides{4 * ks_strides[0], 4 * ks_strides[1], 4 * ks_strides[2]};
+        p.vss = Strides{4 * vs_strides[0], 4 * vs_strides[1], 4 * vs_strides[2]};
         p.os = Strides{o_strides[0], o_strides[1], o_strides[2]};
         p.B = B;
         p.H = H;
@@ -91,7 +93,8 @@ int flame_attn_paged_fwd_q8(const void* Q, const void* K_cache, const void* V_ca
         p.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + z.plan_bytes + z.ml_bytes);
         return attend(p, z, static_cast<hipStream_t>(stream));
     };
-    return cache_dtype == FLAME_ATTN_DTYPE_I8 ? call(Paged8Params<kI8>{}) : call(Paged8Params<kE4m3>{});
+    if (N * (H / H_kv) <= 16) return cache_dtype == FLAME_ATTN_DTYPE_I8 ? call(Paged8Params<kI8, 1>{}) : call(Paged8Params<kE4m3, 1>{});
+    return cache_dtype == FLAME_ATTN_DTYPE_I8 ? call(Paged8Params<kI8, 2>{}) : call(Paged8Params<kE4m3, 2>{});
 }
 
 int flame_kv_store_q8(const void* K, const void* V, void* K_cache, void* V_cache, int cache_dtype, float* K_scale, float* V_scale, int block,
