@@ -28,8 +28,10 @@ __device__ __forceinline__ f32x4 codes_to_f32(uint32_t w) {
 template <int CODE>
 __device__ __forceinline__ uint32_t f32_to_codes(float a, float b, float c, float d) {
     if constexpr (CODE == kI8) {
-        const int i = (int)__builtin_rintf(a), j = (int)__builtin_rintf(b), k = (int)__builtin_rintf(c), l = (int)__builtin_rintf(d);
-        return (uint32_t)(i & 255) | (uint32_t)(j & 255) << 8 | (uint32_t)(k & 255) << 16 | (uint32_t)l << 24;
+        // of a sum with 3 2^22 the last place is 1: the addition rounds, and the low byte is the code
+        const uint32_t i = __builtin_bit_cast(uint32_t, a + 12582912.f), j = __builtin_bit_cast(uint32_t, b + 12582912.f);
+        const uint32_t k = __builtin_bit_cast(uint32_t, c + 12582912.f), l = __builtin_bit_cast(uint32_t, d + 12582912.f);
+        return __builtin_amdgcn_perm(__builtin_amdgcn_perm(l, k, 0x0c0c0400u), __builtin_amdgcn_perm(j, i, 0x0c0c0400u), 0x05040100u);
     } else {
         const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
         return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, lo, true);

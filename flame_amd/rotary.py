@@ -67,7 +67,7 @@ class Rotary:
     def turns_on(self, device) -> torch.Tensor:
         """int64 [rotary_dim / 2] on the device: 2^64 turns per position.  Copied there by the first call, which a captured graph therefore
         has behind it."""
-        device = torch.device(device)
-        if device not in self._on:
-            self._on[device] = self._turns.to(device)
-        return self._on[device]
+        turns = self._on.get(device)
+        if turns is None:
+            turns = self._on[device] = self._turns.to(device)
+        return turns
