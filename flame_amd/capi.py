@@ -186,8 +186,9 @@ def attn_packed_bwd(q, k, v, o, do, lse, cu_q, cu_k, scale, causal=True, workspa
 
 
 # ---------------------------------------------------------------- paged cache of keys and values
-def paged_workspace_bytes(B, H, H_kv, N, D, page, table_pages, prefix_pages=0) -> int:
-    f = lib().flame_attn_paged_workspace_bytes
+def paged_workspace_bytes(B, H, H_kv, N, D, page, table_pages, prefix_pages=0, q8=False) -> int:
+    """q8: of caches in 8 bits"""
+    f = lib().flame_attn_paged_q8_workspace_bytes if q8 else lib().flame_attn_paged_workspace_bytes
     f.restype = ctypes.c_size_t
     return int(f(B, H, H_kv, N, D, page, table_pages, prefix_pages))
 

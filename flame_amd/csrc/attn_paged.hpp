@@ -48,7 +48,9 @@ struct PagedParams {
     int64_t own_slot;              // rows of the partial results that the prefix has (a host bound); the own ones follow
     float* part_o;                 // [row][d]
     f32x2* part_ml;                // m and l of every row
-    int2* plan;                    // [B] first unit and units per (head, row tile) of a sequence, then the splits of the prefix
+    // [B] first unit and units per (head, row tile) of a sequence, then the splits of the prefix and 0; with ranges of tiles: [B] first tile and
+    // tiles per (head, row tile), then the tiles of a range and 1
+    int2* plan;
 };
 
 // How the keys are cut.  A walk (one sequence, key head and tile of rows, or the prefix in place of the sequence) has a tile for every 32 keys; a
@@ -129,7 +131,7 @@ __device__ __forceinline__ int paged_tiles(int keys) { return (keys + PagedCut::
 struct PagedPlan {
     int prefix_keys, prefix_tiles, prefix_unit, prefix_splits, prefix_units;   // keys, tiles, tiles per unit, units per row tile and head, all units
     bool prefix_bad;
-    int own_unit;
+    int own_tiles, own_unit;       // of all walks together, tiles per unit
     int len;                       // raw number of keys of sequence `tid`
 };
 // Every thread of the workgroup (256) calls this; `sums` is 4 ints of LDS.
@@ -148,6 +150,7 @@ __device__ __forceinline__ PagedPlan paged_plan(const PagedParams& p, int* sums)
     __syncthreads();
     const int rows = p.N * (p.H / p.Hkv);
     const int heads = p.Hkv * PagedCut::row_tiles(rows), own = packed_uniform(sums[0] + sums[1] + sums[2] + sums[3]) * heads;
+    c.own_tiles = own;
     c.own_unit = packed_uniform(PagedCut::unit(own, p.B * heads));
     c.prefix_tiles = paged_tiles(c.prefix_keys);
     const int all = p.B * rows, per_split = p.Hkv * PagedCut::prefix_row_tiles(all), total = c.prefix_tiles * per_split;
@@ -157,17 +160,18 @@ __device__ __forceinline__ PagedPlan paged_plan(const PagedParams& p, int* sums)
     return c;
 }
 
-// Walks the sequences in the order of their units and calls take(b, raw keys, first unit, units per row tile and head) in the one
-// thread that has sequence b, for every b (the threads of a workgroup take 256 sequences at a time).  `sums`: 4 ints of LDS.
-template <class F>
-__device__ __forceinline__ void paged_own_units(const PagedParams& p, const PagedPlan& c, int* sums, F&& take) {
+// Walks the sequences in the order of their units, units_of(tiles) for every row tile and head, and calls take(b, raw keys, first unit, units per row
+// tile and head) in the one thread that has sequence b, for every b (the threads of a workgroup take 256 sequences at a time).  `sums`: 4 ints
+// of LDS.
+template <class N, class F>
+__device__ __forceinline__ void paged_own_units(const PagedParams& p, const PagedPlan& c, int* sums, N&& units_of, F&& take) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, most = p.table_pages << p.page_shift;
     const int per_split = p.Hkv * PagedCut::row_tiles(p.N * (p.H / p.Hkv));
     int before = 0;
     for (int b0 = 0; b0 < p.B; b0 += 256) {
         const int b = b0 + tid;
         const int len = b0 == 0 ? c.len : b < p.B ? p.kv_len[b] : 0;
-        const int splits = PagedCut::splits(paged_tiles(min(max(len, 0), most)), c.own_unit, p.B * per_split);
+        const int splits = units_of(paged_tiles(min(max(len, 0), most)));
         const int through = wave_scan(splits * per_split);
         __syncthreads();                               // the sums are free
         if (lane == 63) sums[wave] = through;
@@ -603,7 +607,8 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void paged_fwd_kernel(const P
             const int number = taken < ahead ? spare + taken * free : ahead * free + (int)blockIdx.x + (taken - ahead) * (int)gridDim.x;
             ++taken;
             if (threadIdx.x == 0) found[0] = -1;
-            paged_own_units(p, c, sums, [&](int b, int len, int first, int splits) {
+            auto units_of = [&](int tiles) { return PagedCut::splits(tiles, c.own_unit, p.B * p.Hkv * rt); };
+            paged_own_units(p, c, sums, units_of, [&](int b, int len, int first, int splits) {
                 if (number >= first && number < first + splits * p.Hkv * rt) {
                     found[0] = b;
                     found[1] = first;
@@ -670,14 +675,23 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams p) {
     if (SHARE == 1 && at_row >= p.B * p.H * p.N) return;
     const int G = p.H / p.Hkv, rows = p.N * G, rt = PagedCut::row_tiles(rows), all = p.B * rows, slot_rows = min(32, rows);
     const int pair = packed_uniform(at_row / rows), r = at_row - pair * rows, b = packed_uniform(pair / p.Hkv), kv_head = pair - b * p.Hkv;
-    const int2 mine = p.plan[b];
-    const int own = packed_uniform(mine.y), prefix = packed_uniform(p.plan[p.B].x), parts = own + prefix;
+    const int2 mine = p.plan[b], all_of = p.plan[p.B];
+    const bool ranges = packed_uniform(all_of.y) != 0;
+    const int share = ranges ? packed_uniform(all_of.x) : 1, tiles = packed_uniform(mine.y);
+    // ranges: the walk's first tile, the range that it begins in
+    const int at_tile = packed_uniform(mine.x) + (kv_head * rt + r / 32) * tiles, range = at_tile / share;
+    const int own = !ranges ? tiles : tiles == 0 ? 0 : (at_tile + tiles - 1) / share - range + 1;
+    const int prefix = ranges ? 0 : packed_uniform(all_of.x), parts = own + prefix;
     if (own == 1 && prefix == 0) return;                   // written by the unit itself
     // rows of the partial results: unit s of the prefix, unit s of the own keys
     const int64_t prefix_pad = (int64_t)PagedCut::prefix_row_tiles(all) * PagedCut::prefix_tile_rows(all);
     const int64_t prefix_at = kv_head * prefix_pad + b * rows + r, prefix_step = p.Hkv * prefix_pad;
     const int64_t own_at = p.own_slot + (int64_t)(packed_uniform(mine.x) + (kv_head * rt + r / 32) * own) * slot_rows + r % 32;
-    auto slot_of = [&](int s) { return s < prefix ? prefix_at + s * prefix_step : own_at + (int64_t)(s - prefix) * slot_rows; };
+    auto slot_of = [&](int s) {
+        // a range has two places, for a walk that it ends or goes on with and for one that it begins
+        if (ranges) return p.own_slot + (int64_t)(s == 0 ? 2 * range + 1 : 2 * (range + s)) * slot_rows + r % 32;
+        return s < prefix ? prefix_at + s * prefix_step : own_at + (int64_t)(s - prefix) * slot_rows;
+    };
     float M = -INFINITY, L = 0.f, a0 = 0.f, a1 = 0.f;
     bool nan = false;
     const bool col = 2 * lane < p.d;

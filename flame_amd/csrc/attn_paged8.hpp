@@ -5,7 +5,7 @@
 // numbers out of codes and scales would take one for every element and a rounding.  The codes become bf16 (exactly) on their way from LDS to the
 // matrix instructions: a value's column comes through the transposing read of 8 bits, eight tokens at a time, in the order of the weights.
 //
-// The way of units, plan and merge is that of the bf16 cache.  With half the bytes a tile's arithmetic weighs twice as much, so rows come in blocks of 16
+// Units, partial results and merge are those of the bf16 cache; without a prefix the keys are cut otherwise (paged_ranges_kernel).  With half the bytes a tile's arithmetic weighs twice as much, so rows come in blocks of 16
 // (v_mfma_f32_16x16x32_bf16), one block where a sequence has no more rows than that: half of the exponentials and of what goes with them.  A
 // wavefront has two tiles of K, V and scales in LDS and requests a tile two steps ahead.
 #pragma once
@@ -424,6 +424,68 @@ __device__ __forceinline__ void paged_shared_body(const Paged8Params<CODE, R>& p
         for (int db = 0; db < D / 16; ++db)
             if (16 * db + 4 * g < p.d) *reinterpret_cast<f32x4*>(out_o + (int64_t)r * p.d + 16 * db + 4 * g) = w.oacc[b][db];
         if (g == 0) out_ml[r] = f32x2{w.m_run[b] * w.c_log2, l};
+    }
+}
+
+// Without a prefix: all tiles of all walks (sequence by sequence, key head by key head, one tile of rows after the other) are cut into ranges of the same
+// length, one for every workgroup that runs at once, whatever the sequences' lengths.  A walk that lies in one range is written by its workgroup, the
+// others' parts are joined by the merge; a range has at most one walk that began before it and one that goes on behind it.
+// (In units of up to 64 tiles dealt in turn -> in ranges, us, D = 128, e4m3, 64 sequences of 2000 to 6000 114 -> 105, of 8000 194 -> 185 (5.7 TB/s), one of
+// 131072 61 -> 58; in int8 117 -> 107, 197 -> 189, 63 -> 60.)
+template <int D>
+constexpr int kPaged8Groups = D <= 64 ? 3 : 2;         // workgroups on a compute unit
+template <int D, class P>
+__global__ __launch_bounds__(256, kPaged8Groups<D>) void paged_ranges_kernel(const P p) {
+    extern __shared__ __attribute__((aligned(1024))) uint16_t lds[];
+    __shared__ int sums[4], found[4];
+    const int rows = p.N * (p.H / p.Hkv), rt = PagedCut::row_tiles(rows), heads = p.Hkv * rt, slot_rows = min(32, rows), most = p.table_pages << p.page_shift;
+    const PagedPlan c = paged_plan(p, sums);
+    const int share = packed_uniform(max(PagedCut::kLeast, (int)((c.own_tiles + gridDim.x - 1) / gridDim.x)));
+    const int range = (int)blockIdx.x;                 // (ranges one behind the other on one XCD: no gain, also where its heads' rows share lines)
+    int at = min(range * share, c.own_tiles);
+    const int end = min(at + share, c.own_tiles);
+    if (range != 0 && at >= end) return;
+    paged_own_units(p, c, sums, [](int tiles) { return tiles; }, [&](int b, int len, int first, int tiles) {
+        if (at >= first && at < first + tiles * heads) {
+            found[0] = b;
+            found[1] = first;
+            found[2] = tiles;
+            found[3] = len;
+        }
+        if (range == 0) p.plan[b] = int2{first, tiles};
+    });
+    if (range == 0 && threadIdx.x == 0) p.plan[p.B] = int2{share, 1};
+    if (at >= end) return;
+    __syncthreads();
+    int b = packed_uniform(found[0]), tiles = packed_uniform(found[2]), len = packed_uniform(found[3]);
+    int pair = packed_uniform((at - found[1]) / tiles), tile0 = packed_uniform(at - found[1]) - pair * tiles;
+    while (true) {
+        PagedUnit u;
+        u.own = true;
+        u.table = p.table + b * p.table_stride;
+        u.entries = p.table_pages;
+        u.keys = min(max(len, 0), most);
+        u.kv_head = packed_uniform(pair / rt);
+        u.row0 = 32 * (pair - u.kv_head * rt);
+        u.rows = min(32, rows - u.row0);
+        u.b0 = b;
+        u.lag = p.N - 1;
+        u.tile0 = tile0;
+        u.tiles = min(tiles - tile0, end - at);
+        const int64_t slot = p.own_slot + (int64_t)(2 * range + (tile0 == 0)) * slot_rows;
+        paged_unit_body<D, 4, false>(p, u, lds, len > most, u.tiles == tiles, p.part_o + slot * p.d, p.part_ml + slot);
+        at += u.tiles;
+        if (at >= end) return;
+        tile0 = 0;
+        if (++pair == heads) {
+            pair = 0;
+            do {                                       // (there is another one with keys: the range goes on)
+                len = packed_uniform(p.kv_len[++b]);
+                tiles = paged_tiles(min(max(len, 0), most));
+            } while (tiles == 0 && b + 1 < p.B);
+            if (tiles == 0) return;
+        }
+        __syncthreads();                               // the last unit's LDS is free
     }
 }
 

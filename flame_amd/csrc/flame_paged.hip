@@ -73,7 +73,7 @@ extern "C" {
 size_t flame_attn_paged_workspace_bytes(int B, int H, int H_kv, int N, int D, int page, int table_pages, int prefix_pages) {
     if (B <= 0 || H <= 0 || H_kv <= 0 || N <= 0 || D <= 0 || table_pages <= 0 || prefix_pages < 0 || H % H_kv != 0 || !head_dim_ok(D) || page_shift(page) < 0) return 0;
     PagedSizes z;
-    return paged_sizes(B, H, H_kv, N, D, page, table_pages, prefix_pages, &z) ? z.bytes : 0;
+    return paged_sizes(B, H, H_kv, N, D, page, table_pages, prefix_pages, false, &z) ? z.bytes : 0;
 }
 
 int flame_attn_paged_fwd_bf16(const void* Q, const void* K_cache, const void* V_cache, void* O, void* LSE, const int32_t* page_table,
@@ -92,7 +92,7 @@ int flame_attn_paged_fwd_bf16(const void* Q, const void* K_cache, const void* V_
     const int64_t o_size[4] = {B, H, N, D};
     if (overlaps(o_strides, o_size, 4)) return FLAME_ATTN_ERR_UNSUPPORTED;
     PagedSizes z;
-    if (!paged_sizes(B, H, H_kv, N, D, page, table_pages, prefix_pages, &z) || (int64_t)B * H * N > INT32_MAX / 2) return FLAME_ATTN_ERR_UNSUPPORTED;
+    if (!paged_sizes(B, H, H_kv, N, D, page, table_pages, prefix_pages, false, &z) || (int64_t)B * H * N > INT32_MAX / 2) return FLAME_ATTN_ERR_UNSUPPORTED;
     if (z.bytes && (!workspace || workspace_bytes < z.bytes)) return FLAME_ATTN_ERR_INVALID;
     if (reinterpret_cast<uintptr_t>(workspace) & 15u) return FLAME_ATTN_ERR_UNSUPPORTED;
     PagedParams p{};

@@ -34,14 +34,32 @@ int launch_store(const KvStore8Params& p, int64_t slots, hipStream_t s) {
     return launch_store<CODE, 256, 8>(p, slots, s);    // up to 128 tokens of 128 numbers
 }
 
+template <int D, int CODE, int R>
+int attend(const Paged8Params<CODE, R>& p, const PagedSizes& z, hipStream_t s) {
+    if (z.direct || p.prefix_pages) return launch_paged<D>(p, z, s);
+    static std::atomic<uint64_t> done{0};
+    const auto kern = paged_ranges_kernel<D, Paged8Params<CODE, R>>;
+    constexpr int lds = Paged8Tile<D>::lds_bytes(4);
+    if (const int rc = set_lds_of_device(reinterpret_cast<const void*>(kern), lds, done)) return rc;
+    const int64_t room = 256 * kPaged8Groups<D>;       // workgroups that the card holds
+    hipLaunchKernelGGL(kern, dim3((unsigned)std::max<int64_t>(1, std::min(room, z.own_units / 2))), dim3(256), lds, s, p);
+    if (const hipError_t e = hipGetLastError()) return (int)e;
+    return launch_paged_merge(p, s);
+}
 template <int CODE, int R>
 int attend(const Paged8Params<CODE, R>& p, const PagedSizes& z, hipStream_t s) {
-    return p.d <= 64 ? launch_paged<64>(p, z, s) : launch_paged<128>(p, z, s);
+    return p.d <= 64 ? attend<64>(p, z, s) : attend<128>(p, z, s);
 }
 
 }  // namespace
 
 extern "C" {
+
+size_t flame_attn_paged_q8_workspace_bytes(int B, int H, int H_kv, int N, int D, int page, int table_pages, int prefix_pages) {
+    if (B <= 0 || H <= 0 || H_kv <= 0 || N <= 0 || D <= 0 || table_pages <= 0 || prefix_pages < 0 || H % H_kv != 0 || D % 16 != 0 || D > 128 || page_shift(page) < 0) return 0;
+    PagedSizes z;
+    return paged_sizes(B, H, H_kv, N, D, page, table_pages, prefix_pages, true, &z) ? z.bytes : 0;
+}
 
 int flame_attn_paged_fwd_q8(const void* Q, const void* K_cache, const void* V_cache, int cache_dtype, const float* K_scale, const float* V_scale, int block,
                             void* O, void* LSE, const int32_t* page_table, int64_t table_stride, int table_pages, const int32_t* kv_len,
@@ -61,7 +79,7 @@ int flame_attn_paged_fwd_q8(const void* Q, const void* K_cache, const void* V_ca
     const int64_t o_size[4] = {B, H, N, D};
     if (overlaps(o_strides, o_size, 4)) return FLAME_ATTN_ERR_UNSUPPORTED;
     PagedSizes z;
-    if (!paged_sizes(B, H, H_kv, N, D, page, table_pages, prefix_pages, &z) || (int64_t)B * H * N > INT32_MAX / 2) return FLAME_ATTN_ERR_UNSUPPORTED;
+    if (!paged_sizes(B, H, H_kv, N, D, page, table_pages, prefix_pages, true, &z) || (int64_t)B * H * N > INT32_MAX / 2) return FLAME_ATTN_ERR_UNSUPPORTED;
     if (z.bytes && (!workspace || workspace_bytes < z.bytes)) return FLAME_ATTN_ERR_INVALID;
     if (reinterpret_cast<uintptr_t>(workspace) & 15u) return FLAME_ATTN_ERR_UNSUPPORTED;
     auto call = [&](auto p) {

@@ -45,8 +45,10 @@ struct PagedSizes {
 // 1000 13.0 -> 11.4, 64 of 1000 48 -> 42, 64 of 2000 97 -> 92, 64 of 200 to 2000 57 -> 52.  4 of 2000 15.4, one workgroup each 17.9.)
 constexpr int64_t kDirectKeys = 1024;
 
-// false: too large
-inline bool paged_sizes(int B, int H, int H_kv, int N, int D, int page, int pages, int prefix_pages, PagedSizes* z) {
+constexpr int64_t kMostRanges = 1024;          // workgroups that run at once at most
+
+// false: too large; `ranges`: without a prefix the tiles are cut into ranges
+inline bool paged_sizes(int B, int H, int H_kv, int N, int D, int page, int pages, int prefix_pages, bool ranges, PagedSizes* z) {
     const int64_t rows = (int64_t)N * (H / H_kv), rt = (rows + 31) / 32;
     if (rows > INT32_MAX / 2 || B * rows > INT32_MAX / 2) return false;
     const int64_t prefix_rt = PagedCut::prefix_row_tiles((int)(B * rows));
@@ -56,6 +58,7 @@ inline bool paged_sizes(int B, int H, int H_kv, int N, int D, int page, int page
     z->direct = prefix_pages == 0 && (int64_t)pages * page <= (B * H_kv * rt < PagedCut::kFill / 2 ? kDirectKeys : PagedCut::kLong * PagedCut::kTile);
     if (!grid_fits(z->direct ? B * H_kv * rt : ((int64_t)B * H * N + 3) / 4)) return false;          // as launch_paged launches
     z->own_units = most_units((int64_t)own, B * H_kv * rt);
+    if (ranges && prefix_pages == 0) z->own_units = 2 * std::min<int64_t>(kMostRanges, ((int64_t)own + PagedCut::kLeast - 1) / PagedCut::kLeast);
     z->prefix_units = shared ? most_shared_units((int64_t)prefix, H_kv * prefix_rt) : most_units((int64_t)prefix, H_kv * prefix_rt);
     z->prefix_rows = z->prefix_units * (shared ? 128 : 32);
     z->own_rows = z->own_units * std::min<int64_t>(32, rows);

@@ -45,7 +45,7 @@ using at::Tensor;
     X(flame_attn_bwd_materialised_bf16) X(flame_sage_quant_qk_int8_ks) X(flame_sage_attn_fwd_bias_int8)                 \
     X(flame_attn_packed_fwd_bf16) X(flame_attn_packed_fwd_workspace_bytes) X(flame_attn_packed_bwd_bf16) X(flame_attn_packed_bwd_workspace_bytes)                \
     X(flame_attn_paged_workspace_bytes) X(flame_attn_paged_fwd_bf16) X(flame_kv_store_bf16) X(flame_kv_copy_pages_bf16)  \
-    X(flame_attn_paged_fwd_q8) X(flame_kv_store_q8) X(flame_kv_load) X(flame_kv_copy_pages_q8) X(flame_rotary)           \
+    X(flame_attn_paged_q8_workspace_bytes) X(flame_attn_paged_fwd_q8) X(flame_kv_store_q8) X(flame_kv_load) X(flame_kv_copy_pages_q8) X(flame_rotary)           \
     X(flame_attn_prep_rmsnorm_rope_bf16) X(flame_bf16_to_fp8) X(flame_fp8_to_bf16) X(flame_attn_cast_qkv_f32_to_bf16) X(flame_attn_cast_bf16_to_f32)
 
 struct Api {
@@ -993,11 +993,12 @@ void check_caches(const Tensor& kc, const Tensor& vc, const CacheScales& c, int6
             check_that(t->dim() == dims - 1 && t->scalar_type() == at::kFloat, "the scales are fp32 tensors, of one dimension less than the caches");
             for (int64_t ax = 0; ax + 2 < dims; ++ax) check_that(t->size(ax) == kc.size(ax), "the scales have the caches' pages and heads");
             check_that(t->size(dims - 2) > 0 && t->size(dims - 2) == c.k.size(dims - 2) && kc.size(dims - 2) % t->size(dims - 2) == 0, "the scales divide a page into blocks");
-            check_device(*t, kc, "all tensors are on one GPU");
         }
     }
     check_device(kc, kc, "the tensors are on a GPU");
     check_device(vc, kc, "all tensors are on one GPU");
+    for (const Tensor* t : {&c.k, &c.v})
+        if (t->defined()) check_device(*t, kc, "all tensors are on one GPU");
 }
 void check_ints(const Tensor& t, int64_t n, const Tensor& like, const char* what) {
     check_that(t.dim() == 1 && t.scalar_type() == at::kInt && t.size(0) == n && (n == 1 || t.stride(0) == 1), what);
@@ -1053,7 +1054,8 @@ void call_paged(const Tensor& q, const Tensor& kc, const Tensor& vc, const Paged
     if (!o.defined()) o = empty(q.sizes(), at::kBFloat16, q);
     if (want_lse) lse = empty({(int64_t)B * H, N}, at::kFloat, q);
     if (!workspace.defined())
-        if (const size_t need = g_api.flame_attn_paged_workspace_bytes(B, H, Hkv, N, D, page, pages, prefix)) workspace = bytes_like(need, q);
+        if (const size_t need = (c.scales.codes() ? g_api.flame_attn_paged_q8_workspace_bytes : g_api.flame_attn_paged_workspace_bytes)(B, H, Hkv, N, D, page, pages, prefix))
+            workspace = bytes_like(need, q);
     if (c.scales.codes()) {
         check_rc(g_api.flame_attn_paged_fwd_q8(ptr(q), ptr(kc), ptr(vc), cache_dtype(kc), static_cast<const float*>(ptr(c.scales.k)),
                                                static_cast<const float*>(ptr(c.scales.v)), c.scales.block(kc), ptr(o), ptr(lse), ints(c.table), c.table.stride(0),

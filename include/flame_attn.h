@@ -331,8 +331,9 @@ int flame_kv_copy_pages_bf16(void* K_cache, void* V_cache, int layers, int n_pag
  *     of two, 1 or more, with which a fits, and the older codes are divided by that power and rounded.  A number x becomes x / scale rounded
  *     to the nearest code, the even one of two.  Infinities and NaN, and a block whose beginning was not stored by such a call, make the scale
  *     NaN, and with it every answer that attends to the block, until its first token is stored again.
- *   - Everything else, page tables, lengths, workspaces (flame_attn_paged_workspace_bytes), is as above.
+ *   - Everything else, page tables, lengths, the rules of the workspace, is as above.
  * ---------------------------------------------------------------------------------------------- */
+size_t flame_attn_paged_q8_workspace_bytes(int B, int H, int H_kv, int N, int D, int page, int table_pages, int prefix_pages);
 int flame_attn_paged_fwd_q8(const void* Q, const void* K_cache, const void* V_cache, int cache_dtype, const float* K_scale,
                             const float* V_scale, int block, void* O, void* LSE, const int32_t* page_table, int64_t table_stride,
                             int table_pages, const int32_t* kv_len, const int32_t* prefix_table, int prefix_pages,

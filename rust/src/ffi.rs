@@ -209,6 +209,9 @@ extern "C" {
         d: c_int, k_strides: *const i64, v_strides: *const i64, src: *const i32, dst: *const i32, n: c_int,
         stream: *mut c_void
     ) -> c_int;
+    pub fn flame_attn_paged_q8_workspace_bytes(
+        b: c_int, h: c_int, h_kv: c_int, n: c_int, d: c_int, page: c_int, table_pages: c_int, prefix_pages: c_int
+    ) -> usize;
     pub fn flame_attn_paged_fwd_q8(
         q: *const c_void, k_cache: *const c_void, v_cache: *const c_void, cache_dtype: c_int, k_scale: *const f32,
         v_scale: *const f32, block: c_int, o: *mut c_void, lse: *mut c_void, page_table: *const i32,
