@@ -445,6 +445,7 @@ __global__ __launch_bounds__(256, kPaged8Groups<D>) void paged_ranges_kernel(con
     int at = min(range * share, c.own_tiles);
     const int end = min(at + share, c.own_tiles);
     if (range != 0 && at >= end) return;
+    if (threadIdx.x == 0) found[0] = -1;               // (what the lengths, read again, always replace unless somebody changes them meanwhile)
     paged_own_units(p, c, sums, [](int tiles) { return tiles; }, [&](int b, int len, int first, int tiles) {
         if (at >= first && at < first + tiles * heads) {
             found[0] = b;
@@ -458,6 +459,7 @@ __global__ __launch_bounds__(256, kPaged8Groups<D>) void paged_ranges_kernel(con
     if (at >= end) return;
     __syncthreads();
     int b = packed_uniform(found[0]), tiles = packed_uniform(found[2]), len = packed_uniform(found[3]);
+    if (b < 0) return;
     int pair = packed_uniform((at - found[1]) / tiles), tile0 = packed_uniform(at - found[1]) - pair * tiles;
     while (true) {
         PagedUnit u;
@@ -478,11 +480,11 @@ __global__ __launch_bounds__(256, kPaged8Groups<D>) void paged_ranges_kernel(con
         if (at >= end) return;
         tile0 = 0;
         if (++pair == heads) {
-            pair = 0;
-            do {                                       // (there is another one with keys: the range goes on)
-                len = packed_uniform(p.kv_len[++b]);
+            pair = tiles = 0;
+            while (tiles == 0 && ++b < p.B) {          // (there is another one with keys: the range goes on)
+                len = packed_uniform(p.kv_len[b]);
                 tiles = paged_tiles(min(max(len, 0), most));
-            } while (tiles == 0 && b + 1 < p.B);
+            }
             if (tiles == 0) return;
         }
         __syncthreads();                               // the last unit's LDS is free

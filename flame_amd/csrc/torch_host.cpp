@@ -1298,26 +1298,36 @@ struct Rotary : public torch::autograd::Function<Rotary> {
         ctx->saved_data["interleaved"] = interleaved;
         ctx->saved_data["size"] = size;
         ctx->saved_data["inverse"] = inverse;
+        ctx->saved_data["q"] = q.requires_grad();
+        ctx->saved_data["k"] = k.defined() && k.requires_grad();
         if (!k.defined()) return {yq};
+        // the result of an input that requires no gradient requires none either
+        if (!q.requires_grad()) ctx->mark_non_differentiable({yq});
+        if (!k.requires_grad()) ctx->mark_non_differentiable({yk});
         return {yq, yk};
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
         const auto saved = ctx->get_saved_variables();
         const bool interleaved = ctx->saved_data["interleaved"].toBool(), inverse = ctx->saved_data["inverse"].toBool();
         const double size = ctx->saved_data["size"].toDouble();
-        c10::OptionalDeviceGuard device(grads[0].device());
-        const Tensor dq = rotary_input(grads[0]), dk = grads.size() > 1 ? rotary_input(grads[1]) : Tensor();
+        const bool of_q = ctx->saved_data["q"].toBool() && grads[0].defined(), of_k = ctx->saved_data["k"].toBool() && grads[1].defined();
+        torch::autograd::variable_list result(9);
+        if (!of_q && !of_k) return result;
+        // one tensor, or both
+        const Tensor first = rotary_input(of_q ? grads[0] : grads[1]), second = of_q && of_k ? rotary_input(grads[1]) : Tensor();
+        c10::OptionalDeviceGuard device(first.device());
         torch::autograd::variable_list out;
         if (at::GradMode::is_enabled()) {
-            out = Rotary::apply(dq, maybe(dk), saved[0], maybe(saved[1]), maybe(saved[2]), maybe(saved[3]), interleaved, size, !inverse);
+            out = Rotary::apply(first, maybe(second), saved[0], maybe(saved[1]), maybe(saved[2]), maybe(saved[3]), interleaved, size, !inverse);
         } else {
             const RotaryCall c{saved[0], saved[1], saved[2], saved[3], interleaved, size};
-            Tensor yq = rotary_like(dq), yk = dk.defined() ? rotary_like(dk) : Tensor();
-            const int rc = call_rotary(dq, dk, c, !inverse, yq, yk);
+            out = {rotary_like(first), second.defined() ? rotary_like(second) : Tensor()};
+            const int rc = call_rotary(first, second, c, !inverse, out[0], out[1]);
             if (rc != FLAME_ATTN_OK) throw_python({"flame_rotary", rc});
-            out = {yq, yk};
         }
-        return {out[0], grads.size() > 1 ? out[1] : Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+        if (of_q) result[0] = out[0];
+        if (of_k) result[1] = of_q ? out[1] : out[0];
+        return result;
     }
 };
 

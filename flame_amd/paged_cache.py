@@ -108,7 +108,8 @@ class PagedCache:
             del self._len[seq]
 
     def cut(self, seq, length) -> None:
-        """Forgets the tokens from `length` on (drafted ones that were refused)."""
+        """Forgets the tokens from `length` on (drafted ones that were refused).  In 8 bits the block that `length` lies in keeps the scale that they
+        gave it."""
         if not 0 <= length <= self._len[seq]:
             raise ValueError("a sequence can be cut to at most its length")
         keep = -(-length // self.page)
@@ -232,7 +233,7 @@ class PagedCache:
         """k, v: bf16 [tokens of `held`, kv_heads, head_dim], sequence after sequence."""
         rows = sum(held.counts)
         if not rows:
-            return (torch.empty((0, self.k.shape[2], self.k.shape[4]), dtype=torch.bfloat16, device=self.k.device) for _ in range(2))
+            return tuple(torch.empty((0, self.k.shape[2], self.k.shape[4]), dtype=torch.bfloat16, device=self.k.device) for _ in range(2))
         return capi.kv_load(self.k[layer], self.v[layer], held.page_table, held.cu, held.start, rows, *self._scales(layer))
 
     def attend_rows(self, layer, q, batch, held, scale=None):

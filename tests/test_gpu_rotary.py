@@ -184,6 +184,21 @@ def test_broadcast_leaves_and_second_derivatives():
         yk.sum().backward()
 
 
+@pytest.mark.parametrize("which", [0, 1])
+def test_only_one_requires_a_gradient(which):
+    """The other's result requires none, and is taken where that is refused."""
+    rope = Rotary(64)
+    pos = torch.arange(10, dtype=torch.int32, device="cuda")
+    x = [torch.randn((10, 4, 64), device="cuda"), torch.randn((10, 2, 64), device="cuda")]
+    both = functional.rotary(rope, *x, positions=pos)
+    x[which].requires_grad_(True)
+    y = functional.rotary(rope, *x, positions=pos)
+    assert y[which].requires_grad and not y[1 - which].requires_grad and all(torch.equal(a, b) for a, b in zip(y, both))
+    w = torch.randn_like(y[which])
+    (g,) = torch.autograd.grad((y[which] * w).sum() + y[1 - which].sum(), x[which])
+    close(g, *reference(w, pos, rope, back=True), torch.float32)
+
+
 def test_captured():
     """Forward and backward in a graph, replayed on new inputs and positions; an eager graph of the same leaf that lives on is refused."""
     rope = Rotary(128, interleaved=True)
