@@ -397,34 +397,138 @@ __device__ __forceinline__ void paged_unit_body(const Paged8Params<CODE, R>& p, 
     else paged8_unit<D, NW, STRIDED, 2, CODE>(p, u, reinterpret_cast<uint8_t*>(lds), bad, direct, out_o, out_ml);
 }
 
-// A unit of the prefix with 128 rows: the wavefronts have 32 each.
+// A unit of the prefix with 128 rows: the wavefronts have 32 each and share the tiles, as those of the bf16 cache do (attn_paged.hpp), in blocks of 32 rows.
+// Every wavefront converts a quarter of a tile, on the way from its registers to LDS: eight rows of K and of V, which it has requested two tiles ahead.
+// Three stages: tile t is in stage t % 3; behind the barrier of tile t, tile t + 1 is there and the stage of tile t - 1 free for tile t + 2.  Loads past the
+// last tile re-read it.
+// (Each wavefront with tiles of its own -> shared, us, 64 answers on a prefix of 8192, D = 128: int8 41.8 -> 39.8, e4m3 38.6 -> 36.4.)
 template <int D, int CODE, int R>
 __device__ __forceinline__ void paged_shared_body(const Paged8Params<CODE, R>& p, const PagedUnit& u, uint16_t* lds, bool bad, float* out_o, f32x2* out_ml) {
-    using T = Paged8Tile<D>;
-    using P = Paged8Params<CODE, R>;
-    const int tid = paged_thread(), lane = tid & 63, wave = packed_uniform(tid >> 6), n = lane & 15, g = lane >> 4;
-    const uint8_t* const mine = reinterpret_cast<const uint8_t*>(lds) + wave * T::WAVE;
-    const int row0 = 32 * wave, t_lo = u.tile0, t_hi = u.tile0 + u.tiles;
-    if (row0 >= u.rows) return;
+    using B16 = PagedTile<D>;
+    constexpr int DC = D / 16, DB = D / 32, PIECE = D / 8, TILE = B16::TILE_ELEMS, STAGE = 2 * TILE + 128;       // PIECE: bytes of a lane; 16-bit elements of a stage
+    static_assert(3 * STAGE * 2 <= Paged8Tile<D>::lds_bytes(4), "three stages");
+    const int tid = paged_thread(), lane = tid & 63, wave = packed_uniform(tid >> 6), n = lane & 31, h = lane >> 5;
+    const uint8_t* const k_base = p.k8 + u.kv_head * p.ks.h;
+    const uint8_t* const v_base = p.v8 + u.kv_head * p.vs.h;
+    const int my_row = 8 * wave + (lane >> 3), column = (lane & 7) * PIECE, from_column = column < p.d ? column : 0;      // (columns past d meet zeros of Q or are not stored)
+    const int t_hi = u.tile0 + u.tiles, rows = min(32, u.rows - 32 * wave);
+    const float* const s_base = lane < 32 ? reinterpret_cast<const float*>(reinterpret_cast<const char*>(p.k_scale) + u.kv_head * p.kss.h)
+                                          : reinterpret_cast<const float*>(reinterpret_cast<const char*>(p.v_scale) + u.kv_head * p.vss.h);
+    const int s_page = (int)(lane < 32 ? p.kss.b : p.vss.b), s_block = (int)(lane < 32 ? p.kss.n : p.vss.n);
     PagedPages pages;
-    pages.load(p, u, lane, (t_lo * T::BN) >> p.page_shift);
-    Paged8Copy<D, P> copy(p, u, pages, lane);
-    paged8_start<1>(copy, mine, t_lo, t_hi);
-    Paged8Rows<D, CODE, 2> w;
-    w.begin(p, u, lane, row0);
-    const int limit[2] = {u.keys, u.keys};
-    paged8_walk<1>(copy, w, mine, t_lo, t_hi, limit, u.keys);
-    const bool lost = __any(bad | pages.bad);
+    pages.load(p, u, lane, (u.tile0 * 32) >> p.page_shift);
+    uint32_t piece[2][2][PIECE / 4];                   // of tiles t and t + 1: K, V
+    float scale[2];
+    auto request = [&](int t, uint32_t (&w)[2][PIECE / 4], float& sc) {
+        const int key0 = min(t, t_hi - 1) * 32, most = u.keys - 1 - key0, mask = (1 << p.page_shift) - 1;
+        if (!pages.holds(p, key0 + 31)) pages.load(p, u, lane, key0 >> p.page_shift);
+        const int e0 = __builtin_amdgcn_readlane(pages.mine, (key0 >> p.page_shift) - pages.first);
+        const int e1 = most >= 16 ? __builtin_amdgcn_readlane(pages.mine, ((key0 + 16) >> p.page_shift) - pages.first) : e0;
+        const int key = min(my_row, most), e = key < 16 ? e0 : e1, token = (key0 + key) & mask;
+        const uint8_t* const k = k_base + e * p.ks.b + token * p.ks.n + from_column;
+        const uint8_t* const v = v_base + e * p.vs.b + token * p.vs.n + from_column;
+        if constexpr (PIECE == 16) {
+            const u32x4 a = *reinterpret_cast<const u32x4*>(k), b = *reinterpret_cast<const u32x4*>(v);
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-        const int r = row0 + 16 * b + n;
-        const float l = lost ? __builtin_nanf("") : w.over_groups_sum(w.l_run[b]);
-        if (r >= u.rows) continue;
+            for (int i = 0; i < 4; ++i) w[0][i] = a[i], w[1][i] = b[i];
+        } else {
+            const u32x2 a = *reinterpret_cast<const u32x2*>(k), b = *reinterpret_cast<const u32x2*>(v);
 #pragma unroll
-        for (int db = 0; db < D / 16; ++db)
-            if (16 * db + 4 * g < p.d) *reinterpret_cast<f32x4*>(out_o + (int64_t)r * p.d + 16 * db + 4 * g) = w.oacc[b][db];
-        if (g == 0) out_ml[r] = f32x2{w.m_run[b] * w.c_log2, l};
+            for (int i = 0; i < 2; ++i) w[0][i] = a[i], w[1][i] = b[i];
+        }
+        if (wave == 0) {
+            const int at = min(lane & 31, most), page = at < 16 ? e0 : e1;
+            sc = *reinterpret_cast<const float*>(reinterpret_cast<const char*>(s_base) + (int64_t)page * s_page +
+                                                 (int64_t)(((key0 + at) & mask) >> p.block_shift) * s_block);
+        }
+    };
+    auto stage_of = [&](int t) { return lds + (t - u.tile0) % 3 * STAGE; };
+    auto place = [&](int t, const uint32_t (&w)[2][PIECE / 4], float sc) {
+        uint16_t* const to = stage_of(t);
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int i = 0; i < PIECE / 8; ++i) {
+                const int granule = column / 8 + i;
+                *reinterpret_cast<bf16x8*>(to + x * TILE + my_row * B16::RS + ((granule ^ swz<D>(my_row)) << 3)) = codes_to_bf16<CODE>(w[x][2 * i], w[x][2 * i + 1]);
+            }
+        if (wave == 0) reinterpret_cast<float*>(to + 2 * TILE)[lane] = sc;
+    };
+    auto together = [&]() {                            // everyone has read and written what comes before
+        lds_reads_done();
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    request(u.tile0, piece[0], scale[0]);
+    request(u.tile0 + 1, piece[1], scale[1]);
+    const PagedRow me = paged_row(p, u, min(32 * wave + n, u.rows - 1));
+    PagedRows<D> w;
+    w.begin(p, lane, me, n < rows);
+    place(u.tile0, piece[0], scale[0]);
+    request(u.tile0 + 2, piece[0], scale[0]);
+    place(u.tile0 + 1, piece[1], scale[1]);
+    request(u.tile0 + 3, piece[1], scale[1]);
+    auto scores_of = [&](int t) {
+        const uint16_t* const tile = stage_of(t);
+        bf16x8 kf[DC];
+        w.read_k(kf, tile);
+        f32x16 s = w.scores(kf);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const f32x4 of = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(tile + 2 * TILE) + 8 * i + 4 * h);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[4 * i + r] *= of[r];
+        }
+        return s;
+    };
+    together();
+    f32x16 s = scores_of(u.tile0);
+    if (32 > u.keys - u.tile0 * 32) w.exclude(s, lane, u.keys - u.tile0 * 32);
+    w.fold(s);
+    auto step = [&](int t, uint32_t (&pc)[2][PIECE / 4], float& sc) {
+        if (t != u.tile0) together();
+        place(t + 2, pc, sc);
+        request(t + 4, pc, sc);
+        f32x16 next = scores_of(t + 1);                // (after the last tile: of the last one again, which nobody uses)
+        const uint16_t* const tile = stage_of(t);
+        // as PagedRows::weights, and V's scales
+        const float shift = (w.m_run == -INFINITY ? 0.f : w.m_run) * w.c_log2;
+        float sum[2] = {0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const f32x4 of = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(tile + 2 * TILE) + 32 + 8 * i + 4 * h);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float e = exp2_fast(fmaf(s[4 * i + r], w.c_log2, -shift));
+                sum[r & 1] += e;
+                s[4 * i + r] = e * of[r];
+            }
+        }
+        w.l_run += sum[0] + sum[1];
+        w.add16(tile + TILE, 0, pack8(s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7]));
+        w.add16(tile + TILE, 1, pack8(s[8], s[9], s[10], s[11], s[12], s[13], s[14], s[15]));
+        s = next;
+        if (t + 1 < t_hi) {
+            if ((t + 2) * 32 > u.keys) w.exclude(s, lane, u.keys - (t + 1) * 32);
+            w.fold(s);
+        }
+    };
+    for (int t = u.tile0; t < t_hi; t += 2) {
+        step(t, piece[0], scale[0]);
+        if (t + 1 < t_hi) step(t + 1, piece[1], scale[1]);
     }
+    w.l_run += xhalf(w.l_run);
+    if (__any(bad | pages.bad)) w.l_run = __builtin_nanf("");
+    if (n >= rows) return;
+    float* const out = out_o + (int64_t)(32 * wave + n) * p.d + 4 * h;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const f32x16& a = w.oacc[db];
+            if (32 * db + 8 * g + 4 * h < p.d) *reinterpret_cast<f32x4*>(out + 32 * db + 8 * g) = f32x4{a[4 * g], a[4 * g + 1], a[4 * g + 2], a[4 * g + 3]};
+        }
+    if (h == 0) out_ml[32 * wave + n] = f32x2{w.m_run * w.c_log2, w.l_run};
 }
 
 // Without a prefix: all tiles of all walks (sequence by sequence, key head by key head, one tile of rows after the other) are cut into ranges of the same
