@@ -150,9 +150,10 @@ static __global__ __launch_bounds__(256) void kv_store8_kernel(const KvStore8Par
         } else {
             lost |= !(s_old >= kLeastScale && s_old <= 3.4e38f);
             if (!lost && a > Q * s_old) {
-                int e;
-                const float m = __builtin_frexpf(a / (Q * s_old), &e);
-                grow = m > 0.5f ? e : e - 1;
+                // a <= Q s_old 2^k, by fractions and exponents: their quotient may lie outside of fp32 (2^221 for a block of zeros)
+                int e_new, e_old;
+                const float m_new = __builtin_frexpf(a, &e_new), m_old = __builtin_frexpf(Q * s_old, &e_old);
+                grow = e_new - e_old + (m_new > m_old);
             }
             s = __builtin_ldexpf(s_old, grow);
         }
