@@ -61,7 +61,7 @@ class Rotary:
             raise ValueError('scaling is None, "linear", "ntk", "yarn" or "bands"')
         self.frequencies = f                                    # radians per position
         turns = [round(Fraction(x) * _TURNS_PER_RADIAN * 2 ** 64) for x in f]
-        self._turns = torch.tensor([t - 2 ** 64 if t >= 2 ** 63 else t for t in turns], dtype=torch.int64)
+        self._turns = [t - 2 ** 64 if t >= 2 ** 63 else t for t in turns]
         self._on = {}
 
     def turns_on(self, device) -> torch.Tensor:
@@ -69,5 +69,6 @@ class Rotary:
         has behind it."""
         turns = self._on.get(device)
         if turns is None:
-            turns = self._on[device] = self._turns.to(device)
+            with torch.inference_mode(False):           # a recorded graph saves them, whatever mode the first call is made in
+                turns = self._on[device] = torch.tensor(self._turns, dtype=torch.int64, device=device)
         return turns
