@@ -21,6 +21,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/hip/EmptyTensor.h>
+#include <ATen/hip/impl/HIPCachingAllocatorMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>      // this torch names its HIP devices "cuda"
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
@@ -1379,6 +1380,9 @@ PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
             if (graph && c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None)
                 for (const Tensor* t : {&q, &k})
                     if (t->defined()) check_capture(*t, "rotary positions");
+            // The frequencies are a Rotary's own, made on the stream of its first call: their memory waits for this one, too, before it serves others.
+            c10::hip::HIPCachingAllocatorMasqueradingAsCUDA::recordStreamMasqueradingAsCUDA(c.turns.storage().data_ptr(),
+                                                                                           c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(q.device().index()));
             const Tensor qx = rotary_input(q), kx = k.defined() ? rotary_input(k) : Tensor();
             if (graph) {
                 const auto out = Rotary::apply(qx, Rotary::maybe(kx), c.turns, Rotary::maybe(c.positions), Rotary::maybe(c.cu), Rotary::maybe(c.start), c.interleaved,

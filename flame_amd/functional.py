@@ -74,7 +74,8 @@ def rotary(rope, q, k=None, positions=None, cu_seqlens=None, start=None):
     their bounds cu_seqlens (int32 [sequences + 1], as sdpa_packed takes them) and the position of each one's first row (start, int32
     [sequences]; omitted: 0).  Rows behind the last sequence come out as zeros.  A recorded graph holds these tensors, so
     they may not be refilled before its backward.  Its backward may be captured into a graph, with what sdpa_packed says of leaves; the first
-    call of a `rope` on a device uploads its frequencies and comes before a capture."""
+    call of a `rope` on a device uploads its frequencies and comes before a capture.  A captured graph reads them at each replay: the `rope` stays
+    as long as the graph."""
     if q.shape[-1] != rope.head_dim:
         raise ValueError(f"the head dim is {rope.head_dim}")
     return capi.rotary(q, k, rope.turns_on(q.device), rope.interleaved, rope.size, positions, cu_seqlens, start)
