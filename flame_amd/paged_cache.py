@@ -30,7 +30,7 @@ that its places may belong to others.  Inference only: `store` and `attend` are 
 from __future__ import annotations
 
 import heapq
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 
 import torch
 
@@ -43,11 +43,11 @@ class PagedBatch:
     page_table: torch.Tensor            # [B, pages] of the sequences' own keys
     kv_len: torch.Tensor                # [B] own keys, the new ones among them
     start: torch.Tensor                 # [B] place of the first new token among the own ones
-    past: torch.Tensor                  # [B] its position: all tokens before it, the prefix's too
     cu: torch.Tensor                    # [B + 1] bounds of the new tokens' rows
     prefix_table: torch.Tensor | None   # [pages] that all sequences share in front of their own
     prefix_len: torch.Tensor | None     # [1]
     counts: list[int]                   # new tokens per sequence
+    past: torch.Tensor | None = field(default=None, kw_only=True)      # [B] the first new token's position: all tokens before it, the prefix's too
 
 
 class PagedCache:
@@ -206,7 +206,7 @@ class PagedCache:
             at.append(at[-1] + n)
         up = torch.tensor(data + at, dtype=torch.int32).to(self.k.device)
         prefix, length, table, kv_len, start, past, cu = up.split([common, 1, B * width, B, B, B, B + 1])
-        return PagedBatch(table.view(B, width), kv_len, start, past, cu, prefix if common else None, length if common else None, counts)
+        return PagedBatch(table.view(B, width), kv_len, start, cu, prefix if common else None, length if common else None, counts, past=past)
 
     def store(self, layer, k, v, batch) -> None:
         """Rows k, v [new tokens of the batch, kv_heads, head_dim], sequence after sequence, to their places.  Inference only, as `attend`: rows
