@@ -48,6 +48,7 @@ class PagedBatch:
     prefix_len: torch.Tensor | None     # [1]
     counts: list[int]                   # new tokens per sequence
     past: torch.Tensor | None = field(default=None, kw_only=True)      # [B] the first new token's position: all tokens before it, the prefix's too
+    state: tuple | None = field(default=None, kw_only=True)            # the sequences, and which of their states it was made of
 
 
 class PagedCache:
@@ -78,14 +79,23 @@ class PagedCache:
         self._free = list(range(pages))         # a heap: the lowest page first
         self._pages: dict[int, list[int]] = {}
         self._len: dict[int, int] = {}
-        self._next = 0
+        self._state: dict[int, int] = {}        # another number after every change of the sequence's tokens or pages
+        self._next = self._changes = 0
 
     # ------------------------------------------------------------------------------------------------- sequences
     def new(self) -> int:
         """An empty sequence."""
         seq, self._next = self._next, self._next + 1
         self._pages[seq], self._len[seq] = [], 0
+        self._changed(seq)
         return seq
+
+    def _changed(self, seq) -> None:
+        self._changes += 1
+        self._state[seq] = self._changes
+
+    def _states(self, seqs) -> tuple:
+        return tuple((s, self._state[s]) for s in seqs)
 
     def fork(self, seq) -> int:
         """A sequence with the same tokens.  Its pages are shared; a partly filled last one is copied when either is extended."""
@@ -105,13 +115,15 @@ class PagedCache:
             self._pages[seq]                    # an unknown one: KeyError before anything changes
         for seq in seqs:
             self._drop(self._pages.pop(seq))
-            del self._len[seq]
+            del self._len[seq], self._state[seq]
 
     def cut(self, seq, length) -> None:
         """Forgets the tokens from `length` on (drafted ones that were refused).  In 8 bits the block that `length` lies in keeps the scale that they
         gave it."""
         if not 0 <= length <= self._len[seq]:
             raise ValueError("a sequence can be cut to at most its length")
+        if length < self._len[seq]:
+            self._changed(seq)
         keep = -(-length // self.page)
         self._drop(self._pages[seq][keep:])
         del self._pages[seq][keep:]
@@ -186,6 +198,9 @@ class PagedCache:
         for seq, n, pages in zip(seqs, counts, lists):
             self._pages[seq] = pages
             self._len[seq] += n
+            if n:
+                self._changed(seq)
+        batch.state = self._states(seqs)
         return batch
 
     def _batch(self, lists, lens, counts, share_prefix) -> PagedBatch:
@@ -227,7 +242,9 @@ class PagedCache:
         if not seqs or len(set(seqs)) < len(seqs):
             raise ValueError("different sequences")
         lens = [self._len[s] for s in seqs]
-        return self._batch([self._pages[s] for s in seqs], lens, lens, False)
+        batch = self._batch([self._pages[s] for s in seqs], lens, lens, False)
+        batch.state = self._states(seqs)
+        return batch
 
     def load(self, layer, held):
         """k, v: bf16 [tokens of `held`, kv_heads, head_dim], sequence after sequence."""
@@ -244,6 +261,8 @@ class PagedCache:
             raise ValueError("as many rows as the batch has new tokens")
         if len(held.counts) != len(batch.counts) or any(n > m for n, m in zip(batch.counts, held.counts)):
             raise ValueError("`held` is of other sequences than the batch")
+        if batch.state is not None and held.state != batch.state:           # (None: tables of the caller's own)
+            raise ValueError("`held` is of the batch's sequences, in its order, made after the batch and before anything else changes them")
         if torch.is_grad_enabled() and q.requires_grad:
             raise RuntimeError("attention to the cache has no backward and q requires a gradient: call it under torch.no_grad()")
         if not q.shape[0]:
@@ -271,6 +290,9 @@ class PagedCache:
             for p, q in to.items():
                 self._users[q], self._users[p] = self._users[p], 0
             for seq, pages in self._pages.items():
-                self._pages[seq] = [to.get(p, p) for p in pages]
+                moved = [to.get(p, p) for p in pages]
+                if moved != pages:
+                    self._pages[seq] = moved
+                    self._changed(seq)
             self._free = list(range(held, len(self._users)))
         return len(src)
