@@ -1345,11 +1345,14 @@ PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
             TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), "rotary positions have no forward-mode derivative: an input carries a tangent");
         if (q.dim() != 3 && q.dim() != 4) fail(PyExc_ValueError, "rotary positions expect [rows, heads, D] or [B, heads, S, D]");
         const bool rows = q.dim() == 3;
-        check_that(q.numel() > 0, "rotary positions need at least one element");
+        // a batch without new tokens: every check, no launch
+        const bool none = q.numel() == 0 && q.size(1) > 0 && q.size(-1) > 0 &&
+                          !(c.positions.defined() && c.positions.dim() > 0 && c.positions.size(-1) != q.size(rows ? 0 : 2));
+        check_that(q.numel() > 0 || none, "rotary positions need at least one element, or no rows and as few positions");
         check_that(q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf || q.scalar_type() == at::kFloat, "q and k are bf16, fp16 or fp32");
         check_device(q, q, "the tensors are on a GPU");
         if (k.defined()) {
-            check_that(k.dim() == q.dim() && k.numel() > 0 && k.scalar_type() == q.scalar_type(), "k has q's type and number of axes");
+            check_that(k.dim() == q.dim() && (k.numel() > 0 || (none && k.size(1) > 0)) && k.scalar_type() == q.scalar_type(), "k has q's type and number of axes");
             for (int64_t ax = 0; ax < q.dim(); ++ax) check_that(ax == 1 || k.size(ax) == q.size(ax), "k has q's shape, but for the heads");
             check_device(k, q, "all tensors are on one GPU");
         }
@@ -1361,7 +1364,7 @@ PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
             check_that(!c.start.defined(), "first positions are those of bounded sequences");
             const Tensor& p = c.positions;
             check_that(p.scalar_type() == at::kInt && (p.dim() == 1 || (p.dim() == 2 && !rows && p.size(0) == q.size(0))) && p.size(-1) == q.size(rows ? 0 : 2) &&
-                           (p.stride(-1) == 1 || p.size(-1) == 1),
+                           (p.stride(-1) == 1 || p.size(-1) <= 1),
                        "positions are int32, contiguous, one for every row, or [S] or [B, S]");
             check_device(p, q, "all tensors are on one GPU");
         } else {
@@ -1373,7 +1376,10 @@ PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
             if (t->defined())
                 for (int64_t s : t->sizes()) size32(s);
         Tensor yq, yk;
-        {
+        if (none) {
+            yq = q.clone();
+            if (k.defined()) yk = k.clone();
+        } else {
             WithoutGil nogil;
             c10::OptionalDeviceGuard device(q.device());
             const bool graph = at::GradMode::is_enabled() && (q.requires_grad() || (k.defined() && k.requires_grad()));

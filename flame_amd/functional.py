@@ -72,7 +72,7 @@ def rotary(rope, q, k=None, positions=None, cu_seqlens=None, start=None):
 
     Where the tokens are: positions, int32 on the device, one for every row, or [S] or [B, S]; or, for rows of packed sequences,
     their bounds cu_seqlens (int32 [sequences + 1], as sdpa_packed takes them) and the position of each one's first row (start, int32
-    [sequences]; omitted: 0).  Rows behind the last sequence come out as zeros.  A recorded graph holds these tensors, so
+    [sequences]; omitted: 0).  Rows behind the last sequence come out as zeros; without rows there is nothing to do.  A recorded graph holds these tensors, so
     they may not be refilled before its backward.  Its backward may be captured into a graph, with what sdpa_packed says of leaves; the first
     call of a `rope` on a device uploads its frequencies and comes before a capture.  A captured graph reads them at each replay: the `rope` stays
     as long as the graph."""
