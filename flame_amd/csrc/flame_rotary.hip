@@ -3,6 +3,7 @@
 #include <cmath>
 
 #include "rotary.hpp"
+#include "rotary_rule.hpp"
 #include "view_checks.hpp"
 #include "../../include/flame_attn.h"
 
@@ -15,12 +16,10 @@ int launch(RotaryParams p, hipStream_t s) {
     p.chunks = rotary_chunks<T, WIDE, NEAR>(p.D, p.R);
     const int heads = p.H[0] + p.H[1];
     const double all = (double)p.B * p.S * p.chunks;
-    // Several heads per thread share its sines and have their loads in flight together, from eight workgroups of one head a thread for every compute unit on.  (A head
-    // -> four heads a thread, us, 40 heads of D = 128, bf16, positions given: 64 rows 3.4 -> 5.0, 1024 7.5 -> 8.1, 1638 9.7 -> 9.0, 4096 17.9 -> 15.1, 12593 52 -> 56; by
-    // the bounds of sequences 12593 rows 56 -> 56, 13211 forward and backward 116 -> 112.)
-    const int per_thread = all * heads >= 256.0 * 8 * 256 ? 4 : 1;
+    const double most = (double)(UINT32_MAX - 256);    // threads of a launch
+    const int per_thread = all * heads > most ? 4 : rotary_heads_per_thread(all * heads, WIDE, NEAR, sizeof(typename T::Raw) == 4, p.cu != nullptr);
     p.groups = (heads + per_thread - 1) / per_thread;
-    if (all * p.groups > (double)(UINT32_MAX - 256)) return FLAME_ATTN_ERR_UNSUPPORTED;
+    if (all * p.groups > most) return FLAME_ATTN_ERR_UNSUPPORTED;
     p.items = (uint32_t)p.B * (uint32_t)p.S * (uint32_t)p.chunks * (uint32_t)p.groups;
     const unsigned grid = (p.items + 255u) / 256u;
     if (per_thread == 4) hipLaunchKernelGGL((rotary_kernel<T, WIDE, NEAR, 4>), dim3(grid), dim3(256), 0, s, p);
