@@ -48,8 +48,8 @@ struct PagedParams {
     int64_t own_slot;              // rows of the partial results that the prefix has (a host bound); the own ones follow
     float* part_o;                 // [row][d]
     f32x2* part_ml;                // m and l of every row
-    // [B] first unit and units per (head, row tile) of a sequence, then the splits of the prefix and 0; with ranges of tiles: [B] first tile and
-    // tiles per (head, row tile), then the tiles of a range and 1
+    // [B] first unit and units per (head, row tile) of a sequence, then the splits of the prefix; with ranges of tiles: [B] first tile and
+    // tiles per (head, row tile), then the tiles of a range
     int2* plan;
 };
 
@@ -663,11 +663,12 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? (D <= 64 ? 3 : 2) : 2) void page
     paged_unit_body<D, NW, true>(p, u, lds, bad, true, nullptr, nullptr);
 }
 
-int launch_paged_merge(const PagedParams& p, hipStream_t s);        // compiled in flame_paged.hip
+int launch_paged_merge(const PagedParams& p, bool ranges, hipStream_t s);        // compiled in flame_paged.hip
 
 // Joins the units of a row: SHARE wavefronts take a share of the units each (4: a workgroup per row, 1: a workgroup for four rows).  Bound by the
-// latency of plan, maxima and sums one behind the other, about 6 us with its launch.
-template <int SHARE>
+// latency of plan, maxima and sums one behind the other, about 6 us with its launch.  RANGES: the keys were cut into ranges of tiles.  (One kernel that
+// asks the plan -> one for each, us, bf16: one sequence of 2000 13.3 -> 13.0, of 8000 19.9 -> 19.4, 12 answers on a prefix of 4096 18.2 -> 17.8.)
+template <int SHARE, bool RANGES>
 __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams p) {
     __shared__ f32x2 quarter[4][64];
     const int lane = threadIdx.x & 63, wave = SHARE == 1 ? 0 : packed_uniform(threadIdx.x >> 6);
@@ -675,21 +676,23 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams p) {
     if (SHARE == 1 && at_row >= p.B * p.H * p.N) return;
     const int G = p.H / p.Hkv, rows = p.N * G, rt = PagedCut::row_tiles(rows), all = p.B * rows, slot_rows = min(32, rows);
     const int pair = packed_uniform(at_row / rows), r = at_row - pair * rows, b = packed_uniform(pair / p.Hkv), kv_head = pair - b * p.Hkv;
-    const int2 mine = p.plan[b], all_of = p.plan[p.B];
-    const bool ranges = packed_uniform(all_of.y) != 0;
-    const int share = ranges ? packed_uniform(all_of.x) : 1, tiles = packed_uniform(mine.y);
-    // ranges: the walk's first tile, the range that it begins in
-    const int at_tile = packed_uniform(mine.x) + (kv_head * rt + r / 32) * tiles, range = at_tile / share;
-    const int own = !ranges ? tiles : tiles == 0 ? 0 : (at_tile + tiles - 1) / share - range + 1;
-    const int prefix = ranges ? 0 : packed_uniform(all_of.x), parts = own + prefix;
+    const int2 mine = p.plan[b];
+    const int first = packed_uniform(mine.x), each = packed_uniform(mine.y), all_of = packed_uniform(p.plan[p.B].x);
+    int own = each, prefix = RANGES ? 0 : all_of, range = 0;
+    if constexpr (RANGES) {
+        const int at_tile = first + (kv_head * rt + r / 32) * each;
+        range = at_tile / all_of;                          // that the walk begins in
+        own = each == 0 ? 0 : (at_tile + each - 1) / all_of - range + 1;
+    }
+    const int parts = own + prefix;
     if (own == 1 && prefix == 0) return;                   // written by the unit itself
     // rows of the partial results: unit s of the prefix, unit s of the own keys
     const int64_t prefix_pad = (int64_t)PagedCut::prefix_row_tiles(all) * PagedCut::prefix_tile_rows(all);
     const int64_t prefix_at = kv_head * prefix_pad + b * rows + r, prefix_step = p.Hkv * prefix_pad;
-    const int64_t own_at = p.own_slot + (int64_t)(packed_uniform(mine.x) + (kv_head * rt + r / 32) * own) * slot_rows + r % 32;
+    const int64_t own_at = p.own_slot + (int64_t)(first + (kv_head * rt + r / 32) * own) * slot_rows + r % 32;
     auto slot_of = [&](int s) {
         // a range has two places, for a walk that it ends or goes on with and for one that it begins
-        if (ranges) return p.own_slot + (int64_t)(s == 0 ? 2 * range + 1 : 2 * (range + s)) * slot_rows + r % 32;
+        if (RANGES) return p.own_slot + (int64_t)(s == 0 ? 2 * range + 1 : 2 * (range + s)) * slot_rows + r % 32;
         return s < prefix ? prefix_at + s * prefix_step : own_at + (int64_t)(s - prefix) * slot_rows;
     };
     float M = -INFINITY, L = 0.f, a0 = 0.f, a1 = 0.f;

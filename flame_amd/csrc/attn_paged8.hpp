@@ -559,7 +559,7 @@ __global__ __launch_bounds__(256, kPaged8Groups<D>) void paged_ranges_kernel(con
         }
         if (range == 0) p.plan[b] = int2{first, tiles};
     });
-    if (range == 0 && threadIdx.x == 0) p.plan[p.B] = int2{share, 1};
+    if (range == 0 && threadIdx.x == 0) p.plan[p.B] = int2{share, 0};
     if (at >= end) return;
     __syncthreads();
     int b = packed_uniform(found[0]), tiles = packed_uniform(found[2]), len = packed_uniform(found[3]);

@@ -7,11 +7,12 @@
 
 using namespace fattn;
 
-__attribute__((visibility("hidden"))) int fattn::launch_paged_merge(const PagedParams& p, hipStream_t s) {
+__attribute__((visibility("hidden"))) int fattn::launch_paged_merge(const PagedParams& p, bool ranges, hipStream_t s) {
     // (a workgroup for four rows -> per row, us: 32 rows of 500 units 101 -> 92, 256 rows 21.1 -> 20.4, 992 46.9 -> 47.5, 2048 101.6 -> 104.4)
     const int all = p.B * p.H * p.N;                   // rows
-    if (all >= 1024) hipLaunchKernelGGL(paged_merge_kernel<1>, dim3((unsigned)((all + 3) / 4)), dim3(256), 0, s, p);
-    else hipLaunchKernelGGL(paged_merge_kernel<4>, dim3((unsigned)all), dim3(256), 0, s, p);
+    const bool four = all >= 1024;
+    const auto kern = ranges ? (four ? paged_merge_kernel<1, true> : paged_merge_kernel<4, true>) : four ? paged_merge_kernel<1, false> : paged_merge_kernel<4, false>;
+    hipLaunchKernelGGL(kern, dim3((unsigned)(four ? (all + 3) / 4 : all)), dim3(256), 0, s, p);
     return (int)hipGetLastError();
 }
 

@@ -44,7 +44,7 @@ int attend(const Paged8Params<CODE, R>& p, const PagedSizes& z, hipStream_t s) {
     const int64_t room = 256 * kPaged8Groups<D>;       // workgroups that the card holds
     hipLaunchKernelGGL(kern, dim3((unsigned)std::max<int64_t>(1, std::min(room, z.own_units / 2))), dim3(256), lds, s, p);
     if (const hipError_t e = hipGetLastError()) return (int)e;
-    return launch_paged_merge(p, s);
+    return launch_paged_merge(p, true, s);
 }
 template <int CODE, int R>
 int attend(const Paged8Params<CODE, R>& p, const PagedSizes& z, hipStream_t s) {

@@ -89,7 +89,7 @@ int launch_paged(const P& p, const PagedSizes& z, hipStream_t s) {
     const int64_t room = D <= 64 ? 768 : 512;          // workgroups that the card holds (D = 64, 64 sequences of 4000: 512 of them 105.4 us, 768 102.8)
     hipLaunchKernelGGL(kern, dim3((unsigned)std::min(room, z.prefix_units + z.own_units)), dim3(256), lds, s, p);
     if (const hipError_t e = hipGetLastError()) return (int)e;
-    return launch_paged_merge(p, s);
+    return launch_paged_merge(p, false, s);
 }
 
 }  // namespace fattn
