@@ -379,11 +379,11 @@ struct PagedRows {
 };
 
 // The end of a unit whose wavefronts have walked keys of their own: their states become one, which is the result (direct) or goes to the
-// merge.  `lds`: WAVE_FLOATS floats per wavefront, at least 32 D, into which no copy is under way; `bad`: the rows are NaN.
-template <int D, int NW, int WAVE_FLOATS>
+// merge.  `lds`: the tiles of the wavefronts, into which no copy is under way; `bad`: the rows are NaN.
+template <int D, int NW>
 __device__ __forceinline__ void paged_unit_join(const PagedParams& p, const PagedUnit& u, PagedRows<D>& w, float* lds, int tid, bool bad, bool direct,
                                                 float* out_o, f32x2* out_ml) {
-    constexpr int DB = D / 32;
+    constexpr int DB = D / 32, WAVE_FLOATS = PagedTile<D>::WAVE_ELEMS / 2;
     const int lane = tid & 63, wave = packed_uniform(tid >> 6), n = lane & 31, h = lane >> 5;
     w.l_run += xhalf(w.l_run);
     if (__any(bad)) w.l_run = __builtin_nanf("");    // a page outside the cache, or more keys than pages: NaN
@@ -487,7 +487,7 @@ __device__ __forceinline__ void paged_unit_body(const PagedParams& p, const Page
         w.add(vf, pf);
     }
 
-    paged_unit_join<D, NW, T::WAVE_ELEMS / 2>(p, u, w, reinterpret_cast<float*>(lds), tid, bad | (pages.bad && t_lo < t_hi), direct, out_o, out_ml);
+    paged_unit_join<D, NW>(p, u, w, reinterpret_cast<float*>(lds), tid, bad | (pages.bad && t_lo < t_hi), direct, out_o, out_ml);
 }
 
 // A unit of the prefix with 128 rows: the wavefronts have 32 each and share the tiles, a quarter of each copied by every wavefront.
