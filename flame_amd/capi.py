@@ -212,8 +212,8 @@ def kv_store(k, v, k_cache, v_cache, page_table, cu, start, k_scale=None, v_scal
 
     Caches in 8 bits: int8 or float8_e4m3fn, D a multiple of 16 up to 128, k_scale and v_scale fp32 [pages, H_kv, page / block], `block` tokens
     (a power of two up to 128) sharing one.  A block begun by this call gets the scale its largest magnitude needs; one that
-    holds older tokens keeps its scale or doubles it until the new rows fit, and the older codes follow.  Infinities and NaN make
-    a block's scale NaN.  Autograd records nothing: inputs that require a gradient
+    holds older tokens keeps its scale or doubles it until the new rows fit, and the older codes follow; what it holds behind the new rows
+    is given up.  Infinities and NaN make a block's scale NaN.  Autograd records nothing: inputs that require a gradient
     are refused while it is enabled, and a graph that saved a view of the caches raises in its backward."""
     host().kv_store(k, v, k_cache, v_cache, page_table, cu, start, k_scale, v_scale)
 

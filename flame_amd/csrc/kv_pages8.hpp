@@ -6,8 +6,10 @@
 //   a not finite, or s none that a store has left:  NaN, which every answer that attends to the block then is
 // and a number x becomes x / s, rounded to the nearest code, the even one of two.
 // Growing by powers of two, a block's codes are off by less than one of its last steps however often it grew: 1/2 + 1/4 + ...; by the ratio that
-// a needs they would drift by half a step each time.  Four bits of s cost int8 a sixteenth of its resolution at most, on average a thirty-second, and give this: x has
-// eight significant bits, so x / s either is a border between two codes or is 2^-15 away from it, and fp32 arithmetic finds the same codes as exact arithmetic.
+// a needs they would drift by half a step each time.  What a block holds behind the new rows counts as not stored: its codes stay and its scale does not.
+// Four bits of s make the steps of int8 up to an eighth wider than a / Q would (4 % on average over the fractions of a), and give this: x has
+// eight significant bits, so x / s either is a border between two codes or is 2^-15 away from it, and fp32 arithmetic finds the same codes as exact
+// arithmetic.
 #pragma once
 #include "kv_codes.hpp"
 #include "packed_units.hpp"

@@ -7,7 +7,7 @@
 // either way, also exactly, and only then become fp32: sine and cosine are sums of their power series there, off by less than 2e-7.
 //
 // Bound by memory: every element is read and written once.  A thread serves a chunk of pairs (16 bytes of a head, halves: twice 16) for up to
-// HPT heads, which share the sines: 30 operations a pair, as much as three heads' loads and stores.  Queries and keys go in one launch.
+// HPT heads (rotary_rule.hpp), which share the sines: 30 operations a pair, as much as three heads' loads and stores.  Queries and keys go in one launch.
 #pragma once
 #include "attn_common.hpp"
 #include "packed_units.hpp"

@@ -11,9 +11,10 @@
 //   narrow, D = 72, bf16, positions 6.8 -> 6.7    11.1 -> 9.9   18.5 -> 15.3  35.2 -> 28.2  68.9 -> 56.6  106 -> 86     262 -> 206    518 -> 405
 //   halves, fp32, positions         6.2 -> 7.1    9.3 -> 9.2    19.2 -> 21.0  33.3 -> 38.2  61.8 -> 68.5  96 -> 104     238 -> 253    481 -> 503
 //                 bounds            6.8 -> 7.7    10.2 -> 10.1  20.1 -> 21.8  34.7 -> 38.7  65.4 -> 67.8  101 -> 103    246 -> 247    486 -> 494
-//   halves, bf16: positions, 512 rows 5.0 -> 6.6, 1024 7.3 -> 7.9, 1638 9.5 -> 8.9, 2500 13.8 -> 14.2, 4096 20.2 -> 20.9, 8192 35.8 -> 38.1, 12593 52.3 -> 56.7, 32768 130 -> 131,
-//   131072 511 -> 494;  bounds, 512 5.5 -> 7.0, 1024 7.4 -> 8.3, 1638 9.5 -> 9.5, 2500 15.3 -> 15.1, 4096 22.0 -> 21.6, 8192 38.6 -> 38.3, 12593 56.4 -> 56.0, 32768 141 -> 129, 131072
-//   552 -> 479.  (D = 64, 24 heads on 24, bounds: 4096 14.9 -> 14.2, 8192 26.0 -> 29.4, 13000 37.7 -> 38.4, 32768 88 -> 83, 65536 172 -> 156.)
+//   halves, bf16: positions, 512 rows 5.0 -> 6.6, 1024 7.3 -> 7.9, 1638 9.5 -> 8.9, 2500 13.8 -> 14.2, 4096 20.2 -> 20.9, 8192 35.8 -> 38.1,
+//   12593 52.3 -> 56.7, 32768 130 -> 131, 131072 511 -> 494; bounds, 512 5.5 -> 7.0, 1024 7.4 -> 8.3, 1638 9.5 -> 9.5, 2500 15.3 -> 15.1,
+//   4096 22.0 -> 21.6, 8192 38.6 -> 38.3, 12593 56.4 -> 56.0, 32768 141 -> 129, 131072 552 -> 479.  (D = 64, 24 heads on 24, bounds: 4096
+//   14.9 -> 14.2, 8192 26.0 -> 29.4, 13000 37.7 -> 38.4, 32768 88 -> 83, 65536 172 -> 156.)
 #pragma once
 
 namespace fattn {

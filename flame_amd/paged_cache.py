@@ -15,7 +15,7 @@
 
 Pieces of prompts, different numbers of new tokens against what the sequences hold already:
 
-    batch, held = cache.extend(seqs, counts), cache.held(seqs)
+    batch, held = cache.extend(seqs, counts), cache.held(seqs)     # (held: of what the batch made of them)
     q, k = functional.rotary(rope, q, k, cu_seqlens=batch.cu, start=batch.past)
     for layer in ...:
         cache.store(layer, k, v, batch)
@@ -255,7 +255,8 @@ class PagedCache:
 
     def attend_rows(self, layer, q, batch, held, scale=None):
         """Attention of the batch's new tokens, q [rows, H, head_dim], any number of them of a sequence (stored before), to all that their
-        sequences hold: the cache is read back into packed rows and functional.sdpa_packed attends to those.  `held`: self.held of the
+        sequences hold: the cache is read back into packed rows and functional.sdpa_packed attends to those.  In 8 bits the products of codes and
+        scales are rounded to bf16 on the way, which `attend` does not.  `held`: self.held of the
         batch's sequences, in its order, made after the batch.  Inference only, as `attend`."""
         if q.shape[0] != sum(batch.counts):
             raise ValueError("as many rows as the batch has new tokens")

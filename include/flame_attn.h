@@ -329,8 +329,10 @@ int flame_kv_copy_pages_bf16(void* K_cache, void* V_cache, int layers, int n_pag
  *   - The store decides a block's scale from the largest magnitude a of the rows it brings to it (Q: the largest code).  From the block's first
  *     token on: a / Q, rounded up to four significant bits, at least 2^-100.  Behind older tokens: the scale that is there times the least power
  *     of two, 1 or more, with which a fits, and the older codes are divided by that power and rounded.  A number x becomes x / scale rounded
- *     to the nearest code, the even one of two.  Infinities and NaN, and a block whose beginning was not stored by such a call, make the scale
- *     NaN, and with it every answer that attends to the block, until its first token is stored again.
+ *     to the nearest code, the even one of two.  Tokens that the block holds behind the new rows are given up: their codes stay, their scale
+ *     may not, so a store in the middle of a sequence is followed by stores of all that is behind it in the block.  Infinities and NaN, and a
+ *     block whose beginning was not stored by such a call, make the scale NaN, and with it every answer that attends to the block, until its
+ *     first token is stored again.
  *   - Everything else, page tables, lengths, the rules of the workspace, is as above.
  * ---------------------------------------------------------------------------------------------- */
 size_t flame_attn_paged_q8_workspace_bytes(int B, int H, int H_kv, int N, int D, int page, int table_pages, int prefix_pages);
