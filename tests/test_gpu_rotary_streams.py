@@ -34,6 +34,7 @@ def test_goes_away_while_another_stream_is_late(graph):
     held = [torch.empty(size, dtype=torch.int64, device="cuda") for _ in range(50)]
     for t in held:
         t.copy_(zeros)                             # on the stream that the frequencies were made on
-    assert all(t.data_ptr() != address for t in held)
+    if not side.query():                           # still not
+        assert all(t.data_ptr() != address for t in held)
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
